@@ -14,12 +14,14 @@ library carries its own runtime.
 """
 import argparse
 import os
+import re
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_ROOT = os.path.dirname(os.path.abspath(__file__))
 REPO_ROOT = os.path.dirname(PKG_ROOT)
-SRC = os.path.join(PKG_ROOT, "csrc", "lncc_sm100.cu")
+CSRC = os.path.join(PKG_ROOT, "csrc")
 INCLUDE = os.path.join(REPO_ROOT, "include")
 LIB_DIR = os.path.join(PKG_ROOT, "fused_lncc")
 LIB_NAME = "liblncc_sm100.so"
@@ -34,9 +36,25 @@ def nvcc_path():
     return cand if os.path.exists(cand) else "nvcc"
 
 
-def sources():
-    csrc = os.path.join(PKG_ROOT, "csrc")
-    return sorted(os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith((".cu", ".cuh", ".h")))
+OBJ_DIR = os.path.join(PKG_ROOT, "_build")
+
+
+def sources(suffixes=(".cu", ".cuh", ".h")):
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(suffixes))
+
+
+def _includes(path, seen=None):
+    """The files of csrc/ and include/ that a source includes, itself among them."""
+    seen = set() if seen is None else seen
+    seen.add(path)
+    with open(path) as f:
+        names = re.findall(r'^\s*#include "([^"]+)"', f.read(), re.M)
+    for name in names:
+        for d in (CSRC, INCLUDE):
+            dep = os.path.join(d, name)
+            if os.path.exists(dep) and dep not in seen:
+                _includes(dep, seen)
+    return seen
 
 
 def _stale(out):
@@ -47,20 +65,36 @@ def _stale(out):
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build_library(force=False, checked=False, verbose=False, out=None):
-    """Compile the library if it is missing or older than its sources; return its path."""
-    out = out or (CHECKED_LIB_PATH if checked else LIB_PATH)
-    if not force and not _stale(out):
-        return out
-    cmd = [nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-I", INCLUDE,
-           "-Xcompiler", "-fPIC", "-shared", "-o", out + ".tmp", SRC]
-    if checked:
-        cmd.insert(1, "-DLNCC_CHECKED=1")
+def _run(cmd, out, verbose):
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"nvcc failed building {out}:\n{r.stdout}\n{r.stderr}")
+
+
+def build_library(force=False, checked=False, verbose=False, out=None):
+    """Compile the library if it is missing or older than its sources; return its path. Each .cu file is an object of
+    its own under _build/, compiled side by side and again only where it or what it includes is newer."""
+    out = out or (CHECKED_LIB_PATH if checked else LIB_PATH)
+    if not force and not _stale(out):
+        return out
+    objects = os.path.join(OBJ_DIR, "checked" if checked else "product")
+    os.makedirs(objects, exist_ok=True)
+
+    def compile_one(src):
+        obj = os.path.join(objects, os.path.basename(src)[:-3] + ".o")
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) >= max(map(os.path.getmtime, _includes(src))):
+            return obj
+        cmd = [nvcc_path(), *ARCH_FLAGS, "-lineinfo", "-O3", "-std=c++17", "-I", INCLUDE, "-Xcompiler", "-fPIC",
+               *(["-DLNCC_CHECKED=1"] if checked else []), "-c", "-o", f"{obj}.{os.getpid()}.tmp", src]
+        _run(cmd, obj, verbose)
+        os.replace(f"{obj}.{os.getpid()}.tmp", obj)
+        return obj
+
+    with ThreadPoolExecutor() as pool:
+        built = list(pool.map(compile_one, sources((".cu",))))
+    _run([nvcc_path(), *ARCH_FLAGS, "-Xcompiler", "-fPIC", "-shared", "-o", out + ".tmp", *built], out, verbose)
     os.replace(out + ".tmp", out)
     return out
 

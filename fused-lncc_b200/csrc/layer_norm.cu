@@ -1,0 +1,430 @@
+// Layer norm over the last axis, forward and backward, with the gradients of the weight and the bias.
+//
+//   mu = mean(x), v = mean((x - mu)^2), r = 1/sqrt(v + eps), n = (x - mu) r, y = n w + b
+//   g = dy w, dx = r (g - mean(g) - n mean(g n)), dw = sum over rows of dy n, db = sum over rows of dy
+//
+// A row lives in the registers of LANES threads, 16 elements each, from its one load to its one store: the mean and
+// then the centred squares are summed in fp32 without a second read (the two-step variance does not cancel). LANES is
+// the smallest power of two whose registers hold the row, so a warp takes 8 rows of 64 or one of 512, and a block one of
+// up to 16384. Both directions are bound by their bytes; thread blocks stay and walk over the rows, so that the weight
+// is loaded once and, backward, each thread keeps the fp32 sums of dw and db of its own columns. The next row's loads
+// are issued before the present row is reduced. The sums of the threads of a block meet in shared memory and those of the
+// blocks in a second kernel, each in a fixed order: the gradients are the same bits run after run.
+// Rows wider than 16384 take the looping kernels at the end of this file, which read a row again for each step.
+#include "lncc_block.cuh"
+
+namespace lncc {
+namespace norm {
+
+using namespace blk;
+
+constexpr int kElems = 16;       // elements of a row that one thread holds
+constexpr int kThreads = 256;    // threads of a block (LANES where that is more)
+constexpr int kMaxWidth = 16384; // widest row that 1024 threads hold
+
+struct Args {
+  const void* x;
+  int64_t x_stride;   // elements from row to row
+  const void* dy;     // backward
+  int64_t dy_stride;
+  const void* w;      // null: ones
+  const void* b;      // null: zeros
+  int wdtype;
+  int64_t rows;
+  int width;
+  float eps;
+  void* y;            // forward: y, backward: dx (may be null)
+  float* mean;        // per row, written forward (may be null), read backward
+  float* rstd;
+  float* partial;     // backward: [blocks][2][width] sums of dy n and of dy (null: not wanted)
+};
+
+__device__ __forceinline__ float load_param(const void* p, int dtype, int c) {
+  if (dtype == LNCC_F32) return static_cast<const float*>(p)[c];
+  if (dtype == LNCC_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[c]);
+  return to_f(static_cast<const __half*>(p)[c]);
+}
+
+// Sum over the LANES threads of a row; every one of them gets it. `red` holds one float a warp and is not used again
+// before another barrier has been passed.
+template <int LANES> __device__ __forceinline__ float row_sum(float v, float* red) {
+#pragma unroll
+  for (int o = (LANES < 32 ? LANES : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (LANES > 32) {
+    constexpr int WARPS = LANES / 32 > 0 ? LANES / 32 : 1;
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0) red[warp] = v;
+    __syncthreads();
+    const float* mine = red + warp / WARPS * WARPS;
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; i++) v += mine[i];
+  }
+  return v;
+}
+
+// One thread's share of a row, as it lies in memory: NV vectors of VEC elements, vector v at column (v*LANES + lane)*VEC.
+template <typename T, int LANES, int VEC> struct Share {
+  static constexpr int NV = kElems / VEC;
+  Vec<T, VEC> raw[NV];
+  __device__ __forceinline__ void load(const T* row, int lane, int width, bool live) {
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      const int c = (v * LANES + lane) * VEC;
+      if (live && c < width && LNCC_IN(c, VEC, width)) {
+        raw[v] = *reinterpret_cast<const Vec<T, VEC>*>(row + c);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) raw[v].e[i] = from_f<T>(0.f);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int v, int i) const { return to_f(raw[v].e[i]); }
+};
+
+template <typename T, int LANES, int VEC>
+__global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) forward_kernel(const Args a) {
+  constexpr int THREADS = LANES > kThreads ? LANES : kThreads;
+  constexpr int ROWS = THREADS / LANES, NV = kElems / VEC;
+  __shared__ float red[2][THREADS / 32];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.y);
+  float w[kElems], b[kElems];
+#pragma unroll
+  for (int e = 0; e < kElems; e++) {
+    const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
+    w[e] = a.w && c < a.width ? load_param(a.w, a.wdtype, c) : 1.f;
+    b[e] = a.b && c < a.width ? load_param(a.b, a.wdtype, c) : 0.f;
+  }
+  const float inv = 1.f / float(a.width);
+  const int64_t step = int64_t(gridDim.x) * ROWS;
+  int64_t row = int64_t(blockIdx.x) * ROWS + group;
+  Share<T, LANES, VEC> next;
+  next.load(x + row * a.x_stride, lane, a.width, row < a.rows);
+  // every group of the block takes the same number of turns: the row sums hold barriers
+  for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += step, row += step) {
+    const Share<T, LANES, VEC> cur = next;
+    next.load(x + (row + step) * a.x_stride, lane, a.width, row + step < a.rows);
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < kElems; e++) s += cur.get(e / VEC, e % VEC);
+    const float mu = row_sum<LANES>(s, red[0]) * inv;
+    float q = 0.f;
+#pragma unroll
+    for (int e = 0; e < kElems; e++) {
+      const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
+      const float d = cur.get(e / VEC, e % VEC) - mu;
+      if (c < a.width) q += d * d;
+    }
+    const float rs = rsqrtf(row_sum<LANES>(q, red[1]) * inv + a.eps);
+    if (row >= a.rows) continue;
+    if (lane == 0 && a.mean && LNCC_IN(row, 1, a.rows)) {
+      a.mean[row] = mu;
+      a.rstd[row] = rs;
+    }
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      const int c = (v * LANES + lane) * VEC;
+      float o[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; i++) o[i] = (cur.get(v, i) - mu) * rs * w[v * VEC + i] + b[v * VEC + i];
+      if (c < a.width && LNCC_IN(row * a.width + c, VEC, a.rows * a.width)) store_vec<T, VEC>(y + row * a.width + c, o);
+    }
+  }
+}
+
+template <typename T, int LANES, int VEC>
+__global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) backward_kernel(const Args a) {
+  constexpr int THREADS = LANES > kThreads ? LANES : kThreads;
+  constexpr int ROWS = THREADS / LANES, NV = kElems / VEC;
+  __shared__ float red[2][THREADS / 32];
+  const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  T* dx = static_cast<T*>(a.y);
+  float w[kElems], dw[kElems], db[kElems];
+#pragma unroll
+  for (int e = 0; e < kElems; e++) {
+    const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
+    w[e] = a.w && c < a.width ? load_param(a.w, a.wdtype, c) : 1.f;
+    dw[e] = db[e] = 0.f;
+  }
+  const float inv = 1.f / float(a.width);
+  const int64_t step = int64_t(gridDim.x) * ROWS;
+  int64_t row = int64_t(blockIdx.x) * ROWS + group;
+  Share<T, LANES, VEC> next_x, next_dy;
+  next_x.load(x + row * a.x_stride, lane, a.width, row < a.rows);
+  next_dy.load(dy + row * a.dy_stride, lane, a.width, row < a.rows);
+  for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += step, row += step) {
+    const Share<T, LANES, VEC> cx = next_x, cd = next_dy;
+    const bool live = row < a.rows, more = row + step < a.rows;
+    next_x.load(x + (row + step) * a.x_stride, lane, a.width, more);
+    next_dy.load(dy + (row + step) * a.dy_stride, lane, a.width, more);
+    const float mu = live ? a.mean[row] : 0.f, rs = live ? a.rstd[row] : 0.f;
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < kElems; e++) {  // past the row's end dy is 0, and with it every term
+      const float d = cd.get(e / VEC, e % VEC), n = (cx.get(e / VEC, e % VEC) - mu) * rs;
+      db[e] += d;
+      dw[e] += d * n;
+      s1 += d * w[e];
+      s2 += d * w[e] * n;
+    }
+    if (a.y == nullptr) continue;  // the same for every thread
+    const float m1 = row_sum<LANES>(s1, red[0]) * inv, m2 = row_sum<LANES>(s2, red[1]) * inv;
+    if (!live) continue;
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      const int c = (v * LANES + lane) * VEC;
+      float o[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; i++) {
+        const float n = (cx.get(v, i) - mu) * rs;
+        o[i] = rs * (cd.get(v, i) * w[v * VEC + i] - m1 - n * m2);
+      }
+      if (c < a.width && LNCC_IN(row * a.width + c, VEC, a.rows * a.width)) store_vec<T, VEC>(dx + row * a.width + c, o);
+    }
+  }
+  if (a.partial == nullptr) return;
+  // the block's rows meet: thread t < LANES adds the other groups' sums to its own, group by group
+  float* out = a.partial + int64_t(blockIdx.x) * 2 * a.width;
+  __shared__ float meet[ROWS > 1 ? THREADS : 1];
+#pragma unroll
+  for (int e = 0; e < kElems; e++) {
+    const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+      float v = which ? db[e] : dw[e];
+      if (ROWS > 1) {
+        __syncthreads();
+        meet[threadIdx.x] = v;
+        __syncthreads();
+        if (group == 0) {
+          v = 0.f;
+          for (int g = 0; g < ROWS; g++) v += meet[g * LANES + lane];
+        }
+      }
+      if (group == 0 && c < a.width) out[which * a.width + c] = v;
+    }
+  }
+}
+
+// dw and db: column sums of the blocks' partial sums, eight strands of blocks in order and then the strands in order.
+__global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ partial, int blocks, int width, void* dw,
+                                                     void* db, int wdtype) {
+  __shared__ float sum[8][33];
+  const int strand = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t c = int64_t(blockIdx.x) * 32 + lane, cols = 2 * int64_t(width);
+  float s = 0.f;
+  if (c < cols)
+    for (int p = strand; p < blocks; p += 8) s += partial[p * cols + c];
+  sum[strand][lane] = s;
+  __syncthreads();
+  if (strand != 0 || c >= cols) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; i++) s += sum[i][lane];
+  void* to = c < width ? dw : db;
+  const int64_t i = c < width ? c : c - width;
+  if (to == nullptr || !LNCC_IN(i, 1, width)) return;
+  if (wdtype == LNCC_F32) static_cast<float*>(to)[i] = s;
+  else if (wdtype == LNCC_BF16) static_cast<__nv_bfloat16*>(to)[i] = from_f<__nv_bfloat16>(s);
+  else static_cast<__half*>(to)[i] = from_f<__half>(s);
+}
+
+// Rows that no block's registers hold: a block of 1024 takes one row and reads it once for each step.
+template <typename T> __global__ void __launch_bounds__(1024) wide_forward_kernel(const Args a) {
+  __shared__ float red[2][32];
+  const float inv = 1.f / float(a.width);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    T* y = static_cast<T*>(a.y) + row * a.width;
+    float s = 0.f, q = 0.f;
+    for (int c = threadIdx.x; c < a.width; c += 1024) s += to_f(x[c]);
+    const float mu = row_sum<1024>(s, red[0]) * inv;
+    for (int c = threadIdx.x; c < a.width; c += 1024) q += (to_f(x[c]) - mu) * (to_f(x[c]) - mu);
+    const float rs = rsqrtf(row_sum<1024>(q, red[1]) * inv + a.eps);
+    if (threadIdx.x == 0 && a.mean) {
+      a.mean[row] = mu;
+      a.rstd[row] = rs;
+    }
+    for (int c = threadIdx.x; c < a.width; c += 1024) {
+      const float w = a.w ? load_param(a.w, a.wdtype, c) : 1.f, b = a.b ? load_param(a.b, a.wdtype, c) : 0.f;
+      if (LNCC_IN(row * a.width + c, 1, a.rows * a.width)) y[c] = from_f<T>((to_f(x[c]) - mu) * rs * w + b);
+    }
+  }
+}
+template <typename T> __global__ void __launch_bounds__(1024) wide_dx_kernel(const Args a) {
+  __shared__ float red[2][32];
+  const float inv = 1.f / float(a.width);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+    const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
+    T* dx = static_cast<T*>(a.y) + row * a.width;
+    const float mu = a.mean[row], rs = a.rstd[row];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < a.width; c += 1024) {
+      const float g = to_f(dy[c]) * (a.w ? load_param(a.w, a.wdtype, c) : 1.f);
+      s1 += g;
+      s2 += g * (to_f(x[c]) - mu) * rs;
+    }
+    const float m1 = row_sum<1024>(s1, red[0]) * inv, m2 = row_sum<1024>(s2, red[1]) * inv;
+    for (int c = threadIdx.x; c < a.width; c += 1024) {
+      const float g = to_f(dy[c]) * (a.w ? load_param(a.w, a.wdtype, c) : 1.f), n = (to_f(x[c]) - mu) * rs;
+      if (LNCC_IN(row * a.width + c, 1, a.rows * a.width)) dx[c] = from_f<T>(rs * (g - m1 - n * m2));
+    }
+  }
+}
+// Column sums over the rows of strand blockIdx.y, one thread a column.
+template <typename T> __global__ void __launch_bounds__(kThreads) wide_columns_kernel(const Args a) {
+  const int64_t c = int64_t(blockIdx.x) * kThreads + threadIdx.x;
+  if (c >= a.width) return;
+  float dw = 0.f, db = 0.f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const float d = to_f(static_cast<const T*>(a.dy)[row * a.dy_stride + c]);
+    dw += d * (to_f(static_cast<const T*>(a.x)[row * a.x_stride + c]) - a.mean[row]) * a.rstd[row];
+    db += d;
+  }
+  float* out = a.partial + int64_t(blockIdx.y) * 2 * a.width;
+  out[c] = dw;
+  out[a.width + c] = db;
+}
+
+static int lanes_for(int64_t width) {
+  int lanes = 4;
+  while (int64_t(lanes) * kElems < width) lanes *= 2;
+  return lanes;
+}
+
+// Thread blocks of a call: enough rows for each to pay for its weights, at most what the GPU holds at once.
+// The backward kernel holds about 110 registers a thread, so two blocks of 256 fit on an SM.
+static int blocks_for(int64_t rows, int64_t width, bool backward) {
+  const int sms = sm_count();
+  if (width > kMaxWidth) return int(rows < sms * 2 ? rows : sms * 2);
+  const int lanes = lanes_for(width), threads = lanes > kThreads ? lanes : kThreads;
+  const int64_t need = ceil_div(rows, threads / lanes), fit = int64_t(sms) * ((backward ? 512 : 1024) / threads > 0 ? (backward ? 512 : 1024) / threads : 1);
+  return int(need < fit ? need : fit);
+}
+static int strands_for(int64_t rows, int64_t width) {
+  if (width <= kMaxWidth) return blocks_for(rows, width, true);
+  return int(rows < 64 ? rows : 64);
+}
+
+template <typename T, int VEC> static void launch(const Args& a, bool backward, cudaStream_t st) {
+  const int lanes = lanes_for(a.width), grid = blocks_for(a.rows, a.width, backward);
+#define LNCC_NORM_CASE(L)                                                            \
+  case L:                                                                            \
+    if (backward) backward_kernel<T, L, VEC><<<grid, L > kThreads ? L : kThreads, 0, st>>>(a); \
+    else forward_kernel<T, L, VEC><<<grid, L > kThreads ? L : kThreads, 0, st>>>(a); \
+    break;
+  switch (lanes) {
+    LNCC_NORM_CASE(4)
+    LNCC_NORM_CASE(8)
+    LNCC_NORM_CASE(16)
+    LNCC_NORM_CASE(32)
+    LNCC_NORM_CASE(64)
+    LNCC_NORM_CASE(128)
+    LNCC_NORM_CASE(256)
+    LNCC_NORM_CASE(512)
+    LNCC_NORM_CASE(1024)
+  }
+#undef LNCC_NORM_CASE
+}
+
+// 16-byte accesses where every row of every array starts on a 16-byte boundary, else single elements.
+template <typename T> static void run(const Args& a, bool backward, cudaStream_t st) {
+  constexpr int VEC = 16 / int(sizeof(T));
+  const bool vec = a.width % VEC == 0 && a.x_stride % VEC == 0 && aligned(a.x, 16) && (!a.y || aligned(a.y, 16)) &&
+                   (!backward || (a.dy_stride % VEC == 0 && aligned(a.dy, 16)));
+  if (a.width > kMaxWidth) {
+    const int grid = blocks_for(a.rows, a.width, backward);
+    if (!backward) {
+      wide_forward_kernel<T><<<grid, 1024, 0, st>>>(a);
+      return;
+    }
+    if (a.y) wide_dx_kernel<T><<<grid, 1024, 0, st>>>(a);
+    if (a.partial)
+      wide_columns_kernel<T><<<dim3(unsigned(ceil_div(a.width, kThreads)), strands_for(a.rows, a.width)), kThreads, 0, st>>>(a);
+    return;
+  }
+  if (vec) launch<T, VEC>(a, backward, st);
+  else launch<T, 1>(a, backward, st);
+}
+
+static void dispatch(const Args& a, int dtype, bool backward, cudaStream_t st) {
+  if (dtype == LNCC_F32) run<float>(a, backward, st);
+  else if (dtype == LNCC_BF16) run<__nv_bfloat16>(a, backward, st);
+  else run<__half>(a, backward, st);
+}
+
+static int check_common(int dtype, int wdtype, int64_t rows, int64_t width, const void* x, int64_t x_stride) {
+  if (!valid_dtype(dtype) || !valid_dtype(wdtype)) return LNCC_ERR_DTYPE;
+  if (wdtype != dtype && wdtype != LNCC_F32) return LNCC_ERR_DTYPE;
+  if (rows < 0 || width < 1) return LNCC_ERR_BAD_ARG;
+  if (width > INT32_MAX / 4) return LNCC_ERR_TOO_LARGE;
+  if (rows > 0 && (!x || !aligned(x, elem_size(dtype)) || (x_stride < width && rows > 1))) return LNCC_ERR_BAD_ARG;
+  return LNCC_OK;
+}
+
+}  // namespace norm
+}  // namespace lncc
+
+using namespace lncc;
+
+extern "C" {
+
+int lncc_layer_norm_forward(const void* x, int64_t x_stride, const void* weight, const void* bias, int dtype, int wdtype,
+                            int64_t rows, int64_t width, float eps, void* y, float* mean, float* rstd,
+                            cudaStream_t stream) {
+  const int st = norm::check_common(dtype, wdtype, rows, width, x, x_stride);
+  if (st != LNCC_OK) return st;
+  if (rows == 0) return LNCC_OK;
+  if (!y || !blk::aligned(y, blk::elem_size(dtype)) || (mean == nullptr) != (rstd == nullptr)) return LNCC_ERR_BAD_ARG;
+  const int cb = blk::check_begin();
+  if (cb != LNCC_OK) return cb;
+  norm::Args a = {};
+  a.x = x, a.x_stride = x_stride, a.w = weight, a.b = bias, a.wdtype = wdtype, a.rows = rows, a.width = int(width);
+  a.eps = eps, a.y = y, a.mean = mean, a.rstd = rstd;
+  norm::dispatch(a, dtype, false, stream);
+  return blk::check_end(stream);
+}
+
+size_t lncc_layer_norm_scratch_bytes(int64_t rows, int64_t width) {
+  if (rows < 1 || width < 1 || width > INT32_MAX / 4) return 0;
+  return size_t(norm::strands_for(rows, width)) * 2 * size_t(width) * sizeof(float);
+}
+
+int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
+                             int dtype, int wdtype, int64_t rows, int64_t width, const float* mean, const float* rstd,
+                             void* dx, void* dweight, void* dbias, void* scratch, size_t scratch_bytes,
+                             cudaStream_t stream) {
+  const int st = norm::check_common(dtype, wdtype, rows, width, x, x_stride);
+  if (st != LNCC_OK) return st;
+  const bool params = dweight || dbias;
+  if (rows == 0) {  // sums over no rows
+    const size_t n = size_t(width) * blk::elem_size(wdtype);
+    if (dweight && cudaMemsetAsync(dweight, 0, n, stream) != cudaSuccess) return LNCC_ERR_CUDA;
+    if (dbias && cudaMemsetAsync(dbias, 0, n, stream) != cudaSuccess) return LNCC_ERR_CUDA;
+    return LNCC_OK;
+  }
+  const int e = blk::elem_size(dtype);
+  if (!dy || !blk::aligned(dy, e) || (dy_stride < width && rows > 1) || !mean || !rstd || (dx && !blk::aligned(dx, e)))
+    return LNCC_ERR_BAD_ARG;
+  if (params && (!scratch || !blk::aligned(scratch, 4) || scratch_bytes < lncc_layer_norm_scratch_bytes(rows, width)))
+    return LNCC_ERR_WORKSPACE;
+  if (!dx && !params) return LNCC_OK;
+  const int cb = blk::check_begin();
+  if (cb != LNCC_OK) return cb;
+  norm::Args a = {};
+  a.x = x, a.x_stride = x_stride, a.dy = dy, a.dy_stride = dy_stride, a.w = weight, a.wdtype = wdtype, a.rows = rows;
+  a.width = int(width), a.y = dx, a.mean = const_cast<float*>(mean), a.rstd = const_cast<float*>(rstd);
+  a.partial = params ? static_cast<float*>(scratch) : nullptr;
+  norm::dispatch(a, dtype, true, stream);
+  if (params)
+    norm::reduce_kernel<<<unsigned(blk::ceil_div(2 * width, 32)), 256, 0, stream>>>(
+        a.partial, norm::strands_for(rows, width), a.width, dweight, dbias, wdtype);
+  return blk::check_end(stream);
+}
+
+}  // extern "C"

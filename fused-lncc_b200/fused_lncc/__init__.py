@@ -21,7 +21,8 @@ import torch
 
 from . import _lib
 
-__all__ = ["fused_lncc_loss", "lncc_fused", "loss_map", "FusedLNCC", "FusedLNCCMap", "compat", "window"]
+__all__ = ["fused_lncc_loss", "lncc_fused", "loss_map", "FusedLNCC", "FusedLNCCMap", "compat", "window",
+           "fused_layer_norm", "fused_gated_scan", "fused_gated_ffn"]
 
 REDUCTIONS = {"mean": 0, "sum": 1}  # the fused kernel's reductions; 'none' has its own path
 
@@ -364,3 +365,6 @@ def fused_lncc_loss(pred, target, kernel_size=7, smooth_dr=1e-5, reduction="mean
 
 from . import compat  # noqa: E402  (registers the reference's fused_lncc::forward/backward ops)
 from . import window  # noqa: E402  (non-cubic windows)
+from .gated_ffn import fused_gated_ffn  # noqa: E402  (the block of a network trained on the loss)
+from .gated_scan import fused_gated_scan  # noqa: E402
+from .layer_norm import fused_layer_norm  # noqa: E402

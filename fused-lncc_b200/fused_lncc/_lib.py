@@ -99,6 +99,41 @@ SIGNATURES = {
         _vp, _vp, _vp, ctypes.c_int, _c_i64, _c_i64, _c_i64, _c_i64,
         ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float, _vp, _vp, ctypes.c_size_t, _vp,
     ]),
+    "lncc_layer_norm_forward": (ctypes.c_int, [
+        _vp, _c_i64, _vp, _vp, ctypes.c_int, ctypes.c_int,   # x, x_stride, weight, bias, dtype, wdtype
+        _c_i64, _c_i64, ctypes.c_float,                      # rows, width, eps
+        _vp, _vp, _vp, _vp,                                  # y, mean, rstd, stream
+    ]),
+    "lncc_layer_norm_scratch_bytes": (ctypes.c_size_t, [_c_i64, _c_i64]),
+    "lncc_layer_norm_backward": (ctypes.c_int, [
+        _vp, _c_i64, _vp, _c_i64, _vp, ctypes.c_int, ctypes.c_int,  # dy, dy_stride, x, x_stride, weight, dtype, wdtype
+        _c_i64, _c_i64, _vp, _vp,                            # rows, width, mean, rstd
+        _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp,            # dx, dweight, dbias, scratch, bytes, stream
+    ]),
+    "lncc_gated_scan_kept_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64]),
+    "lncc_gated_scan_scratch_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64]),
+    "lncc_gated_scan_forward": (ctypes.c_int, [
+        _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, ctypes.c_int,  # x, x_b, x_t, gate, gate_b, gate_t, state, dtype
+        _c_i64, _c_i64, _c_i64, ctypes.c_int,                # B, T, C, reverse
+        _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp,            # h, last, kept, scratch, bytes, stream
+    ]),
+    "lncc_gated_scan_backward": (ctypes.c_int, [
+        _vp, _c_i64, _c_i64, _vp,                            # dh, dh_b, dh_t, dlast
+        _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, ctypes.c_int,  # x, x_b, x_t, gate, gate_b, gate_t, kept, dtype
+        _c_i64, _c_i64, _c_i64, ctypes.c_int,                # B, T, C, reverse
+        _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp,            # dx, dgate, dstate, scratch, bytes, stream
+    ]),
+    "lncc_gated_ffn_scratch_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int]),
+    "lncc_gated_ffn_forward": (ctypes.c_int, [
+        _vp, _c_i64, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int,  # x, x_stride, w_gate, w_up, w_down, dtype, act
+        _c_i64, _c_i64, _c_i64, _c_i64,                      # M, K, F, N
+        _vp, _vp, ctypes.c_size_t, _vp,                      # y, scratch, bytes, stream
+    ]),
+    "lncc_gated_ffn_backward": (ctypes.c_int, [
+        _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, ctypes.c_int, ctypes.c_int,  # dy, dy_stride, x, x_stride, weights, dtype, act
+        _c_i64, _c_i64, _c_i64, _c_i64,                      # M, K, F, N
+        _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp,       # dx, dw_gate, dw_up, dw_down, scratch, bytes, stream
+    ]),
 }
 
 _lock = threading.Lock()

@@ -286,6 +286,83 @@ int lncc_set_companion(int enable);
 int lncc_launch_count(int64_t B, int64_t D, int64_t H, int64_t W, int kernel_size, int dtype,
                       int64_t z_begin, int64_t z_end, int grad);
 
+/*
+ * ---- Token blocks: the operators of a network trained on the loss ------------------------------------------------
+ * Layer norm, the gated linear recurrence and the gated feed-forward block, over arrays whose last axis is contiguous.
+ * dtype (LNCC_F32, LNCC_BF16, LNCC_F16) is the type of every array whose parameter is a void*, except where said;
+ * float* parameters are fp32 for every dtype. All arithmetic and every sum is fp32; results are rounded once, on the
+ * store. Strides are in elements. Results are the same bits run after run: no sum's order depends on timing. Pointers
+ * need the alignment of their element, scratch 16 bytes; arrays whose rows lie on 16-byte boundaries run fastest. No
+ * counterpart in the reference.
+ */
+
+/*
+ * y = (x - mean) * rstd * weight + bias over rows of `width`, rstd = 1/sqrt(var + eps) with the biased variance.
+ *   x           : `rows` rows, x_stride elements apart.
+ *   weight, bias: `width` values of type wdtype, which is dtype or LNCC_F32; NULL stands for ones and zeros.
+ *   y           : (rows, width) contiguous.
+ *   mean, rstd  : NULL, or one float a row each, for the backward pass.
+ */
+int lncc_layer_norm_forward(const void* x, int64_t x_stride, const void* weight, const void* bias, int dtype, int wdtype,
+                            int64_t rows, int64_t width, float eps, void* y, float* mean, float* rstd,
+                            cudaStream_t stream);
+/*
+ * Gradients of the layer norm: dx (rows, width) contiguous, dweight and dbias (`width` values of wdtype, summed over the
+ * rows in a fixed order). Each may be NULL. rows == 0 gives zero dweight and dbias. scratch is needed for dweight and
+ * dbias only.
+ */
+size_t lncc_layer_norm_scratch_bytes(int64_t rows, int64_t width);
+int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* weight,
+                             int dtype, int wdtype, int64_t rows, int64_t width, const float* mean, const float* rstd,
+                             void* dx, void* dweight, void* dbias, void* scratch, size_t scratch_bytes,
+                             cudaStream_t stream);
+
+/*
+ * The gated linear recurrence over (B, T, C):
+ *   a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t, h_0 = state,
+ * for t = 1 .. T, or from the last step to the first with reverse != 0. gate = +inf keeps the state, -inf drops it.
+ *   x, gate  : batch strides x_b, gate_b, time strides x_t, gate_t.
+ *   state    : NULL (zeros) or (B, C).
+ *   h        : (B, T, C) contiguous.        last: (B, C), the state after the last step taken (T == 0: state).
+ *   kept     : NULL, or lncc_gated_scan_kept_bytes(...) bytes that receive the states the backward pass starts from.
+ * Limits: B <= 65535, T <= 65535 * 64, C <= 2^24 (LNCC_ERR_TOO_LARGE).
+ */
+size_t lncc_gated_scan_kept_bytes(int64_t B, int64_t T, int64_t C);
+size_t lncc_gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t C);
+int lncc_gated_scan_forward(const void* x, int64_t x_b, int64_t x_t, const void* gate, int64_t gate_b, int64_t gate_t,
+                            const float* state, int dtype, int64_t B, int64_t T, int64_t C, int reverse, void* h,
+                            float* last, float* kept, void* scratch, size_t scratch_bytes, cudaStream_t stream);
+/*
+ * Its gradients: dx and dgate (B, T, C) contiguous, dstate NULL or (B, C). dh has strides dh_b and dh_t; dlast is NULL
+ * (zeros) or (B, C). x, gate and reverse as in the forward call, kept as it left them.
+ */
+int lncc_gated_scan_backward(const void* dh, int64_t dh_b, int64_t dh_t, const float* dlast, const void* x, int64_t x_b,
+                             int64_t x_t, const void* gate, int64_t gate_b, int64_t gate_t, const float* kept, int dtype,
+                             int64_t B, int64_t T, int64_t C, int reverse, void* dx, void* dgate, float* dstate,
+                             void* scratch, size_t scratch_bytes, cudaStream_t stream);
+
+/* Activations of the gated feed-forward block: x sigmoid(x), x (1 + erf(x / sqrt 2)) / 2, max(x, 0). */
+enum lncc_activation { LNCC_ACT_SILU = 0, LNCC_ACT_GELU = 1, LNCC_ACT_RELU = 2 };
+
+/*
+ * The gated feed-forward block over M tokens: g = x Wg^T, u = x Wu^T, h = act(g) u, y = h Wd^T.
+ *   x          : M rows of K, x_stride elements apart.     w_gate, w_up: (F, K) contiguous.     w_down: (N, F) contiguous.
+ *   y          : (M, N) contiguous.
+ * Limits: K, F, N <= 2^20, M <= 2^30 - 1 (LNCC_ERR_TOO_LARGE).
+ */
+size_t lncc_gated_ffn_scratch_bytes(int64_t M, int64_t K, int64_t F, int64_t N, int dtype, int backward);
+int lncc_gated_ffn_forward(const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down,
+                           int dtype, int act, int64_t M, int64_t K, int64_t F, int64_t N, void* y, void* scratch,
+                           size_t scratch_bytes, cudaStream_t stream);
+/*
+ * Its gradients, each of the shape of what it belongs to, contiguous, and each NULL where it is not wanted. g, u and h
+ * are formed again from x, so the forward pass keeps nothing. M == 0 gives zero weight gradients.
+ */
+int lncc_gated_ffn_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w_gate,
+                            const void* w_up, const void* w_down, int dtype, int act, int64_t M, int64_t K, int64_t F,
+                            int64_t N, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* scratch,
+                            size_t scratch_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
