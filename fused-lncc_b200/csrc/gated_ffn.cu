@@ -4,114 +4,677 @@
 //   dh = dy Wd, dg = dh u act'(g), du = dh act(g), dx = dg Wg + du Wu
 //   dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
-// One 64 x 64 tile of a product a block, 16 of its inner axis at a time through shared memory, fp32 throughout.
-#include "lncc_block.cuh"
+// Every product runs on the tensor cores, in one kernel whose epilogue does what follows it: UP forms g and u side by side
+// in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h; the others write
+// a result or, where a long inner axis is split over the GPU, fp32 partial sums that a last kernel adds in order.
+//
+// A pair of CTAs takes a tile of 256 rows by up to 256 columns (cta_group::2): each loads its 128 rows of A and half the
+// columns of B, 64 steps of the inner axis at a time, into a ring of TMA stages; one thread of the pair issues
+// the products into tensor memory, and eight warps of each CTA read finished tiles back while the next one runs.
+// Halving B between the pair matters: a tile of 256 x 256 asks L2 for 64 bytes a clock and SM at the full rate of the
+// tensor cores, one of 128 x 256 for 96. The grid stays (one pair for each two SMs) and walks over the tiles, columns
+// first, so that the pairs at work share rows of A and the weights stay in L2.
+//
+// Nothing of the hidden layer is kept between forward and backward. Forming g and u again costs 4 of 22 M F K products of a
+// training step, and saves writing and reading 4 M F bytes and a rounding of g and u.
+//
+// Roundings. For 16-bit types h, dg and du are rounded to the type, since they are operands of the next product; g, u and dh
+// never leave fp32. fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
+// the nine products are summed, smallest first (the other three are below 2^-24 of the result). An infinity taken apart
+// so meets zeros: it gives NaN where fp32 would give an infinity.
+#include "lncc_tc.cuh"
 
 namespace lncc {
 namespace ffn {
 
 using namespace blk;
+using namespace tc;
 
-constexpr int kTile = 64, kInner = 16;
+enum Kind { UP, HIDDEN, DOWN, DX, DW_UP, DW_DOWN };
 
-// out[m][n] = sum_k a[m*a_m + k*a_k] * b[n*b_n + k*b_k], and where a2 is given the same sum of a2 and b2 on top
-template <typename TA, typename TB, typename TO>
-__global__ void __launch_bounds__(256) product_kernel(const TA* a, const TA* a2, int64_t a_m, int64_t a_k, const TB* b,
-                                                      const TB* b2, int64_t b_n, int64_t b_k, TO* out, int64_t M,
-                                                      int64_t N, int64_t K) {
-  __shared__ float sa[kInner][kTile + 1], sb[kInner][kTile + 1];
-  const int64_t m0 = int64_t(blockIdx.x) * kTile, n0 = int64_t(blockIdx.y) * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int pair = 0; pair < (a2 ? 2 : 1); pair++) {
-    for (int64_t k0 = 0; k0 < K; k0 += kInner) {
-      for (int i = threadIdx.x; i < kTile * kInner; i += 256) {
-        const int r = i / kInner, k = i % kInner;
-        sa[k][r] = m0 + r < M && k0 + k < K ? to_f((pair ? a2 : a)[(m0 + r) * a_m + (k0 + k) * a_k]) : 0.f;
-        sb[k][r] = n0 + r < N && k0 + k < K ? to_f((pair ? b2 : b)[(n0 + r) * b_n + (k0 + k) * b_k]) : 0.f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kInner; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) acc[i][j] += sa[k][ty * 4 + i] * sb[k][tx * 4 + j];
-      __syncthreads();
-    }
-  }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m < M && n < N && LNCC_IN(m * N + n, 1, M * N)) out[m * N + n] = from_f<TO>(acc[i][j]);
-    }
-}
+constexpr int kThreads = 384;              // warps 0 TMA, 1 products, 4 - 11 epilogue
+constexpr int kATile = 128 * 64 * 2;       // bytes of a CTA's share of A in a stage
 
-// act(g) and act'(g)
-__device__ __forceinline__ void activate(int act, float g, float& a, float& da) {
+__host__ __device__ constexpr bool a_mn(int kind) { return kind == DW_UP || kind == DW_DOWN; }
+__host__ __device__ constexpr bool b_mn(int kind) { return kind == DX || kind == DW_UP || kind == DW_DOWN; }
+__host__ __device__ constexpr int b_tile(int bn) { return bn / 2 * 64 * 2; }  // a CTA's share of B
+__host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 6 : 8; }
+__host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256; }
+
+// Planes of the six products of operands that are taken apart, smallest first.
+__device__ __constant__ const int8_t kPlaneA[6] = {2, 1, 0, 1, 0, 0}, kPlaneB[6] = {0, 1, 2, 0, 1, 0};
+
+struct Gemm {
+  CUtensorMap a0, a1, b0, b1, b2;
+  int64_t rows, cols;        // of a result
+  int m_tiles, n_tiles, whichs, splits;
+  int parts;                 // 6 for operands taken apart, else 1
+  int k_steps, k_steps2;     // blocks of 64 of the inner axis (HIDDEN: of g and u, and of dh)
+  int pairs;                 // products summed into a tile (DX: 2)
+  int bf16, act;
+  void *out0, *out1, *out2;  // results (DW_UP: of which = 0, 1; HIDDEN: dg, du, h)
+  int64_t ld, plane;         // of the results; plane for hidden results taken apart
+  int align;                 // bytes on which every row of the results starts: 32, 16 or the element's
+  float* partial;            // [splits][whichs][rows][cols rounded up to 4], where splits > 1
+  const float* gate;         // HIDDEN, ReLU of fp32: g (rows, cols)
+  unsigned* abort_word;
+  int clear_abort;
+};
+
+// act(g) and act'(g). For 16-bit types the fast exponential and reciprocal (a few u32, and |g| u32 for the exponential),
+// and erf by Abramowitz and Stegun 7.1.26: with z = |g|/sqrt 2 and t = 1/(1 + 0.3275911 z), erfc(z) = t (a1 + t (a2 + ...))
+// exp(-z^2) to 1.5e-7, whose exponential is the one of the derivative.
+template <bool FAST> __device__ __forceinline__ void activate(int act, float g, float& a, float& da) {
   if (act == LNCC_ACT_RELU) {
     a = g < 0.f ? 0.f : g;
     da = g > 0.f ? 1.f : 0.f;
   } else if (act == LNCC_ACT_SILU) {
-    const float p = 1.f / (1.f + expf(-g));
+    const float p = FAST ? __fdividef(1.f, 1.f + __expf(-g)) : 1.f / (1.f + expf(-g));
     a = g * p;
     da = p * (1.f + g * (1.f - p));
   } else {
-    const float p = 0.5f * (1.f + erff(g * 0.70710678f));
+    const float e = FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g);
+    float p;
+    if (FAST) {
+      const float z = fabsf(g) * 0.70710678f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+      const float q = 0.5f * e * t *
+                      fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
+                           0.254829592f);
+      p = g < 0.f ? q : 1.f - q;
+    } else {
+      p = 0.5f * erfcf(-g * 0.70710678f);
+    }
     a = g * p;
-    da = p + g * expf(-0.5f * g * g) * 0.39894228f;
+    da = fmaf(g * 0.39894228f, e, p);
   }
 }
 
-__global__ void __launch_bounds__(256) hidden_kernel(int act, float* g, float* u, float* h, const float* dh, int64_t n) {
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-    float a, da;
-    activate(act, g[i], a, da);
-    const float up = u[i];
-    h[i] = a * up;
-    if (dh) {
-      g[i] = dh[i] * up * da;
-      u[i] = dh[i] * a;
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
+  return uint32_t(__bfloat16_as_ushort(a)) | uint32_t(__bfloat16_as_ushort(b)) << 16;
+}
+__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
+  return uint32_t(__half_as_ushort(a)) | uint32_t(__half_as_ushort(b)) << 16;
+}
+__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+// 16 neighbours of a row, those of them that lie before column `cols`.
+template <typename T>
+__device__ __forceinline__ void emit(T* base, int64_t ld, int64_t row, int64_t col, int64_t cols, int align,
+                                     const T (&v)[16]) {
+  T* p = base + row * ld + col;
+  if (col + 16 <= cols && align >= 16) {
+    constexpr int WORDS = 16 * int(sizeof(T)) / 4;
+    uint32_t w[WORDS];
+#pragma unroll
+    for (int i = 0; i < WORDS; i++) {
+      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+      else w[i] = pack2(v[2 * i], v[2 * i + 1]);
+    }
+    if (align >= 32) {
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 8) {
+        const uint32_t u[8] = {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
+        store32(reinterpret_cast<uint32_t*>(p) + i, u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; i += 4)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      if (col + i < cols) p[i] = v[i];
+  }
+}
+// fp32 as three bf16 numbers that add up to it. The first is cut, not rounded, so that it stays finite; all 24 bits are held.
+__device__ __forceinline__ void take_apart(float v, __nv_bfloat16& hi, __nv_bfloat16& mid, __nv_bfloat16& lo) {
+  hi = __float2bfloat16_rz(v);
+  const float r = v - __bfloat162float(hi);
+  const bool fine = fabsf(v) <= 3.4028235e38f;
+  mid = __float2bfloat16_rn(fine ? r : 0.f);
+  lo = __float2bfloat16_rn(fine ? r - __bfloat162float(mid) : 0.f);
+}
+// Hidden results: of the type, or taken apart for fp32.
+template <typename T>
+__device__ __forceinline__ void emit_hidden(void* base, const Gemm& g, int64_t row, int64_t col, const float (&v)[16]) {
+  if (row >= g.rows || col >= g.cols || !LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) return;
+  if constexpr (sizeof(T) == 2) {
+    T o[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[i] = from_f<T>(v[i]);
+    emit<T>(static_cast<T*>(base), g.ld, row, col, g.cols, g.align, o);
+  } else {
+    __nv_bfloat16 o[3][16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) take_apart(v[i], o[0][i], o[1][i], o[2][i]);
+#pragma unroll
+    for (int k = 0; k < 3; k++)
+      emit<__nv_bfloat16>(static_cast<__nv_bfloat16*>(base) + k * g.plane, g.ld, row, col, g.cols, g.align, o[k]);
+  }
+}
+
+struct Tile {
+  int n, m, which, split;
+};
+__device__ __forceinline__ Tile tile_of(const Gemm& g, int t) {
+  Tile r;
+  r.n = t % g.n_tiles, t /= g.n_tiles;
+  r.m = t % g.m_tiles, t /= g.m_tiles;
+  r.which = t % g.whichs;
+  r.split = t / g.whichs;
+  return r;
+}
+
+// T: type of the results (for float, bf16 operands taken apart). KIND, BN: see above; UP and HIDDEN hold BN/2 columns of g
+// and of u, HIDDEN BN/2 of dh beside them.
+template <int KIND, int BN, typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Gemm g) {
+  constexpr int STAGES = stages(BN), BT = b_tile(BN), HALF = BN / 2;
+  constexpr bool AM = a_mn(KIND), BM = b_mn(KIND);
+  constexpr int ACCS = KIND == HIDDEN ? 1 : 2;  // tiles of accumulators in tensor memory
+  constexpr bool FAST = sizeof(T) == 2;
+  static_assert(KIND != HIDDEN || BN == 256, "dh's share of B is one block of 64 columns a CTA");
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
+  const uint32_t tiles_at = smem_addr(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * (kATile + BT));
+  const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16;
+  __shared__ uint32_t tmem_at;
+  __shared__ int gave_up_flag;
+  volatile int* gave_up = &gave_up_flag;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cta_rank();
+
+  if (g.clear_abort && blockIdx.x == 0 && threadIdx.x == 0) *g.abort_word = 0u;  // waits give up seconds later
+  if (threadIdx.x == 0) {
+    gave_up_flag = 0;
+    for (int i = 0; i < STAGES; i++) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; i++) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, 16);  // eight epilogue warps of each CTA
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    tmem_alloc<512>(smem_addr(&tmem_at));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();
+  fence_after();
+  const uint32_t tmem = tmem_at;
+  const int pairs_at_work = gridDim.x / 2, tiles = g.n_tiles * g.m_tiles * g.whichs * g.splits;
+  const int gu_steps = g.k_steps * g.parts;
+  const int dh_steps = KIND == HIDDEN ? g.k_steps2 * g.parts : 0;
+  const int all_steps = KIND == HIDDEN ? gu_steps + dh_steps : gu_steps * g.pairs;
+
+  if (warp == 0 && lane == 0) {
+    // ---- TMA: this CTA's shares of A and B, counted on the first CTA's barrier
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs_at_work) {
+      const Tile w = tile_of(g, t);
+      const int from = int(int64_t(all_steps) * w.split / g.splits), to = int(int64_t(all_steps) * (w.split + 1) / g.splits);
+      const int m0 = w.m * 256 + int(rank) * 128;
+      for (int s = from; s < to; s++) {
+        if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up))) break;
+        const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile, bar = peer_addr(full + 8 * stage, 0);
+        const bool dh_phase = KIND == HIDDEN && s < dh_steps;
+        const int in = KIND == HIDDEN && !dh_phase ? s - dh_steps : s, ks = dh_phase ? g.k_steps2 : g.k_steps;
+        const int k = in % ks * 64, part = in / ks % g.parts, pair = in / ks / g.parts;
+        const int pa = g.parts > 1 ? kPlaneA[part] : 0, pb = g.parts > 1 ? kPlaneB[part] : 0;
+        if (rank == 0) mbar_expect(full + 8 * stage, 2 * (kATile + (dh_phase ? 8192 : BT)));
+        const CUtensorMap* am = dh_phase || (KIND == DX && pair) || (KIND == DW_UP && w.which) ? &g.a1 : &g.a0;
+        if (AM) {
+          tma_load(am, at, bar, m0, k, pa);
+          tma_load(am, at + kATile / 2, bar, m0 + 64, k, pa);
+        } else {
+          tma_load(am, at, bar, k, m0, pa);
+        }
+        if (dh_phase) {  // half of the tile's 128 columns of Wd, which memory holds along F
+          tma_load(&g.b2, bt, bar, w.n * HALF + int(rank) * 64, k, pb);
+        } else if (KIND == UP || KIND == HIDDEN) {  // the gate's rows in one CTA, the up projection's in the other
+          tma_load(rank ? &g.b1 : &g.b0, bt, bar, k, w.n * HALF, pb);
+        } else if (BM) {
+          const CUtensorMap* bm = KIND == DX && pair ? &g.b1 : &g.b0;
+#pragma unroll
+          for (int i = 0; i < HALF; i += 64) tma_load(bm, bt + i / 64 * 8192, bar, w.n * BN + int(rank) * HALF + i, k, pb);
+        } else {
+          tma_load(&g.b0, bt, bar, k, w.n * BN + int(rank) * HALF, pb);
+        }
+        if (++stage == STAGES) stage = 0, phase ^= 1;
+      }
+    }
+    // every copy has landed once its stage has been read; after giving up, copies in flight get 10 ms to land
+    for (int i = 0; i < STAGES && ok; i++) {
+      ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up);
+      if (++stage == STAGES) stage = 0, phase ^= 1;
+    }
+    if (!ok)
+      for (const unsigned long long start = now_ns(); now_ns() - start < 10000000ull;) __nanosleep(1000);
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ---- products of the pair
+    int stage = 0, turn = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t wide = instr_desc(g.bf16, AM, BM, BN), narrow = instr_desc(g.bf16, false, true, HALF);
+    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs_at_work, turn++) {
+      const Tile w = tile_of(g, t);
+      const int from = int(int64_t(all_steps) * w.split / g.splits), to = int(int64_t(all_steps) * (w.split + 1) / g.splits);
+      const int acc = ACCS == 2 ? turn & 1 : 0;
+      const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
+      // HIDDEN: dh alternates between two places, so it may run while the last tile is read; g and u wait for that
+      const uint32_t d_dh = tmem + BN + (turn & 1) * HALF, d = tmem + (ACCS == 2 ? acc * 256 : 0);
+      if (KIND != HIDDEN) {
+        if (!(ok = mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, gave_up))) break;
+        fence_after();
+      }
+      for (int s = from; s < to; s++) {
+        const bool dh_phase = KIND == HIDDEN && s < dh_steps;
+        if (KIND == HIDDEN && s == dh_steps) {
+          if (!(ok = mbar_wait(acc_empty, acc_phase ^ 1, gave_up))) break;
+          fence_after();
+        }
+        if (!(ok = mbar_wait(full + 8 * stage, phase, gave_up))) break;
+        fence_after();
+        const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile;
+        const uint64_t da = AM ? desc_mn(at, 8192) : desc_k(at);
+        const uint64_t db = BM || dh_phase ? desc_mn(bt, 8192) : desc_k(bt);
+        const uint64_t a_step = AM ? 128 : 2, b_step = BM || dh_phase ? 128 : 2;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          mma(dh_phase ? d_dh : d, da + k * a_step, db + k * b_step, dh_phase ? narrow : wide,
+              k > 0 || (dh_phase ? s > 0 : s > (KIND == HIDDEN ? dh_steps : from)));
+        commit_pair(empty + 8 * stage);
+        if (++stage == STAGES) stage = 0, phase ^= 1;
+      }
+      if (ok) commit_pair(acc_full + 8 * acc);
+    }
+  } else if (warp >= 4) {
+    // ---- epilogue: lanes are rows; two warps share a row, half of the columns each
+    const int sub = warp & 3, half = (warp - 4) / 4;
+    int turn = 0;
+    for (int t = blockIdx.x / 2; t < tiles; t += pairs_at_work, turn++) {
+      const Tile w = tile_of(g, t);
+      const int acc = ACCS == 2 ? turn & 1 : 0;
+      const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
+      const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_phase, gave_up));
+      fence_after();
+      const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (ACCS == 2 ? acc * 256 : 0);
+      const int64_t row = int64_t(w.m) * 256 + rank * 128 + sub * 32 + lane;
+      const float nan = __int_as_float(0x7fffffff);
+      if constexpr (KIND == UP || KIND == HIDDEN) {
+#pragma unroll 1
+        for (int c = half * (HALF / 2); c < (half + 1) * (HALF / 2); c += 16) {
+          const int64_t col = int64_t(w.n) * HALF + c;
+          __syncwarp();
+          uint32_t vg[16], vu[16], vd[16];
+          if (ok) {
+            tmem_load(d + c, vg);
+            tmem_load(d + HALF + c, vu);
+            if (KIND == HIDDEN) tmem_load(d + BN + (turn & 1) * HALF + c, vd);
+            wait_ld(vg);
+            wait_ld(vu);
+            if (KIND == HIDDEN) wait_ld(vd);
+          }
+          float h[16], dg[16], du[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            float gate = ok ? __uint_as_float(vg[i]) : nan, a, da;
+            const float up = ok ? __uint_as_float(vu[i]) : nan;
+            if (KIND == HIDDEN && !FAST && g.gate && row < g.rows && col + i < g.cols) gate = g.gate[row * g.cols + col + i];
+            activate<FAST>(g.act, gate, a, da);
+            h[i] = a * up;
+            if (KIND == HIDDEN) {
+              const float dh = ok ? __uint_as_float(vd[i]) : nan;
+              dg[i] = dh * up * da;
+              du[i] = dh * a;
+            }
+          }
+          if (KIND == HIDDEN) {
+            emit_hidden<T>(g.out0, g, row, col, dg);
+            emit_hidden<T>(g.out1, g, row, col, du);
+            emit_hidden<T>(g.out2, g, row, col, h);
+          } else {
+            emit_hidden<T>(g.out0, g, row, col, h);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = half * HALF; c < (half + 1) * HALF; c += 16) {
+          const int64_t col = int64_t(w.n) * BN + c;
+          __syncwarp();
+          uint32_t v[16];
+          if (ok) {
+            tmem_load(d + c, v);
+            wait_ld(v);
+          }
+          if (row < g.rows && col < g.cols) {
+            if (g.splits > 1) {
+              const int64_t ld = (g.cols + 3) / 4 * 4;
+              float o[16];
+#pragma unroll
+              for (int i = 0; i < 16; i++) o[i] = ok ? __uint_as_float(v[i]) : nan;
+              emit<float>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row, col, ld, 16, o);
+            } else if (LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) {
+              T o[16];
+#pragma unroll
+              for (int i = 0; i < 16; i++) o[i] = from_f<T>(ok ? __uint_as_float(v[i]) : nan);
+              emit<T>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row, col, g.cols, g.align, o);
+            }
+          }
+        }
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty + 8 * acc, 0));
     }
   }
+  __syncwarp();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while the other may still signal it or read its shares
+  if (*gave_up && threadIdx.x == 0) atomicOr(g.abort_word, 1u);
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-template <typename TA, typename TB, typename TO>
-static void product(const TA* a, const TA* a2, int64_t a_m, int64_t a_k, const TB* b, const TB* b2, int64_t b_n,
-                    int64_t b_k, TO* out, int64_t M, int64_t N, int64_t K, cudaStream_t st) {
-  product_kernel<<<dim3(unsigned(ceil_div(M, kTile)), unsigned(ceil_div(N, kTile))), 256, 0, st>>>(
-      a, a2, a_m, a_k, b, b2, b_n, b_k, out, M, N, K);
+// Partial sums of the splits, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int whichs, int64_t rows,
+                                                   int64_t cols, T* out0, T* out1) {
+  const int64_t ld = (cols + 3) / 4 * 4, quads = whichs * rows * (ld / 4), slab = whichs * rows * ld;
+  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < quads; q += int64_t(gridDim.x) * 256) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < splits; i++) {
+      const float4 v = *reinterpret_cast<const float4*>(partial + i * slab + q * 4);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const int64_t row = q / (ld / 4) % rows, col = q % (ld / 4) * 4;
+    T* out = q / (ld / 4) / rows ? out1 : out0;
+    if (out == nullptr) continue;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) out[row * cols + col + i] = from_f<T>(v[i]);
+  }
 }
 
+// A matrix that TMA cannot read as it lies (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows.
+template <typename T, typename TO>
+__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, int64_t stride, int64_t rows, int64_t cols,
+                                                   TO* dst, int64_t ld, int64_t plane) {
+  const int64_t eights = rows * (ld / 8);
+  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < eights; q += int64_t(gridDim.x) * 256) {
+    const int64_t row = q / (ld / 8), col = q % (ld / 8) * 8;
+    Vec<TO, 8> o[3];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const T v = col + i < cols && LNCC_IN(row * stride + col + i, 1, (rows - 1) * stride + cols) ? src[row * stride + col + i]
+                                                                                                  : from_f<T>(0.f);
+      if constexpr (sizeof(T) == 4) take_apart(v, o[0].e[i], o[1].e[i], o[2].e[i]);
+      else o[0].e[i] = v;
+    }
+#pragma unroll
+    for (int k = 0; k < (sizeof(T) == 4 ? 3 : 1); k++)
+      *reinterpret_cast<Vec<TO, 8>*>(dst + k * plane + row * ld + col) = o[k];
+  }
+}
+
+// g = x Wg^T by fp32 multiply-adds in the order of k, for the backward pass of ReLU in fp32 alone: the derivative jumps at
+// g = 0, where the last bit of g decides, so g is the plain fp32 sum there.
+constexpr int kTile = 64, kInner = 16;
+__global__ void __launch_bounds__(256) gate_kernel(const float* x, int64_t x_stride, const float* w, float* out, int64_t M,
+                                                   int64_t N, int64_t K) {
+  __shared__ float sa[kInner][kTile + 1], sb[kInner][kTile + 1];
+  const int64_t m0 = int64_t(blockIdx.x) * kTile, n0 = int64_t(blockIdx.y) * kTile;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  float acc[4][4] = {};
+  for (int64_t k0 = 0; k0 < K; k0 += kInner) {
+    for (int i = threadIdx.x; i < kTile * kInner; i += 256) {
+      const int r = i / kInner, k = i % kInner;
+      sa[k][r] = m0 + r < M && k0 + k < K ? x[(m0 + r) * x_stride + k0 + k] : 0.f;
+      sb[k][r] = n0 + r < N && k0 + k < K ? w[(n0 + r) * K + k0 + k] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kInner; k++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) acc[i][j] += sa[k][ty * 4 + i] * sb[k][tx * 4 + j];
+    __syncthreads();
+  }
+  for (int i = 0; i < 4; i++)
+    for (int j = 0; j < 4; j++) {
+      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
+      if (m < M && n < N && LNCC_IN(m * N + n, 1, M * N)) out[m * N + n] = acc[i][j];
+    }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
 struct Args {
   const void *x, *wg, *wu, *wd, *dy;
   int64_t x_stride, dy_stride, M, K, F, N;
-  int act;
+  int act, dtype;
   void *y, *dx, *dwg, *dwu, *dwd;
-  float *g, *u, *h, *dh;
 };
 
-template <typename T> static void forward(const Args& p, cudaStream_t st) {
-  const T *x = static_cast<const T*>(p.x), *wg = static_cast<const T*>(p.wg), *wu = static_cast<const T*>(p.wu);
-  const T *wd = static_cast<const T*>(p.wd), *none = nullptr;
-  const float* nof = nullptr;
-  product(x, none, p.x_stride, 1, wg, none, p.K, 1, p.g, p.M, p.F, p.K, st);
-  product(x, none, p.x_stride, 1, wu, none, p.K, 1, p.u, p.M, p.F, p.K, st);
-  hidden_kernel<<<sm_count() * 4, 256, 0, st>>>(p.act, p.g, p.u, p.h, nullptr, p.M * p.F);
-  product((const float*)p.h, nof, p.F, 1, wd, none, p.F, 1, static_cast<T*>(p.y), p.M, p.N, p.F, st);
+constexpr size_t kHeader = 256;  // the abort word, as in the loss's workspace
+inline size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
+inline int64_t lead(int64_t cols) { return (cols + 15) / 16 * 16; }  // rows of hidden and packed matrices: 32-byte starts
+
+// How a product is cut into tiles: 256 columns, or 128 where that would leave pairs of SMs without work or columns
+// empty, and then the inner axis over the pairs that are still free.
+struct Cut {
+  int bn, m_tiles, n_tiles, splits;
+};
+static Cut cut_for(int kind, int64_t rows, int64_t cols, int whichs, int64_t steps) {
+  const int pairs = sm_count() / 2;
+  const bool gated = kind == UP || kind == HIDDEN;
+  Cut c;
+  c.m_tiles = int(ceil_div(rows, 256));
+  c.bn = 256;
+  c.n_tiles = int(ceil_div(cols, gated ? 128 : 256));
+  if (kind != HIDDEN && (int64_t(c.m_tiles) * c.n_tiles * whichs < pairs || cols <= (gated ? 64 : 128))) {
+    c.bn = 128;
+    c.n_tiles = int(ceil_div(cols, gated ? 64 : 128));
+  }
+  c.splits = 1;
+  const int64_t tiles = int64_t(c.m_tiles) * c.n_tiles * whichs;
+  if (!gated && tiles <= pairs / 2) {  // at least 8 steps for each split
+    const int64_t want = pairs / tiles, most = steps / 8;
+    c.splits = int(want < most ? want : most);
+    if (c.splits < 1) c.splits = 1;
+  }
+  return c;
 }
-template <typename T> static void backward(const Args& p, cudaStream_t st) {
-  const T *x = static_cast<const T*>(p.x), *dy = static_cast<const T*>(p.dy), *wd = static_cast<const T*>(p.wd);
-  const T *wg = static_cast<const T*>(p.wg), *wu = static_cast<const T*>(p.wu), *none = nullptr;
-  const float *nof = nullptr, *g = p.g, *u = p.u;
-  product(x, none, p.x_stride, 1, wg, none, p.K, 1, p.g, p.M, p.F, p.K, st);
-  product(x, none, p.x_stride, 1, wu, none, p.K, 1, p.u, p.M, p.F, p.K, st);
-  product(dy, none, p.dy_stride, 1, wd, none, 1, p.F, p.dh, p.M, p.F, p.N, st);
-  hidden_kernel<<<sm_count() * 4, 256, 0, st>>>(p.act, p.g, p.u, p.h, p.dh, p.M * p.F);
-  if (p.dx) product(g, u, p.F, 1, wg, wu, 1, p.K, static_cast<T*>(p.dx), p.M, p.K, p.F, st);
-  if (p.dwg) product(g, nof, 1, p.F, x, none, 1, p.x_stride, static_cast<T*>(p.dwg), p.F, p.K, p.M, st);
-  if (p.dwu) product(u, nof, 1, p.F, x, none, 1, p.x_stride, static_cast<T*>(p.dwu), p.F, p.K, p.M, st);
-  if (p.dwd) product(dy, none, 1, p.dy_stride, (const float*)p.h, nof, 1, p.F, static_cast<T*>(p.dwd), p.N, p.F, p.M, st);
+
+// Scratch of a call, laid out in one place for its size and its use.
+struct Plan {
+  int parts, planes;
+  size_t x, wg, wu, wd, dy, h, dg, du, gate, partial, total;
+  int64_t ldf;
+};
+static size_t partial_bytes(int kind, int64_t rows, int64_t cols, int whichs, int64_t steps) {
+  const Cut c = cut_for(kind, rows, cols, whichs, steps);
+  return c.splits > 1 ? size_t(c.splits) * whichs * rows * ((cols + 3) / 4 * 4) * 4 : 0;
+}
+static int64_t k_steps(int64_t k) { return ceil_div(k, 64); }
+static Plan plan_for(const Args& a, bool backward) {
+  Plan p = {};
+  p.planes = a.dtype == LNCC_F32 ? 3 : 1;
+  p.parts = a.dtype == LNCC_F32 ? 6 : 1;
+  p.ldf = lead(a.F);
+  size_t at = kHeader;
+  const auto take = [&](int64_t rows, int64_t ld) {
+    const size_t here = at;
+    at += round_up(size_t(p.planes) * rows * ld * 2);
+    return here;
+  };
+  p.x = take(a.M, lead(a.K));
+  p.wg = take(a.F, lead(a.K));
+  p.wu = take(a.F, lead(a.K));
+  p.wd = take(a.N, p.ldf);
+  p.h = take(a.M, p.ldf);
+  size_t most = 0;
+  const auto partial = [&](size_t n) { most = n > most ? n : most; };
+  if (backward) {
+    p.dy = take(a.M, lead(a.N));
+    p.dg = take(a.M, p.ldf);
+    p.du = take(a.M, p.ldf);
+    p.gate = at;
+    if (a.dtype == LNCC_F32 && a.act == LNCC_ACT_RELU) at += round_up(size_t(a.M) * a.F * 4);
+    partial(partial_bytes(DX, a.M, a.K, 1, 2 * p.parts * k_steps(a.F)));
+    partial(partial_bytes(DW_UP, a.F, a.K, 2, p.parts * k_steps(a.M)));
+    partial(partial_bytes(DW_DOWN, a.N, a.F, 1, p.parts * k_steps(a.M)));
+  } else {
+    partial(partial_bytes(DOWN, a.M, a.N, 1, p.parts * k_steps(a.F)));
+  }
+  p.partial = at;
+  p.total = at + round_up(most);
+  return p;
+}
+
+struct Call {
+  const Args& a;
+  Plan plan;
+  char* scratch;
+  cudaStream_t stream;
+  int status;
+  bool first;  // the next product kernel is the call's first
+
+  // src as TMA reads it: in place, or packed to `to`
+  Matrix operand(const void* src, int64_t rows, int64_t cols, int64_t stride, size_t to) {
+    Matrix m = {const_cast<void*>(src), rows, cols, stride, 0, 1, a.dtype != LNCC_F16};
+    if (a.dtype != LNCC_F32 && aligned(src, 16) && (stride % 8 == 0 || rows == 1)) {
+      if (rows == 1) m.ld = lead(cols);
+      return m;
+    }
+    m.p = scratch + to;
+    m.ld = lead(cols);
+    m.plane = rows * m.ld;
+    m.planes = plan.planes;
+    const int64_t blocks = ceil_div(rows * (m.ld / 8), 256), most = int64_t(sm_count()) * 8;
+    const unsigned grid = unsigned(blocks < most ? blocks : most);
+    if (a.dtype == LNCC_F32)
+      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(src), stride, rows, cols,
+                                            static_cast<__nv_bfloat16*>(m.p), m.ld, m.plane);
+    else if (a.dtype == LNCC_BF16)
+      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(src), stride, rows, cols,
+                                            static_cast<__nv_bfloat16*>(m.p), m.ld, m.plane);
+    else
+      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const __half*>(src), stride, rows, cols, static_cast<__half*>(m.p),
+                                            m.ld, m.plane);
+    return m;
+  }
+  Matrix hidden(size_t at) const {
+    return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.planes, a.dtype != LNCC_F16};
+  }
+
+  template <int KIND, int BN, typename T> void launch(Gemm& g) {
+    const int smem = smem_bytes(BN), pairs = sm_count() / 2;
+    if (cudaFuncSetAttribute(product_kernel<KIND, BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+      cudaGetLastError();
+      status = LNCC_ERR_SMEM;
+      return;
+    }
+    const int64_t tiles = int64_t(g.m_tiles) * g.n_tiles * g.whichs * g.splits;
+    product_kernel<KIND, BN, T><<<unsigned(2 * (tiles < pairs ? tiles : pairs)), kThreads, smem, stream>>>(g);
+  }
+  template <int KIND, typename T> void launch_bn(Gemm& g, int bn) {
+    if constexpr (KIND == HIDDEN) launch<KIND, 256, T>(g);
+    else if (bn == 256) launch<KIND, 256, T>(g);
+    else launch<KIND, 128, T>(g);
+  }
+
+  // One product: A (a0, a1) and B (b0, b1, b2) as the kind takes them, results out (rows x cols, ld apart).
+  template <int KIND>
+  void product(const Matrix& a0, const Matrix& a1, const Matrix& b0, const Matrix& b1, const Matrix& b2, int64_t rows,
+               int64_t cols, int whichs, int64_t inner, int64_t inner2, void* out0, void* out1, void* out2, int64_t ld,
+               int64_t plane) {
+    if (status != LNCC_OK) return;
+    Gemm g = {};
+    g.parts = plan.parts;
+    g.k_steps = int(k_steps(inner));
+    g.k_steps2 = int(k_steps(inner2));
+    g.pairs = KIND == DX ? 2 : 1;
+    const Cut c = cut_for(KIND, rows, cols, whichs, int64_t(g.pairs) * g.parts * g.k_steps);
+    g.m_tiles = c.m_tiles, g.n_tiles = c.n_tiles, g.splits = c.splits, g.whichs = whichs;
+    const int a_box = a_mn(KIND) ? 64 : 128, b_box = b_mn(KIND) ? 64 : c.bn / 2;
+    if (!make_map(&g.a0, a0, a_box) || !make_map(&g.a1, a1, a_box) || !make_map(&g.b0, b0, b_box) ||
+        !make_map(&g.b1, b1, b_box) || !make_map(&g.b2, b2, 64)) {
+      status = LNCC_ERR_CUDA;
+      return;
+    }
+    g.rows = rows, g.cols = cols, g.bf16 = a0.bf16, g.act = a.act;
+    g.out0 = out0, g.out1 = out1, g.out2 = out2, g.ld = ld, g.plane = plane;
+    const int es = KIND == UP || KIND == HIDDEN ? 2 : elem_size(a.dtype);
+    g.align = es;
+    for (int al = 16; al <= 32; al *= 2)
+      if (aligned(out0, al) && aligned(out1, al) && aligned(out2, al) && ld * es % al == 0) g.align = al;
+    g.partial = reinterpret_cast<float*>(scratch + plan.partial);
+    g.gate = KIND == HIDDEN && a.dtype == LNCC_F32 && a.act == LNCC_ACT_RELU
+                 ? reinterpret_cast<const float*>(scratch + plan.gate) : nullptr;
+    g.abort_word = reinterpret_cast<unsigned*>(scratch);
+    g.clear_abort = first;
+    first = false;
+    if (a.dtype == LNCC_F32) launch_bn<KIND, float>(g, c.bn);
+    else if (a.dtype == LNCC_BF16) launch_bn<KIND, __nv_bfloat16>(g, c.bn);
+    else launch_bn<KIND, __half>(g, c.bn);
+    if (g.splits > 1 && status == LNCC_OK) {
+      const int64_t blocks = ceil_div(whichs * rows * ceil_div(cols, 4), 256), most = int64_t(sm_count()) * 8;
+      const unsigned grid = unsigned(blocks < most ? blocks : most);
+      if (a.dtype == LNCC_F32)
+        join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<float*>(out0),
+                                              static_cast<float*>(out1));
+      else if (a.dtype == LNCC_BF16)
+        join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<__nv_bfloat16*>(out0),
+                                              static_cast<__nv_bfloat16*>(out1));
+      else
+        join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<__half*>(out0),
+                                              static_cast<__half*>(out1));
+    }
+    if (cudaPeekAtLastError() != cudaSuccess) status = LNCC_ERR_LAUNCH;
+  }
+};
+
+static int forward(const Args& a, void* scratch, cudaStream_t stream) {
+  Call c = {a, plan_for(a, false), static_cast<char*>(scratch), stream, LNCC_OK, true};
+  const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg),
+               wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu), wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd),
+               h = c.hidden(c.plan.h);
+  c.product<UP>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, h.p, nullptr, nullptr, h.ld, h.plane);
+  c.product<DOWN>(h, h, wd, wd, wd, a.M, a.N, 1, a.F, 0, a.y, nullptr, nullptr, a.N, 0);
+  return c.status;
+}
+
+static int backward(const Args& a, void* scratch, cudaStream_t stream) {
+  Call c = {a, plan_for(a, true), static_cast<char*>(scratch), stream, LNCC_OK, true};
+  const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), dy = c.operand(a.dy, a.M, a.N, a.dy_stride, c.plan.dy),
+               wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg), wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu),
+               wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd);
+  const Matrix h = c.hidden(c.plan.h), dg = c.hidden(c.plan.dg), du = c.hidden(c.plan.du);
+  if (a.dtype == LNCC_F32 && a.act == LNCC_ACT_RELU)
+    gate_kernel<<<dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, stream>>>(
+        static_cast<const float*>(a.x), a.x_stride, static_cast<const float*>(a.wg),
+        reinterpret_cast<float*>(c.scratch + c.plan.gate), a.M, a.F, a.K);
+  c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
+  if (a.dx) c.product<DX>(dg, du, wg, wu, wg, a.M, a.K, 1, a.F, 0, a.dx, nullptr, nullptr, a.K, 0);
+  if (a.dwg || a.dwu) {
+    // one product for both where both are wanted
+    const Matrix& first = a.dwg ? dg : du;
+    c.product<DW_UP>(first, du, x, x, x, a.F, a.K, a.dwg && a.dwu ? 2 : 1, a.M, 0, a.dwg ? a.dwg : a.dwu, a.dwu, nullptr, a.K, 0);
+  }
+  if (a.dwd) c.product<DW_DOWN>(dy, dy, h, h, h, a.N, a.F, 1, a.M, 0, a.dwd, nullptr, nullptr, a.F, 0);
+  return c.status;
 }
 
 static int check_sizes(int dtype, int act, int64_t M, int64_t K, int64_t F, int64_t N) {
@@ -130,8 +693,10 @@ using namespace lncc;
 extern "C" {
 
 size_t lncc_gated_ffn_scratch_bytes(int64_t M, int64_t K, int64_t F, int64_t N, int dtype, int backward) {
-  if (ffn::check_sizes(dtype, 0, M, K, F, N) != LNCC_OK) return 0;
-  return size_t(backward ? 4 : 3) * size_t(M) * size_t(F) * sizeof(float);
+  if (ffn::check_sizes(dtype, 0, M, K, F, N) != LNCC_OK || M == 0) return 0;
+  ffn::Args a = {};
+  a.M = M, a.K = K, a.F = F, a.N = N, a.dtype = dtype, a.act = LNCC_ACT_RELU;  // the activation that needs most
+  return ffn::plan_for(a, backward != 0).total;
 }
 
 int lncc_gated_ffn_forward(const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down,
@@ -148,13 +713,11 @@ int lncc_gated_ffn_forward(const void* x, int64_t x_stride, const void* w_gate, 
   const int cb = blk::check_begin();
   if (cb != LNCC_OK) return cb;
   ffn::Args p = {};
-  p.x = x, p.x_stride = x_stride, p.wg = w_gate, p.wu = w_up, p.wd = w_down, p.act = act, p.y = y;
+  p.x = x, p.x_stride = x_stride, p.wg = w_gate, p.wu = w_up, p.wd = w_down, p.act = act, p.dtype = dtype, p.y = y;
   p.M = M, p.K = K, p.F = F, p.N = N;
-  p.g = static_cast<float*>(scratch), p.u = p.g + M * F, p.h = p.u + M * F;
-  if (dtype == LNCC_F32) ffn::forward<float>(p, stream);
-  else if (dtype == LNCC_BF16) ffn::forward<__nv_bfloat16>(p, stream);
-  else ffn::forward<__half>(p, stream);
-  return blk::check_end(stream);
+  const int run = ffn::forward(p, scratch, stream);
+  const int ended = blk::check_end(stream);
+  return run != LNCC_OK ? run : ended;
 }
 
 int lncc_gated_ffn_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* w_gate,
@@ -181,12 +744,11 @@ int lncc_gated_ffn_backward(const void* dy, int64_t dy_stride, const void* x, in
   if (cb != LNCC_OK) return cb;
   ffn::Args p = {};
   p.x = x, p.x_stride = x_stride, p.dy = dy, p.dy_stride = dy_stride, p.wg = w_gate, p.wu = w_up, p.wd = w_down;
-  p.act = act, p.dx = dx, p.dwg = dw_gate, p.dwu = dw_up, p.dwd = dw_down, p.M = M, p.K = K, p.F = F, p.N = N;
-  p.g = static_cast<float*>(scratch), p.u = p.g + M * F, p.h = p.u + M * F, p.dh = p.h + M * F;
-  if (dtype == LNCC_F32) ffn::backward<float>(p, stream);
-  else if (dtype == LNCC_BF16) ffn::backward<__nv_bfloat16>(p, stream);
-  else ffn::backward<__half>(p, stream);
-  return blk::check_end(stream);
+  p.act = act, p.dtype = dtype, p.dx = dx, p.dwg = dw_gate, p.dwu = dw_up, p.dwd = dw_down;
+  p.M = M, p.K = K, p.F = F, p.N = N;
+  const int run = ffn::backward(p, scratch, stream);
+  const int ended = blk::check_end(stream);
+  return run != LNCC_OK ? run : ended;
 }
 
 }  // extern "C"
