@@ -5,8 +5,9 @@
 //   dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
 // Every product runs on the tensor cores, in one kernel whose epilogue does what follows it: UP forms g and u side by side
-// in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h; the others write
-// a result or, where a long inner axis is split over the GPU, fp32 partial sums that a last kernel adds in order.
+// in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h (for fp32 GATES
+// writes g and u, and DH forms dh and reads them); the others write a result or, where a long inner axis is split over
+// the GPU, fp32 partial sums that a last kernel adds in order.
 //
 // A pair of CTAs takes a tile of 256 rows by up to 256 columns (cta_group::2): each loads its 128 rows of A and half the
 // columns of B, 64 steps of the inner axis at a time, into a ring of TMA stages; one thread of the pair issues
@@ -20,8 +21,10 @@
 //
 // Roundings. For 16-bit types h, dg and du are rounded to the type, since they are operands of the next product; g, u and dh
 // never leave fp32. fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
-// the nine products are summed, smallest first (the other three are below 2^-24 of the result). An infinity taken apart
-// so meets zeros: it gives NaN where fp32 would give an infinity.
+// the nine products are summed, smallest first (the other three are below 2^-24 of the result). The tensor cores cut, not
+// round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of the result. So for fp32 an
+// accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each time. An
+// infinity taken apart meets zeros: it gives NaN where fp32 would give an infinity.
 #include "lncc_tc.cuh"
 
 namespace lncc {
@@ -30,13 +33,15 @@ namespace ffn {
 using namespace blk;
 using namespace tc;
 
-enum Kind { UP, HIDDEN, DOWN, DX, DW_UP, DW_DOWN };
+enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
 
 constexpr int kThreads = 384;              // warps 0 TMA, 1 products, 4 - 11 epilogue
 constexpr int kATile = 128 * 64 * 2;       // bytes of a CTA's share of A in a stage
+constexpr int kChunk = 4;                  // blocks of 64 that an accumulator of fp32 takes
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == DW_UP || kind == DW_DOWN; }
-__host__ __device__ constexpr bool b_mn(int kind) { return kind == DX || kind == DW_UP || kind == DW_DOWN; }
+__host__ __device__ constexpr bool b_mn(int kind) { return kind == DH || kind == DX || kind == DW_UP || kind == DW_DOWN; }
+__host__ __device__ constexpr bool gated(int kind) { return kind == UP || kind == GATES || kind == HIDDEN; }
 __host__ __device__ constexpr int b_tile(int bn) { return bn / 2 * 64 * 2; }  // a CTA's share of B
 __host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 6 : 8; }
 __host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256; }
@@ -48,15 +53,14 @@ struct Gemm {
   CUtensorMap a0, a1, b0, b1, b2;
   int64_t rows, cols;        // of a result
   int m_tiles, n_tiles, whichs, splits;
-  int parts;                 // 6 for operands taken apart, else 1
   int k_steps, k_steps2;     // blocks of 64 of the inner axis (HIDDEN: of g and u, and of dh)
-  int pairs;                 // products summed into a tile (DX: 2)
-  int bf16, act;
-  void *out0, *out1, *out2;  // results (DW_UP: of which = 0, 1; HIDDEN: dg, du, h)
+  int blocks;                // of a tile: k_steps times the products summed into it (DX: 2)
+  int bf16;
+  void *out0, *out1, *out2;  // results (DW_UP: of which = 0, 1; HIDDEN, DH: dg, du, h; GATES: g, u)
   int64_t ld, plane;         // of the results; plane for hidden results taken apart
   int align;                 // bytes on which every row of the results starts: 32, 16 or the element's
   float* partial;            // [splits][whichs][rows][cols rounded up to 4], where splits > 1
-  const float* gate;         // HIDDEN, ReLU of fp32: g (rows, cols)
+  const float *gate, *up;    // DH: g and u, rows ld apart
   unsigned* abort_word;
   int clear_abort;
 };
@@ -64,11 +68,11 @@ struct Gemm {
 // act(g) and act'(g). For 16-bit types the fast exponential and reciprocal (a few u32, and |g| u32 for the exponential),
 // and erf by Abramowitz and Stegun 7.1.26: with z = |g|/sqrt 2 and t = 1/(1 + 0.3275911 z), erfc(z) = t (a1 + t (a2 + ...))
 // exp(-z^2) to 1.5e-7, whose exponential is the one of the derivative.
-template <bool FAST> __device__ __forceinline__ void activate(int act, float g, float& a, float& da) {
-  if (act == LNCC_ACT_RELU) {
+template <int ACT, bool FAST> __device__ __forceinline__ void activate(float g, float& a, float& da) {
+  if (ACT == LNCC_ACT_RELU) {
     a = g < 0.f ? 0.f : g;
     da = g > 0.f ? 1.f : 0.f;
-  } else if (act == LNCC_ACT_SILU) {
+  } else if (ACT == LNCC_ACT_SILU) {
     const float p = FAST ? __fdividef(1.f, 1.f + __expf(-g)) : 1.f / (1.f + expf(-g));
     a = g * p;
     da = p * (1.f + g * (1.f - p));
@@ -157,8 +161,9 @@ __device__ __forceinline__ void emit_hidden(void* base, const Gemm& g, int64_t r
   }
 }
 
+// One tile: 256 rows m, columns n, one of the results, blocks [from, to) of its inner axis.
 struct Tile {
-  int n, m, which, split;
+  int n, m, which, split, from, to;
 };
 __device__ __forceinline__ Tile tile_of(const Gemm& g, int t) {
   Tile r;
@@ -166,18 +171,22 @@ __device__ __forceinline__ Tile tile_of(const Gemm& g, int t) {
   r.m = t % g.m_tiles, t /= g.m_tiles;
   r.which = t % g.whichs;
   r.split = t / g.whichs;
+  r.from = int(int64_t(g.blocks) * r.split / g.splits);
+  r.to = int(int64_t(g.blocks) * (r.split + 1) / g.splits);
   return r;
 }
 
-// T: type of the results (for float, bf16 operands taken apart). KIND, BN: see above; UP and HIDDEN hold BN/2 columns of g
-// and of u, HIDDEN BN/2 of dh beside them.
-template <int KIND, int BN, typename T>
+// T: type of the results (for float, bf16 operands taken apart). KIND, BN: see above; gated kinds hold BN/2 columns of g
+// and of u, HIDDEN BN/2 of dh beside them. ACT: the activation of UP, HIDDEN and DH.
+template <int KIND, int BN, int ACT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Gemm g) {
   constexpr int STAGES = stages(BN), BT = b_tile(BN), HALF = BN / 2;
-  constexpr bool AM = a_mn(KIND), BM = b_mn(KIND);
-  constexpr int ACCS = KIND == HIDDEN ? 1 : 2;  // tiles of accumulators in tensor memory
-  constexpr bool FAST = sizeof(T) == 2;
-  static_assert(KIND != HIDDEN || BN == 256, "dh's share of B is one block of 64 columns a CTA");
+  constexpr bool AM = a_mn(KIND), BM = b_mn(KIND), F32 = sizeof(T) == 4;
+  constexpr int ACCS = KIND == HIDDEN ? 1 : 2;         // accumulators in tensor memory
+  constexpr int PARTS = F32 ? 6 : 1;                   // products of parts of the operands
+  constexpr int CHUNK = F32 ? kChunk : 1 << 30;        // blocks that one accumulator takes
+  static_assert(KIND != HIDDEN || (BN == 256 && !F32), "dh's share of B is one block of 64 columns a CTA");
+  static_assert(!F32 || BN == 128, "the epilogue's sums of fp32 take 64 registers");
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
   const uint32_t tiles_at = smem_addr(smem);
@@ -212,46 +221,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   fence_after();
   const uint32_t tmem = tmem_at;
   const int pairs_at_work = gridDim.x / 2, tiles = g.n_tiles * g.m_tiles * g.whichs * g.splits;
-  const int gu_steps = g.k_steps * g.parts;
-  const int dh_steps = KIND == HIDDEN ? g.k_steps2 * g.parts : 0;
-  const int all_steps = KIND == HIDDEN ? gu_steps + dh_steps : gu_steps * g.pairs;
 
   if (warp == 0 && lane == 0) {
     // ---- TMA: this CTA's shares of A and B, counted on the first CTA's barrier
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
+    const uint32_t full_of_pair = peer_addr(full, 0);
     for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
-      const int from = int(int64_t(all_steps) * w.split / g.splits), to = int(int64_t(all_steps) * (w.split + 1) / g.splits);
       const int m0 = w.m * 256 + int(rank) * 128;
-      for (int s = from; s < to; s++) {
-        if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up))) break;
-        const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile, bar = peer_addr(full + 8 * stage, 0);
-        const bool dh_phase = KIND == HIDDEN && s < dh_steps;
-        const int in = KIND == HIDDEN && !dh_phase ? s - dh_steps : s, ks = dh_phase ? g.k_steps2 : g.k_steps;
-        const int k = in % ks * 64, part = in / ks % g.parts, pair = in / ks / g.parts;
-        const int pa = g.parts > 1 ? kPlaneA[part] : 0, pb = g.parts > 1 ? kPlaneB[part] : 0;
-        if (rank == 0) mbar_expect(full + 8 * stage, 2 * (kATile + (dh_phase ? 8192 : BT)));
-        const CUtensorMap* am = dh_phase || (KIND == DX && pair) || (KIND == DW_UP && w.which) ? &g.a1 : &g.a0;
-        if (AM) {
-          tma_load(am, at, bar, m0, k, pa);
-          tma_load(am, at + kATile / 2, bar, m0 + 64, k, pa);
-        } else {
-          tma_load(am, at, bar, k, m0, pa);
-        }
-        if (dh_phase) {  // half of the tile's 128 columns of Wd, which memory holds along F
-          tma_load(&g.b2, bt, bar, w.n * HALF + int(rank) * 64, k, pb);
-        } else if (KIND == UP || KIND == HIDDEN) {  // the gate's rows in one CTA, the up projection's in the other
-          tma_load(rank ? &g.b1 : &g.b0, bt, bar, k, w.n * HALF, pb);
-        } else if (BM) {
-          const CUtensorMap* bm = KIND == DX && pair ? &g.b1 : &g.b0;
+      const CUtensorMap* a_first = KIND == DW_UP && w.which ? &g.a1 : &g.a0;
+      for (int c = w.from; c < w.to && ok; c += CHUNK) {
+        const int c_end = F32 ? min(c + CHUNK, w.to) : w.to;
+        for (int part = 0; part < PARTS && ok; part++) {
+          const int pa = F32 ? kPlaneA[part] : 0, pb = F32 ? kPlaneB[part] : 0;
+          for (int b = c; b < c_end; b++) {
+            if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up))) break;
+            const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile, bar = full_of_pair + 8 * stage;
+            const bool dh = KIND == HIDDEN && b < g.k_steps2;              // HIDDEN: dh first
+            const bool second = KIND == DX && b >= g.k_steps;              // DX: du Wu after dg Wg
+            const int k = 64 * (KIND == HIDDEN && !dh ? b - g.k_steps2 : second ? b - g.k_steps : b);
+            if (rank == 0) mbar_expect(full + 8 * stage, 2 * (kATile + (dh ? 8192 : BT)));
+            const CUtensorMap* am = dh || second ? &g.a1 : a_first;
+            if (AM) {
+              tma_load(am, at, bar, m0, k, pa);
+              tma_load(am, at + kATile / 2, bar, m0 + 64, k, pa);
+            } else {
+              tma_load(am, at, bar, k, m0, pa);
+            }
+            if (dh) {  // half of the tile's 128 columns of Wd, which memory holds along F
+              tma_load(&g.b2, bt, bar, w.n * HALF + int(rank) * 64, k, pb);
+            } else if (gated(KIND)) {  // the gate's rows in one CTA, the up projection's in the other
+              tma_load(rank ? &g.b1 : &g.b0, bt, bar, k, w.n * HALF, pb);
+            } else if (BM) {
+              const CUtensorMap* bm = second ? &g.b1 : &g.b0;
 #pragma unroll
-          for (int i = 0; i < HALF; i += 64) tma_load(bm, bt + i / 64 * 8192, bar, w.n * BN + int(rank) * HALF + i, k, pb);
-        } else {
-          tma_load(&g.b0, bt, bar, k, w.n * BN + int(rank) * HALF, pb);
+              for (int i = 0; i < HALF; i += 64) tma_load(bm, bt + i / 64 * 8192, bar, w.n * BN + int(rank) * HALF + i, k, pb);
+            } else {
+              tma_load(&g.b0, bt, bar, k, w.n * BN + int(rank) * HALF, pb);
+            }
+            if (++stage == STAGES) stage = 0, phase ^= 1;
+          }
         }
-        if (++stage == STAGES) stage = 0, phase ^= 1;
       }
     }
     // every copy has landed once its stage has been read; after giving up, copies in flight get 10 ms to land
@@ -263,82 +275,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       for (const unsigned long long start = now_ns(); now_ns() - start < 10000000ull;) __nanosleep(1000);
   } else if (warp == 1 && lane == 0 && rank == 0) {
     // ---- products of the pair
-    int stage = 0, turn = 0;
+    int stage = 0, turn = 0;  // turn counts the accumulators filled
     uint32_t phase = 0;
     bool ok = true;
     const uint32_t wide = instr_desc(g.bf16, AM, BM, BN), narrow = instr_desc(g.bf16, false, true, HALF);
-    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs_at_work, turn++) {
+    for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
-      const int from = int(int64_t(all_steps) * w.split / g.splits), to = int(int64_t(all_steps) * (w.split + 1) / g.splits);
-      const int acc = ACCS == 2 ? turn & 1 : 0;
-      const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
-      // HIDDEN: dh alternates between two places, so it may run while the last tile is read; g and u wait for that
-      const uint32_t d_dh = tmem + BN + (turn & 1) * HALF, d = tmem + (ACCS == 2 ? acc * 256 : 0);
-      if (KIND != HIDDEN) {
-        if (!(ok = mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, gave_up))) break;
-        fence_after();
-      }
-      for (int s = from; s < to; s++) {
-        const bool dh_phase = KIND == HIDDEN && s < dh_steps;
-        if (KIND == HIDDEN && s == dh_steps) {
-          if (!(ok = mbar_wait(acc_empty, acc_phase ^ 1, gave_up))) break;
+      for (int c = w.from; c < w.to && ok; c += CHUNK, turn++) {
+        const int steps = (F32 ? min(CHUNK, w.to - c) : w.to - c) * PARTS;
+        const int acc = ACCS == 2 ? turn & 1 : 0;
+        const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
+        // HIDDEN: dh alternates between two places, so it may run while the last tile is read; g and u wait for that
+        const uint32_t d_dh = tmem + BN + (turn & 1) * HALF, d = tmem + (ACCS == 2 ? acc * 256 : 0);
+        if (KIND != HIDDEN) {
+          if (!(ok = mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, gave_up))) break;
           fence_after();
         }
-        if (!(ok = mbar_wait(full + 8 * stage, phase, gave_up))) break;
-        fence_after();
-        const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile;
-        const uint64_t da = AM ? desc_mn(at, 8192) : desc_k(at);
-        const uint64_t db = BM || dh_phase ? desc_mn(bt, 8192) : desc_k(bt);
-        const uint64_t a_step = AM ? 128 : 2, b_step = BM || dh_phase ? 128 : 2;
+        for (int s = 0; s < steps; s++) {
+          const bool dh = KIND == HIDDEN && s < g.k_steps2;
+          if (KIND == HIDDEN && s == g.k_steps2) {
+            if (!(ok = mbar_wait(acc_empty, acc_phase ^ 1, gave_up))) break;
+            fence_after();
+          }
+          if (!(ok = mbar_wait(full + 8 * stage, phase, gave_up))) break;
+          fence_after();
+          const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile;
+          const uint64_t da = AM ? desc_mn(at, 8192) : desc_k(at);
+          const uint64_t db = BM || dh ? desc_mn(bt, 8192) : desc_k(bt);
+          const uint64_t a_step = AM ? 128 : 2, b_step = BM || dh ? 128 : 2;
+          const bool first = s == 0 || (KIND == HIDDEN && s == g.k_steps2);
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-          mma(dh_phase ? d_dh : d, da + k * a_step, db + k * b_step, dh_phase ? narrow : wide,
-              k > 0 || (dh_phase ? s > 0 : s > (KIND == HIDDEN ? dh_steps : from)));
-        commit_pair(empty + 8 * stage);
-        if (++stage == STAGES) stage = 0, phase ^= 1;
+          for (int k = 0; k < 4; k++)
+            mma(dh ? d_dh : d, da + k * a_step, db + k * b_step, dh ? narrow : wide, k > 0 || !first);
+          commit_pair(empty + 8 * stage);
+          if (++stage == STAGES) stage = 0, phase ^= 1;
+        }
+        if (ok) commit_pair(acc_full + 8 * acc);
       }
-      if (ok) commit_pair(acc_full + 8 * acc);
     }
   } else if (warp >= 4) {
     // ---- epilogue: lanes are rows; two warps share a row, half of the columns each
     const int sub = warp & 3, half = (warp - 4) / 4;
+    constexpr int COLS = gated(KIND) ? HALF / 2 : HALF;  // columns of a result that a warp takes
+    const float nan = __int_as_float(0x7fffffff);
     int turn = 0;
-    for (int t = blockIdx.x / 2; t < tiles; t += pairs_at_work, turn++) {
+    for (int t = blockIdx.x / 2; t < tiles; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
-      const int acc = ACCS == 2 ? turn & 1 : 0;
-      const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_phase, gave_up));
-      fence_after();
-      const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (ACCS == 2 ? acc * 256 : 0);
       const int64_t row = int64_t(w.m) * 256 + rank * 128 + sub * 32 + lane;
-      const float nan = __int_as_float(0x7fffffff);
-      if constexpr (KIND == UP || KIND == HIDDEN) {
-#pragma unroll 1
-        for (int c = half * (HALF / 2); c < (half + 1) * (HALF / 2); c += 16) {
-          const int64_t col = int64_t(w.n) * HALF + c;
-          __syncwarp();
-          uint32_t vg[16], vu[16], vd[16];
-          if (ok) {
-            tmem_load(d + c, vg);
-            tmem_load(d + HALF + c, vu);
-            if (KIND == HIDDEN) tmem_load(d + BN + (turn & 1) * HALF + c, vd);
-            wait_ld(vg);
-            wait_ld(vu);
-            if (KIND == HIDDEN) wait_ld(vd);
-          }
+      const int64_t col0 = int64_t(w.n) * (gated(KIND) ? HALF : BN) + half * COLS;
+
+      // 16 columns: v0 (g, or the product), v1 (u), v2 (dh) as fp32
+      const auto finish = [&](int64_t col, const float (&v0)[16], const float (&v1)[16], const float (&v2)[16]) {
+        if (row >= g.rows || col >= g.cols) return;
+        if constexpr (KIND == UP || KIND == HIDDEN) {
           float h[16], dg[16], du[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            float gate = ok ? __uint_as_float(vg[i]) : nan, a, da;
-            const float up = ok ? __uint_as_float(vu[i]) : nan;
-            if (KIND == HIDDEN && !FAST && g.gate && row < g.rows && col + i < g.cols) gate = g.gate[row * g.cols + col + i];
-            activate<FAST>(g.act, gate, a, da);
-            h[i] = a * up;
-            if (KIND == HIDDEN) {
-              const float dh = ok ? __uint_as_float(vd[i]) : nan;
-              dg[i] = dh * up * da;
-              du[i] = dh * a;
-            }
+            float a, da;
+            activate<ACT, !F32>(v0[i], a, da);
+            h[i] = a * v1[i];
+            dg[i] = v2[i] * v1[i] * da;
+            du[i] = v2[i] * a;
           }
           if (KIND == HIDDEN) {
             emit_hidden<T>(g.out0, g, row, col, dg);
@@ -347,36 +344,98 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           } else {
             emit_hidden<T>(g.out0, g, row, col, h);
           }
+        } else if constexpr (KIND == DH) {
+          float h[16], dg[16], du[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const bool in = col + i < g.cols;
+            const float gate = in ? g.gate[row * g.ld + col + i] : 0.f, up = in ? g.up[row * g.ld + col + i] : 0.f;
+            float a, da;
+            activate<ACT, !F32>(gate, a, da);
+            h[i] = a * up;
+            dg[i] = v0[i] * up * da;
+            du[i] = v0[i] * a;
+          }
+          emit_hidden<T>(g.out0, g, row, col, dg);
+          emit_hidden<T>(g.out1, g, row, col, du);
+          emit_hidden<T>(g.out2, g, row, col, h);
+        } else if constexpr (KIND == GATES) {
+          if (!LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) return;
+          emit<float>(static_cast<float*>(g.out0), g.ld, row, col, g.cols, g.align, v0);
+          emit<float>(static_cast<float*>(g.out1), g.ld, row, col, g.cols, g.align, v1);
+        } else if (g.splits > 1) {
+          const int64_t ld = (g.cols + 3) / 4 * 4;
+          emit<float>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row, col, ld, 16, v0);
+        } else if (LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) {
+          T o[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[i] = from_f<T>(v0[i]);
+          emit<T>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row, col, g.cols, g.align, o);
+        }
+      };
+      const auto done = [&](int acc) {  // this warp has read the accumulator
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty + 8 * acc, 0));
+      };
+
+      if constexpr (F32) {
+        float sum[4][16];
+#pragma unroll
+        for (int i = 0; i < 64; i++) sum[i / 16][i % 16] = 0.f;
+        for (int c = w.from; c < w.to; c += CHUNK, turn++) {
+          const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * (turn & 1), (turn >> 1) & 1, gave_up));
+          fence_after();
+          const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (turn & 1) * 256 + half * COLS;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {  // gated: 32 columns of g and 32 of u, else 64 of the product
+            uint32_t v[16];
+            if (ok) {
+              tmem_load(d + (gated(KIND) ? i / 2 * HALF + i % 2 * 16 : i * 16), v);
+              wait_ld(v);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; j++) sum[i][j] += ok ? __uint_as_float(v[j]) : nan;
+          }
+          done(turn & 1);
+        }
+        if (gated(KIND)) {
+          finish(col0, sum[0], sum[2], sum[2]);
+          finish(col0 + 16, sum[1], sum[3], sum[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; i++) finish(col0 + i * 16, sum[i], sum[i], sum[i]);
         }
       } else {
+        const int acc = ACCS == 2 ? turn & 1 : 0;
+        const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
+        const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_phase, gave_up));
+        fence_after();
+        const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (ACCS == 2 ? acc * 256 : 0) + half * COLS;
 #pragma unroll 1
-        for (int c = half * HALF; c < (half + 1) * HALF; c += 16) {
-          const int64_t col = int64_t(w.n) * BN + c;
+        for (int c = 0; c < COLS; c += 16) {
           __syncwarp();
-          uint32_t v[16];
+          uint32_t v[3][16];
           if (ok) {
-            tmem_load(d + c, v);
-            wait_ld(v);
+            tmem_load(d + c, v[0]);
+            if (gated(KIND)) tmem_load(d + HALF + c, v[1]);
+            if (KIND == HIDDEN) tmem_load(d + BN + (turn & 1) * HALF + c, v[2]);
+            wait_ld(v[0]);
+            if (gated(KIND)) wait_ld(v[1]);
+            if (KIND == HIDDEN) wait_ld(v[2]);
           }
-          if (row < g.rows && col < g.cols) {
-            if (g.splits > 1) {
-              const int64_t ld = (g.cols + 3) / 4 * 4;
-              float o[16];
+          if (c + 16 == COLS) done(acc);
+          float f[3][16];
 #pragma unroll
-              for (int i = 0; i < 16; i++) o[i] = ok ? __uint_as_float(v[i]) : nan;
-              emit<float>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row, col, ld, 16, o);
-            } else if (LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) {
-              T o[16];
-#pragma unroll
-              for (int i = 0; i < 16; i++) o[i] = from_f<T>(ok ? __uint_as_float(v[i]) : nan);
-              emit<T>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row, col, g.cols, g.align, o);
-            }
+          for (int i = 0; i < 16; i++) {
+            f[0][i] = ok ? __uint_as_float(v[0][i]) : nan;
+            f[1][i] = ok ? __uint_as_float(v[gated(KIND) ? 1 : 0][i]) : nan;
+            f[2][i] = ok ? __uint_as_float(v[KIND == HIDDEN ? 2 : 0][i]) : nan;
           }
+          finish(col0 + c, f[0], f[1], f[2]);
         }
+        turn++;
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty + 8 * acc, 0));
     }
   }
   __syncwarp();
@@ -386,25 +445,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Partial sums of the splits, added in order.
+// Partial sums of the splits: eight strands of splits for each 32 quads of columns, then the strands, each in order.
 template <typename T>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int whichs, int64_t rows,
                                                    int64_t cols, T* out0, T* out1) {
-  const int64_t ld = (cols + 3) / 4 * 4, quads = whichs * rows * (ld / 4), slab = whichs * rows * ld;
-  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < quads; q += int64_t(gridDim.x) * 256) {
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < splits; i++) {
-      const float4 v = *reinterpret_cast<const float4*>(partial + i * slab + q * 4);
+  __shared__ float4 meet[8][32];
+  const int strand = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t ld = (cols + 3) / 4 * 4, quads = whichs * rows * (ld / 4), q = int64_t(blockIdx.x) * 32 + lane;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (q < quads) {
+#pragma unroll 4
+    for (int i = strand; i < splits; i += 8) {
+      const float4 v = reinterpret_cast<const float4*>(partial)[i * quads + q];
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const int64_t row = q / (ld / 4) % rows, col = q % (ld / 4) * 4;
-    T* out = q / (ld / 4) / rows ? out1 : out0;
-    if (out == nullptr) continue;
-    const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) out[row * cols + col + i] = from_f<T>(v[i]);
   }
+  meet[strand][lane] = s;
+  __syncthreads();
+  if (strand != 0 || q >= quads) return;
+  for (int i = 1; i < 8; i++) {
+    const float4 v = meet[i][lane];
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  const int64_t row = q / (ld / 4) % rows, col = q % (ld / 4) * 4;
+  T* out = q / (ld / 4) / rows ? out1 : out0;
+  if (out == nullptr) return;
+  const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) out[row * cols + col + i] = from_f<T>(v[i]);
 }
 
 // A matrix that TMA cannot read as it lies (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows.
@@ -429,33 +498,51 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, in
 }
 
 // g = x Wg^T by fp32 multiply-adds in the order of k, for the backward pass of ReLU in fp32 alone: the derivative jumps at
-// g = 0, where the last bit of g decides, so g is the plain fp32 sum there.
-constexpr int kTile = 64, kInner = 16;
-__global__ void __launch_bounds__(256) gate_kernel(const float* x, int64_t x_stride, const float* w, float* out, int64_t M,
-                                                   int64_t N, int64_t K) {
-  __shared__ float sa[kInner][kTile + 1], sb[kInner][kTile + 1];
+// g = 0, where the last bit of g decides, so g is the plain fp32 sum there. A block takes 128 x 128, a thread 8 x 8 of it,
+// 16 of k at a time through shared memory; the next 16 are loaded while these are summed.
+constexpr int kTile = 128, kInner = 16;
+__global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ x, int64_t x_stride,
+                                                   const float* __restrict__ w, float* out, int64_t ld, int64_t M, int64_t N,
+                                                   int64_t K) {
+  __shared__ __align__(16) float sa[kInner][kTile + 4], sb[kInner][kTile + 4];
   const int64_t m0 = int64_t(blockIdx.x) * kTile, n0 = int64_t(blockIdx.y) * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += kInner) {
-    for (int i = threadIdx.x; i < kTile * kInner; i += 256) {
-      const int r = i / kInner, k = i % kInner;
-      sa[k][r] = m0 + r < M && k0 + k < K ? x[(m0 + r) * x_stride + k0 + k] : 0.f;
-      sb[k][r] = n0 + r < N && k0 + k < K ? w[(n0 + r) * K + k0 + k] : 0.f;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // also: column of k, and first row, of the thread's loads
+  float acc[8][8] = {}, la[8], lb[8];
+  const auto load = [&](int64_t k) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int64_t r = ty + 16 * i;
+      la[i] = m0 + r < M && k + tx < K ? x[(m0 + r) * x_stride + k + tx] : 0.f;
+      lb[i] = n0 + r < N && k + tx < K ? w[(n0 + r) * K + k + tx] : 0.f;
     }
+  };
+  load(0);
+  for (int64_t k0 = 0; k0 < K; k0 += kInner) {
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kInner; k++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) acc[i][j] += sa[k][ty * 4 + i] * sb[k][tx * 4 + j];
+    for (int i = 0; i < 8; i++) sa[tx][ty + 16 * i] = la[i], sb[tx][ty + 16 * i] = lb[i];
     __syncthreads();
+    load(k0 + kInner);
+#pragma unroll
+    for (int k = 0; k < kInner; k++) {
+      float a[8], b[8];
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        *reinterpret_cast<float4*>(a + i) = *reinterpret_cast<const float4*>(&sa[k][ty * 4 + i * 16]);
+        *reinterpret_cast<float4*>(b + i) = *reinterpret_cast<const float4*>(&sb[k][tx * 4 + i * 16]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+    }
   }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m < M && n < N && LNCC_IN(m * N + n, 1, M * N)) out[m * N + n] = acc[i][j];
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int64_t m = m0 + ty * 4 + i % 4 + i / 4 * 64, n = n0 + tx * 4 + j % 4 + j / 4 * 64;
+      if (m < M && n < N && LNCC_IN(m * ld + n, 1, M * ld)) out[m * ld + n] = acc[i][j];
     }
 }
 
@@ -476,21 +563,21 @@ inline int64_t lead(int64_t cols) { return (cols + 15) / 16 * 16; }  // rows of 
 struct Cut {
   int bn, m_tiles, n_tiles, splits;
 };
-static Cut cut_for(int kind, int64_t rows, int64_t cols, int whichs, int64_t steps) {
+static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
   const int pairs = sm_count() / 2;
-  const bool gated = kind == UP || kind == HIDDEN;
   Cut c;
   c.m_tiles = int(ceil_div(rows, 256));
   c.bn = 256;
-  c.n_tiles = int(ceil_div(cols, gated ? 128 : 256));
-  if (kind != HIDDEN && (int64_t(c.m_tiles) * c.n_tiles * whichs < pairs || cols <= (gated ? 64 : 128))) {
+  c.n_tiles = int(ceil_div(cols, gated(kind) ? 128 : 256));
+  if (dtype == LNCC_F32 ||
+      (kind != HIDDEN && (int64_t(c.m_tiles) * c.n_tiles * whichs < pairs || cols <= (gated(kind) ? 64 : 128)))) {
     c.bn = 128;
-    c.n_tiles = int(ceil_div(cols, gated ? 64 : 128));
+    c.n_tiles = int(ceil_div(cols, gated(kind) ? 64 : 128));
   }
   c.splits = 1;
   const int64_t tiles = int64_t(c.m_tiles) * c.n_tiles * whichs;
-  if (!gated && tiles <= pairs / 2) {  // at least 8 steps for each split
-    const int64_t want = pairs / tiles, most = steps / 8;
+  if (!gated(kind) && kind != DH && tiles <= pairs / 2) {  // at least 8 blocks for each split
+    const int64_t want = pairs / tiles, most = blocks / 8;
     c.splits = int(want < most ? want : most);
     if (c.splits < 1) c.splits = 1;
   }
@@ -499,19 +586,18 @@ static Cut cut_for(int kind, int64_t rows, int64_t cols, int whichs, int64_t ste
 
 // Scratch of a call, laid out in one place for its size and its use.
 struct Plan {
-  int parts, planes;
-  size_t x, wg, wu, wd, dy, h, dg, du, gate, partial, total;
+  int planes;
+  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, partial, total;
   int64_t ldf;
 };
-static size_t partial_bytes(int kind, int64_t rows, int64_t cols, int whichs, int64_t steps) {
-  const Cut c = cut_for(kind, rows, cols, whichs, steps);
+static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
+  const Cut c = cut_for(kind, dtype, rows, cols, whichs, blocks);
   return c.splits > 1 ? size_t(c.splits) * whichs * rows * ((cols + 3) / 4 * 4) * 4 : 0;
 }
 static int64_t k_steps(int64_t k) { return ceil_div(k, 64); }
 static Plan plan_for(const Args& a, bool backward) {
   Plan p = {};
   p.planes = a.dtype == LNCC_F32 ? 3 : 1;
-  p.parts = a.dtype == LNCC_F32 ? 6 : 1;
   p.ldf = lead(a.F);
   size_t at = kHeader;
   const auto take = [&](int64_t rows, int64_t ld) {
@@ -530,13 +616,16 @@ static Plan plan_for(const Args& a, bool backward) {
     p.dy = take(a.M, lead(a.N));
     p.dg = take(a.M, p.ldf);
     p.du = take(a.M, p.ldf);
-    p.gate = at;
-    if (a.dtype == LNCC_F32 && a.act == LNCC_ACT_RELU) at += round_up(size_t(a.M) * a.F * 4);
-    partial(partial_bytes(DX, a.M, a.K, 1, 2 * p.parts * k_steps(a.F)));
-    partial(partial_bytes(DW_UP, a.F, a.K, 2, p.parts * k_steps(a.M)));
-    partial(partial_bytes(DW_DOWN, a.N, a.F, 1, p.parts * k_steps(a.M)));
+    if (a.dtype == LNCC_F32) {
+      p.gate = at, at += round_up(size_t(a.M) * p.ldf * 4);
+      p.up = at, at += round_up(size_t(a.M) * p.ldf * 4);
+    }
+    partial(partial_bytes(DX, a.dtype, a.M, a.K, 1, 2 * k_steps(a.F)));
+    partial(partial_bytes(DW_UP, a.dtype, a.F, a.K, 2, k_steps(a.M)));
+    partial(partial_bytes(DW_UP, a.dtype, a.F, a.K, 1, k_steps(a.M)));
+    partial(partial_bytes(DW_DOWN, a.dtype, a.N, a.F, 1, k_steps(a.M)));
   } else {
-    partial(partial_bytes(DOWN, a.M, a.N, 1, p.parts * k_steps(a.F)));
+    partial(partial_bytes(DOWN, a.dtype, a.M, a.N, 1, k_steps(a.F)));
   }
   p.partial = at;
   p.total = at + round_up(most);
@@ -579,20 +668,30 @@ struct Call {
     return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.planes, a.dtype != LNCC_F16};
   }
 
-  template <int KIND, int BN, typename T> void launch(Gemm& g) {
+  template <int KIND, int BN, int ACT, typename T> void launch(Gemm& g) {
     const int smem = smem_bytes(BN), pairs = sm_count() / 2;
-    if (cudaFuncSetAttribute(product_kernel<KIND, BN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    if (cudaFuncSetAttribute(product_kernel<KIND, BN, ACT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+        cudaSuccess) {
       cudaGetLastError();
       status = LNCC_ERR_SMEM;
       return;
     }
     const int64_t tiles = int64_t(g.m_tiles) * g.n_tiles * g.whichs * g.splits;
-    product_kernel<KIND, BN, T><<<unsigned(2 * (tiles < pairs ? tiles : pairs)), kThreads, smem, stream>>>(g);
+    product_kernel<KIND, BN, ACT, T><<<unsigned(2 * (tiles < pairs ? tiles : pairs)), kThreads, smem, stream>>>(g);
   }
-  template <int KIND, typename T> void launch_bn(Gemm& g, int bn) {
-    if constexpr (KIND == HIDDEN) launch<KIND, 256, T>(g);
-    else if (bn == 256) launch<KIND, 256, T>(g);
-    else launch<KIND, 128, T>(g);
+  template <int KIND, int BN, typename T> void launch_act(Gemm& g) {
+    if constexpr (KIND == UP || KIND == HIDDEN || KIND == DH) {
+      if (a.act == LNCC_ACT_SILU) launch<KIND, BN, LNCC_ACT_SILU, T>(g);
+      else if (a.act == LNCC_ACT_GELU) launch<KIND, BN, LNCC_ACT_GELU, T>(g);
+      else launch<KIND, BN, LNCC_ACT_RELU, T>(g);
+    } else {
+      launch<KIND, BN, 0, T>(g);
+    }
+  }
+  template <int KIND, typename T> void launch_type(Gemm& g, int bn) {
+    if constexpr (KIND == HIDDEN) launch_act<KIND, 256, T>(g);
+    else if (bn == 256) launch_act<KIND, 256, T>(g);
+    else launch_act<KIND, 128, T>(g);
   }
 
   // One product: A (a0, a1) and B (b0, b1, b2) as the kind takes them, results out (rows x cols, ld apart).
@@ -602,11 +701,10 @@ struct Call {
                int64_t plane) {
     if (status != LNCC_OK) return;
     Gemm g = {};
-    g.parts = plan.parts;
     g.k_steps = int(k_steps(inner));
     g.k_steps2 = int(k_steps(inner2));
-    g.pairs = KIND == DX ? 2 : 1;
-    const Cut c = cut_for(KIND, rows, cols, whichs, int64_t(g.pairs) * g.parts * g.k_steps);
+    g.blocks = KIND == DX ? 2 * g.k_steps : KIND == HIDDEN ? g.k_steps + g.k_steps2 : g.k_steps;
+    const Cut c = cut_for(KIND, a.dtype, rows, cols, whichs, g.blocks);
     g.m_tiles = c.m_tiles, g.n_tiles = c.n_tiles, g.splits = c.splits, g.whichs = whichs;
     const int a_box = a_mn(KIND) ? 64 : 128, b_box = b_mn(KIND) ? 64 : c.bn / 2;
     if (!make_map(&g.a0, a0, a_box) || !make_map(&g.a1, a1, a_box) || !make_map(&g.b0, b0, b_box) ||
@@ -614,24 +712,29 @@ struct Call {
       status = LNCC_ERR_CUDA;
       return;
     }
-    g.rows = rows, g.cols = cols, g.bf16 = a0.bf16, g.act = a.act;
+    g.rows = rows, g.cols = cols, g.bf16 = a0.bf16;
     g.out0 = out0, g.out1 = out1, g.out2 = out2, g.ld = ld, g.plane = plane;
-    const int es = KIND == UP || KIND == HIDDEN ? 2 : elem_size(a.dtype);
+    const int es = KIND == UP || KIND == HIDDEN || KIND == DH ? 2 : elem_size(a.dtype);
     g.align = es;
     for (int al = 16; al <= 32; al *= 2)
       if (aligned(out0, al) && aligned(out1, al) && aligned(out2, al) && ld * es % al == 0) g.align = al;
     g.partial = reinterpret_cast<float*>(scratch + plan.partial);
-    g.gate = KIND == HIDDEN && a.dtype == LNCC_F32 && a.act == LNCC_ACT_RELU
-                 ? reinterpret_cast<const float*>(scratch + plan.gate) : nullptr;
+    g.gate = reinterpret_cast<const float*>(scratch + plan.gate);
+    g.up = reinterpret_cast<const float*>(scratch + plan.up);
     g.abort_word = reinterpret_cast<unsigned*>(scratch);
     g.clear_abort = first;
     first = false;
-    if (a.dtype == LNCC_F32) launch_bn<KIND, float>(g, c.bn);
-    else if (a.dtype == LNCC_BF16) launch_bn<KIND, __nv_bfloat16>(g, c.bn);
-    else launch_bn<KIND, __half>(g, c.bn);
+    if constexpr (KIND == GATES || KIND == DH) {
+      launch_act<KIND, 128, float>(g);
+    } else if (a.dtype == LNCC_F32) {
+      if constexpr (KIND != HIDDEN) launch_act<KIND, 128, float>(g);
+    } else if (a.dtype == LNCC_BF16) {
+      launch_type<KIND, __nv_bfloat16>(g, c.bn);
+    } else {
+      launch_type<KIND, __half>(g, c.bn);
+    }
     if (g.splits > 1 && status == LNCC_OK) {
-      const int64_t blocks = ceil_div(whichs * rows * ceil_div(cols, 4), 256), most = int64_t(sm_count()) * 8;
-      const unsigned grid = unsigned(blocks < most ? blocks : most);
+      const unsigned grid = unsigned(ceil_div(whichs * rows * ceil_div(cols, 4), 32));
       if (a.dtype == LNCC_F32)
         join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<float*>(out0),
                                               static_cast<float*>(out1));
@@ -662,11 +765,16 @@ static int backward(const Args& a, void* scratch, cudaStream_t stream) {
                wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg), wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu),
                wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd);
   const Matrix h = c.hidden(c.plan.h), dg = c.hidden(c.plan.dg), du = c.hidden(c.plan.du);
-  if (a.dtype == LNCC_F32 && a.act == LNCC_ACT_RELU)
-    gate_kernel<<<dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, stream>>>(
-        static_cast<const float*>(a.x), a.x_stride, static_cast<const float*>(a.wg),
-        reinterpret_cast<float*>(c.scratch + c.plan.gate), a.M, a.F, a.K);
-  c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
+  if (a.dtype == LNCC_F32) {
+    float* const gate = reinterpret_cast<float*>(c.scratch + c.plan.gate);
+    c.product<GATES>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, gate, c.scratch + c.plan.up, nullptr, h.ld, 0);
+    if (a.act == LNCC_ACT_RELU)
+      gate_kernel<<<dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, stream>>>(
+          static_cast<const float*>(a.x), a.x_stride, static_cast<const float*>(a.wg), gate, h.ld, a.M, a.F, a.K);
+    c.product<DH>(dy, dy, wd, wd, wd, a.M, a.F, 1, a.N, 0, dg.p, du.p, h.p, h.ld, h.plane);
+  } else {
+    c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
+  }
   if (a.dx) c.product<DX>(dg, du, wg, wu, wg, a.M, a.K, 1, a.F, 0, a.dx, nullptr, nullptr, a.K, 0);
   if (a.dwg || a.dwu) {
     // one product for both where both are wanted
