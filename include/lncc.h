@@ -325,7 +325,7 @@ int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, i
  *   state    : NULL (zeros) or (B, C).
  *   h        : (B, T, C) contiguous.        last: (B, C), the state after the last step taken (T == 0: state).
  *   kept     : NULL, or lncc_gated_scan_kept_bytes(...) bytes that receive the states the backward pass starts from.
- * Limits: B <= 65535, T <= 65535 * 64, C <= 2^24 (LNCC_ERR_TOO_LARGE).
+ * Limits: B <= 65535, T <= 2^30, C <= 2^24 (LNCC_ERR_TOO_LARGE).
  */
 size_t lncc_gated_scan_kept_bytes(int64_t B, int64_t T, int64_t C);
 size_t lncc_gated_scan_scratch_bytes(int64_t B, int64_t T, int64_t C);
