@@ -1,4 +1,5 @@
-"""Build liblncc_sm100.so (the C-ABI CUDA library) in-tree for sm_100a.
+"""Build liblncc_sm100.so (the C-ABI CUDA library) in-tree for sm_100a, and libfused_lncc_torch.so, the torch operators of the
+token blocks over it.
 
 Usage: python fused-lncc_b200/build.py [--force] [--checked]
 
@@ -27,6 +28,7 @@ LIB_DIR = os.path.join(PKG_ROOT, "fused_lncc")
 LIB_NAME = "liblncc_sm100.so"
 LIB_PATH = os.path.join(LIB_DIR, LIB_NAME)
 CHECKED_LIB_PATH = os.path.join(LIB_DIR, "liblncc_sm100_checked.so")
+TORCH_OPS_PATH = os.path.join(LIB_DIR, "libfused_lncc_torch.so")  # torch's view of the token-block operators
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -70,7 +72,7 @@ def _run(cmd, out, verbose):
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed building {out}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed building {out}:\n{r.stdout}\n{r.stderr}")
 
 
 def build_library(force=False, checked=False, verbose=False, out=None):
@@ -99,6 +101,26 @@ def build_library(force=False, checked=False, verbose=False, out=None):
     return out
 
 
+def build_torch_ops(force=False, verbose=False):
+    """Compile csrc/torch_ops.cpp against the torch that is installed and the library beside it; return its path."""
+    out, src = TORCH_OPS_PATH, os.path.join(CSRC, "torch_ops.cpp")
+    lib = build_library(verbose=verbose)
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(map(os.path.getmtime, _includes(src))):
+        return out
+    import torch
+    torch_dir = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc_path())) or "/usr/local/cuda"
+    includes = [INCLUDE, os.path.join(torch_dir, "include"),
+                os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in includes),
+           "-o", out + ".tmp", src, f"-L{LIB_DIR}", f"-l:{os.path.basename(lib)}", f"-L{os.path.join(torch_dir, 'lib')}",
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]
+    _run(cmd, out, verbose)
+    os.replace(out + ".tmp", out)
+    return out
+
+
 if __name__ == "__main__":
     ap = argparse.ArgumentParser()
     ap.add_argument("--force", action="store_true")
@@ -106,4 +128,6 @@ if __name__ == "__main__":
     args = ap.parse_args()
     p = build_library(force=args.force, checked=args.checked, verbose=True)
     print(p)
+    if not args.checked:
+        print(build_torch_ops(force=args.force, verbose=True))
     sys.exit(0)

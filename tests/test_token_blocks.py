@@ -161,6 +161,6 @@ def test_ffn_backward_rejects_bad_arguments(lib, kw, status):
 
 
 def test_kept_size_is_the_bindings(lib):
-    from fused_lncc import gated_scan
+    from fused_lncc import _native
     for B, T, C in ((1, 1, 1), (2, 16, 5), (3, 17, 8), (1, 1000, 33)):
-        assert lib.lncc_gated_scan_kept_bytes(B, T, C) == 4 * gated_scan._kept_numel(B, T, C)
+        assert lib.lncc_gated_scan_kept_bytes(B, T, C) == 4 * _native.kept_numel(B, T, C)
