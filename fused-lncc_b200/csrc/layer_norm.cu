@@ -6,12 +6,16 @@
 // A row lives in the registers of LANES threads, 16 elements each, from its one load to its one store: the mean and
 // then the centred squares are summed in fp32 without a second read (the two-step variance does not cancel). LANES is
 // the smallest power of two whose registers hold the row, so a warp takes 8 rows of 64 or one of 512, and a block one of
-// up to 16384. Both directions are bound by their bytes; thread blocks stay and walk over the rows, so that the weight
-// is loaded once and, backward, each thread keeps the fp32 sums of dw and db of its own columns. The next row's loads
-// are issued before the present row is reduced. The sums of the threads of a block meet in shared memory and those of the
-// blocks in a second kernel, each in a fixed order: the gradients are the same bits run after run.
-// Rows wider than 16384 take the looping kernels at the end of this file, which read a row again for each step.
+// up to 8192. Both directions are bound by their bytes; thread blocks stay and walk over the rows, so that the weight
+// is loaded once and, backward, each thread keeps the fp32 sums of dw and db of its own columns. The next three rows are
+// under way meanwhile, copied asynchronously into shared memory that only the thread itself reads (so no barrier waits for
+// them): with one row ahead in registers 24 KB an SM were in flight, and the forward pass took 60 us where its bytes
+// take 25 (107520 x 384 bf16). The sums of the threads of a block meet in shared memory and those of the blocks in a
+// second kernel, each in a fixed order: the gradients are the same bits run after run.
+// Rows wider than 8192 take the looping kernels at the end of this file, which read a row again for each step.
 #include "lncc_block.cuh"
+
+#include <type_traits>
 
 namespace lncc {
 namespace norm {
@@ -20,7 +24,7 @@ using namespace blk;
 
 constexpr int kElems = 16;       // elements of a row that one thread holds
 constexpr int kThreads = 256;    // threads of a block (LANES where that is more)
-constexpr int kMaxWidth = 16384; // widest row that 1024 threads hold
+constexpr int kMaxWidth = 8192;  // widest row that 512 threads hold
 
 struct Args {
   const void* x;
@@ -63,33 +67,84 @@ template <int LANES> __device__ __forceinline__ float row_sum(float v, float* re
   return v;
 }
 
-// One thread's share of a row, as it lies in memory: NV vectors of VEC elements, vector v at column (v*LANES + lane)*VEC.
-template <typename T, int LANES, int VEC> struct Share {
-  static constexpr int NV = kElems / VEC;
-  Vec<T, VEC> raw[NV];
-  __device__ __forceinline__ void load(const T* row, int lane, int width, bool live) {
+// One thread's shares of the rows to come: NV vectors of VEC elements each, vector v at column (v*LANES + lane)*VEC. A ring
+// of rows in shared memory, filled by asynchronous copies of 4 or 16 bytes; single 16-bit elements, which have
+// none, wait in registers instead, one row ahead.
+template <typename T, int LANES, int VEC, int THREADS> struct Rows {
+  static constexpr int NV = kElems / VEC, BYTES = VEC * int(sizeof(T));
+  static constexpr int kStages = sizeof(T) == 4 ? 3 : 4;  // at most 48 KB a ring for 256 threads
+  static constexpr bool ASYNC = BYTES >= 4;
+  typedef Vec<T, VEC> V;
+  struct Empty {};
+  typename std::conditional<ASYNC, Empty, V[NV]>::type held;
+  const T* base;
+  int64_t stride, rows;
+  int width, lane;
+  V* ring;  // this thread's vector 0 of stage 0
+  int in, out;
+
+  __host__ __device__ static constexpr int smem() { return ASYNC ? kStages * NV * THREADS * BYTES : 0; }
+  __device__ __forceinline__ Rows(const void* p, int64_t stride_, int64_t rows_, int width_, int lane_, void* smem_at)
+      : base(static_cast<const T*>(p)), stride(stride_), rows(rows_), width(width_), lane(lane_),
+        ring(static_cast<V*>(smem_at) + threadIdx.x), in(0), out(0) {}
+  // begin to fetch a row (past the end: zeros)
+  __device__ __forceinline__ void fetch(int64_t row) {
+    const T* from = base + (row < rows ? row * stride : 0);
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = (v * LANES + lane) * VEC;
-      if (live && c < width && LNCC_IN(c, VEC, width)) {
-        raw[v] = *reinterpret_cast<const Vec<T, VEC>*>(row + c);
+      const bool live = row < rows && c < width && LNCC_IN(c, VEC, width);
+      if constexpr (ASYNC) {
+        const uint32_t dst = uint32_t(__cvta_generic_to_shared(ring + (in * NV + v) * THREADS));
+        const T* src = live ? from + c : base;
+        const int bytes = live ? BYTES : 0;  // what is not copied is zero
+        if constexpr (BYTES == 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
       } else {
 #pragma unroll
-        for (int i = 0; i < VEC; i++) raw[v].e[i] = from_f<T>(0.f);
+        for (int i = 0; i < VEC; i++) held[v].e[i] = live ? from[c + i] : from_f<T>(0.f);
       }
     }
+    in = in + 1 == kStages ? 0 : in + 1;
   }
-  __device__ __forceinline__ float get(int v, int i) const { return to_f(raw[v].e[i]); }
+  // the oldest row fetched, as floats
+  __device__ __forceinline__ void take(float (&f)[kElems]) {
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+      V r;
+      if constexpr (ASYNC) r = ring[(out * NV + v) * THREADS];
+      else r = held[v];
+#pragma unroll
+      for (int i = 0; i < VEC; i++) f[v * VEC + i] = to_f(r.e[i]);
+    }
+    out = out + 1 == kStages ? 0 : out + 1;
+  }
 };
+__device__ __forceinline__ void close_fetch() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER> __device__ __forceinline__ void wait_fetch() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
+
+template <int LANES> __host__ __device__ constexpr int threads_of() { return LANES > kThreads ? LANES : kThreads; }
 
 template <typename T, int LANES, int VEC>
-__global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) forward_kernel(const Args a) {
+__global__ void __launch_bounds__(threads_of<LANES>(), LANES > kThreads ? 1 : VEC * sizeof(T) >= 4 ? 3 : 2) forward_kernel(const Args a) {
   constexpr int THREADS = LANES > kThreads ? LANES : kThreads;
   constexpr int ROWS = THREADS / LANES, NV = kElems / VEC;
+  typedef Rows<T, LANES, VEC, THREADS> R;
+  constexpr int AHEAD = R::ASYNC ? R::kStages - 1 : 1;
+  extern __shared__ __align__(16) unsigned char stage[];
   __shared__ float red[2][THREADS / 32];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.y);
+  const int64_t step = int64_t(gridDim.x) * ROWS;
+  int64_t row = int64_t(blockIdx.x) * ROWS + group;
+  R rows(a.x, a.x_stride, a.rows, a.width, lane, stage);
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    rows.fetch(row + i * step);
+    close_fetch();
+  }
   float w[kElems], b[kElems];
 #pragma unroll
   for (int e = 0; e < kElems; e++) {
@@ -98,24 +153,23 @@ __global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) forward_k
     b[e] = a.b && c < a.width ? load_param(a.b, a.wdtype, c) : 0.f;
   }
   const float inv = 1.f / float(a.width);
-  const int64_t step = int64_t(gridDim.x) * ROWS;
-  int64_t row = int64_t(blockIdx.x) * ROWS + group;
-  Share<T, LANES, VEC> next;
-  next.load(x + row * a.x_stride, lane, a.width, row < a.rows);
   // every group of the block takes the same number of turns: the row sums hold barriers
   for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += step, row += step) {
-    const Share<T, LANES, VEC> cur = next;
-    next.load(x + (row + step) * a.x_stride, lane, a.width, row + step < a.rows);
+    float x[kElems];
+    if (R::ASYNC) wait_fetch<AHEAD - 1>();
+    rows.take(x);
+    rows.fetch(row + AHEAD * step);
+    close_fetch();
     float s = 0.f;
 #pragma unroll
-    for (int e = 0; e < kElems; e++) s += cur.get(e / VEC, e % VEC);
+    for (int e = 0; e < kElems; e++) s += x[e];
     const float mu = row_sum<LANES>(s, red[0]) * inv;
     float q = 0.f;
 #pragma unroll
     for (int e = 0; e < kElems; e++) {
       const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
-      const float d = cur.get(e / VEC, e % VEC) - mu;
-      if (c < a.width) q += d * d;
+      x[e] -= mu;
+      if (c < a.width) q += x[e] * x[e];
     }
     const float rs = rsqrtf(row_sum<LANES>(q, red[1]) * inv + a.eps);
     if (row >= a.rows) continue;
@@ -128,21 +182,31 @@ __global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) forward_k
       const int c = (v * LANES + lane) * VEC;
       float o[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; i++) o[i] = (cur.get(v, i) - mu) * rs * w[v * VEC + i] + b[v * VEC + i];
+      for (int i = 0; i < VEC; i++) o[i] = x[v * VEC + i] * rs * w[v * VEC + i] + b[v * VEC + i];
       if (c < a.width && LNCC_IN(row * a.width + c, VEC, a.rows * a.width)) store_vec<T, VEC>(y + row * a.width + c, o);
     }
   }
 }
 
 template <typename T, int LANES, int VEC>
-__global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) backward_kernel(const Args a) {
+__global__ void __launch_bounds__(threads_of<LANES>(), LANES <= kThreads && VEC * sizeof(T) >= 4 ? 2 : 1) backward_kernel(const Args a) {
   constexpr int THREADS = LANES > kThreads ? LANES : kThreads;
   constexpr int ROWS = THREADS / LANES, NV = kElems / VEC;
+  typedef Rows<T, LANES, VEC, THREADS> R;
+  constexpr int AHEAD = R::ASYNC ? R::kStages - 1 : 1;
+  extern __shared__ __align__(16) unsigned char stage[];
   __shared__ float red[2][THREADS / 32];
   const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const T* x = static_cast<const T*>(a.x);
-  const T* dy = static_cast<const T*>(a.dy);
   T* dx = static_cast<T*>(a.y);
+  const int64_t step = int64_t(gridDim.x) * ROWS;
+  int64_t row = int64_t(blockIdx.x) * ROWS + group;
+  R rows_x(a.x, a.x_stride, a.rows, a.width, lane, stage), rows_dy(a.dy, a.dy_stride, a.rows, a.width, lane, stage + R::smem());
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    rows_x.fetch(row + i * step);
+    rows_dy.fetch(row + i * step);
+    close_fetch();
+  }
   float w[kElems], dw[kElems], db[kElems];
 #pragma unroll
   for (int e = 0; e < kElems; e++) {
@@ -151,41 +215,41 @@ __global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) backward_
     dw[e] = db[e] = 0.f;
   }
   const float inv = 1.f / float(a.width);
-  const int64_t step = int64_t(gridDim.x) * ROWS;
-  int64_t row = int64_t(blockIdx.x) * ROWS + group;
-  Share<T, LANES, VEC> next_x, next_dy;
-  next_x.load(x + row * a.x_stride, lane, a.width, row < a.rows);
-  next_dy.load(dy + row * a.dy_stride, lane, a.width, row < a.rows);
+  float mu_next = row < a.rows ? a.mean[row] : 0.f, rs_next = row < a.rows ? a.rstd[row] : 0.f;
   for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += step, row += step) {
-    const Share<T, LANES, VEC> cx = next_x, cd = next_dy;
-    const bool live = row < a.rows, more = row + step < a.rows;
-    next_x.load(x + (row + step) * a.x_stride, lane, a.width, more);
-    next_dy.load(dy + (row + step) * a.dy_stride, lane, a.width, more);
-    const float mu = live ? a.mean[row] : 0.f, rs = live ? a.rstd[row] : 0.f;
+    float n[kElems], d[kElems];
+    const float mu = mu_next, rs = rs_next;
+    mu_next = row + step < a.rows ? a.mean[row + step] : 0.f;
+    rs_next = row + step < a.rows ? a.rstd[row + step] : 0.f;
+    if (R::ASYNC) wait_fetch<AHEAD - 1>();
+    rows_x.take(n);
+    rows_dy.take(d);
+    rows_x.fetch(row + AHEAD * step);
+    rows_dy.fetch(row + AHEAD * step);
+    close_fetch();
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int e = 0; e < kElems; e++) {  // past the row's end dy is 0, and with it every term
-      const float d = cd.get(e / VEC, e % VEC), n = (cx.get(e / VEC, e % VEC) - mu) * rs;
-      db[e] += d;
-      dw[e] += d * n;
-      s1 += d * w[e];
-      s2 += d * w[e] * n;
+      n[e] = (n[e] - mu) * rs;
+      db[e] += d[e];
+      dw[e] += d[e] * n[e];
+      d[e] *= w[e];
+      s1 += d[e];
+      s2 += d[e] * n[e];
     }
     if (a.y == nullptr) continue;  // the same for every thread
     const float m1 = row_sum<LANES>(s1, red[0]) * inv, m2 = row_sum<LANES>(s2, red[1]) * inv;
-    if (!live) continue;
+    if (row >= a.rows) continue;
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = (v * LANES + lane) * VEC;
       float o[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; i++) {
-        const float n = (cx.get(v, i) - mu) * rs;
-        o[i] = rs * (cd.get(v, i) * w[v * VEC + i] - m1 - n * m2);
-      }
+      for (int i = 0; i < VEC; i++) o[i] = rs * (d[v * VEC + i] - m1 - n[v * VEC + i] * m2);
       if (c < a.width && LNCC_IN(row * a.width + c, VEC, a.rows * a.width)) store_vec<T, VEC>(dx + row * a.width + c, o);
     }
   }
+  if (R::ASYNC) wait_fetch<0>();  // nothing is under way to shared memory any more
   if (a.partial == nullptr) return;
   // the block's rows meet: thread t < LANES adds the other groups' sums to its own, group by group
   float* out = a.partial + int64_t(blockIdx.x) * 2 * a.width;
@@ -210,21 +274,23 @@ __global__ void __launch_bounds__(LANES > kThreads ? LANES : kThreads) backward_
   }
 }
 
-// dw and db: column sums of the blocks' partial sums, eight strands of blocks in order and then the strands in order.
-__global__ void __launch_bounds__(256) reduce_kernel(const float* __restrict__ partial, int blocks, int width, void* dw,
-                                                     void* db, int wdtype) {
-  __shared__ float sum[8][33];
+// dw and db: column sums of the blocks' partial sums, 32 strands of blocks in order and then the strands in order.
+__global__ void __launch_bounds__(1024) reduce_kernel(const float* __restrict__ partial, int blocks, int width, void* dw,
+                                                      void* db, int wdtype) {
+  __shared__ float sum[32][33];
   const int strand = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t c = int64_t(blockIdx.x) * 32 + lane, cols = 2 * int64_t(width);
   float s = 0.f;
-  if (c < cols)
-    for (int p = strand; p < blocks; p += 8) s += partial[p * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int p = strand; p < blocks; p += 32) s += partial[p * cols + c];
+  }
   sum[strand][lane] = s;
   __syncthreads();
   if (strand != 0 || c >= cols) return;
   s = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; i++) s += sum[i][lane];
+  for (int i = 0; i < 32; i++) s += sum[i][lane];
   void* to = c < width ? dw : db;
   const int64_t i = c < width ? c : c - width;
   if (to == nullptr || !LNCC_IN(i, 1, width)) return;
@@ -297,13 +363,13 @@ static int lanes_for(int64_t width) {
   return lanes;
 }
 
-// Thread blocks of a call: enough rows for each to pay for its weights, at most what the GPU holds at once.
-// The backward kernel holds about 110 registers a thread, so two blocks of 256 fit on an SM.
+// Thread blocks of a call: as many as have rows, at most what the GPU holds at once (three of 256 threads an SM forward, two
+// backward, whose sums take 120 registers; one of 512).
 static int blocks_for(int64_t rows, int64_t width, bool backward) {
   const int sms = sm_count();
   if (width > kMaxWidth) return int(rows < sms * 2 ? rows : sms * 2);
   const int lanes = lanes_for(width), threads = lanes > kThreads ? lanes : kThreads;
-  const int64_t need = ceil_div(rows, threads / lanes), fit = int64_t(sms) * ((backward ? 512 : 1024) / threads > 0 ? (backward ? 512 : 1024) / threads : 1);
+  const int64_t need = ceil_div(rows, threads / lanes), fit = int64_t(sms) * (threads > kThreads ? 1 : backward ? 2 : 3);
   return int(need < fit ? need : fit);
 }
 static int strands_for(int64_t rows, int64_t width) {
@@ -311,25 +377,25 @@ static int strands_for(int64_t rows, int64_t width) {
   return int(rows < 64 ? rows : 64);
 }
 
+template <typename T, int VEC, int LANES> static void launch_lanes(const Args& a, bool backward, int grid, cudaStream_t st) {
+  constexpr int threads = threads_of<LANES>();
+  const int ring = Rows<T, LANES, VEC, threads>::smem(), smem = backward ? 2 * ring : ring;
+  const auto kernel = backward ? backward_kernel<T, LANES, VEC> : forward_kernel<T, LANES, VEC>;
+  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  kernel<<<grid, threads, smem, st>>>(a);
+}
 template <typename T, int VEC> static void launch(const Args& a, bool backward, cudaStream_t st) {
-  const int lanes = lanes_for(a.width), grid = blocks_for(a.rows, a.width, backward);
-#define LNCC_NORM_CASE(L)                                                            \
-  case L:                                                                            \
-    if (backward) backward_kernel<T, L, VEC><<<grid, L > kThreads ? L : kThreads, 0, st>>>(a); \
-    else forward_kernel<T, L, VEC><<<grid, L > kThreads ? L : kThreads, 0, st>>>(a); \
-    break;
-  switch (lanes) {
-    LNCC_NORM_CASE(4)
-    LNCC_NORM_CASE(8)
-    LNCC_NORM_CASE(16)
-    LNCC_NORM_CASE(32)
-    LNCC_NORM_CASE(64)
-    LNCC_NORM_CASE(128)
-    LNCC_NORM_CASE(256)
-    LNCC_NORM_CASE(512)
-    LNCC_NORM_CASE(1024)
+  const int grid = blocks_for(a.rows, a.width, backward);
+  switch (lanes_for(a.width)) {
+    case 4: launch_lanes<T, VEC, 4>(a, backward, grid, st); break;
+    case 8: launch_lanes<T, VEC, 8>(a, backward, grid, st); break;
+    case 16: launch_lanes<T, VEC, 16>(a, backward, grid, st); break;
+    case 32: launch_lanes<T, VEC, 32>(a, backward, grid, st); break;
+    case 64: launch_lanes<T, VEC, 64>(a, backward, grid, st); break;
+    case 128: launch_lanes<T, VEC, 128>(a, backward, grid, st); break;
+    case 256: launch_lanes<T, VEC, 256>(a, backward, grid, st); break;
+    default: launch_lanes<T, VEC, 512>(a, backward, grid, st); break;
   }
-#undef LNCC_NORM_CASE
 }
 
 // 16-byte accesses where every row of every array starts on a 16-byte boundary, else single elements.
@@ -422,7 +488,7 @@ int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, i
   a.partial = params ? static_cast<float*>(scratch) : nullptr;
   norm::dispatch(a, dtype, true, stream);
   if (params)
-    norm::reduce_kernel<<<unsigned(blk::ceil_div(2 * width, 32)), 256, 0, stream>>>(
+    norm::reduce_kernel<<<unsigned(blk::ceil_div(2 * width, 32)), 1024, 0, stream>>>(
         a.partial, norm::strands_for(rows, width), a.width, dweight, dbias, wdtype);
   return blk::check_end(stream);
 }
