@@ -27,6 +27,8 @@
 // infinity taken apart meets zeros: it gives NaN where fp32 would give an infinity.
 #include "lncc_tc.cuh"
 
+#include <type_traits>
+
 namespace lncc {
 namespace ffn {
 
@@ -44,7 +46,7 @@ __host__ __device__ constexpr bool b_mn(int kind) { return kind == DH || kind ==
 __host__ __device__ constexpr bool gated(int kind) { return kind == UP || kind == GATES || kind == HIDDEN; }
 __host__ __device__ constexpr int b_tile(int bn) { return bn / 2 * 64 * 2; }  // a CTA's share of B
 __host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 6 : 8; }
-__host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256; }
+__host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256 + 8 * 32 * 17 * 4; }
 
 // Planes of the six products of operands that are taken apart, smallest first.
 __device__ __constant__ const int8_t kPlaneA[6] = {2, 1, 0, 1, 0, 0}, kPlaneB[6] = {0, 1, 2, 0, 1, 0};
@@ -65,57 +67,74 @@ struct Gemm {
   int clear_abort;
 };
 
-// act(g) and act'(g). For 16-bit types the fast exponential and reciprocal (a few u32, and |g| u32 for the exponential),
-// and erf by Abramowitz and Stegun 7.1.26: with z = |g|/sqrt 2 and t = 1/(1 + 0.3275911 z), erfc(z) = t (a1 + t (a2 + ...))
-// exp(-z^2) to 1.5e-7, whose exponential is the one of the derivative.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_fast(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// act(g) and act'(g). For 16-bit types by the fast exponential of 2 and reciprocal (a few u32, and |g| u32 for the
+// exponential), and erf by Abramowitz and Stegun 7.1.26: with z = |g|/sqrt 2 and t = 1/(1 + 0.3275911 z),
+// erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2) to 1.5e-7, whose exponential is the one of the derivative. The epilogue is bound
+// by its instructions where K is small: constants are folded (log2 e into the exponent, 1/2 into the coefficients).
 template <int ACT, bool FAST> __device__ __forceinline__ void activate(float g, float& a, float& da) {
   if (ACT == LNCC_ACT_RELU) {
     a = g < 0.f ? 0.f : g;
     da = g > 0.f ? 1.f : 0.f;
   } else if (ACT == LNCC_ACT_SILU) {
-    const float p = FAST ? __fdividef(1.f, 1.f + __expf(-g)) : 1.f / (1.f + expf(-g));
+    const float p = FAST ? rcp_fast(1.f + exp2_fast(g * -1.44269504f)) : 1.f / (1.f + expf(-g));
     a = g * p;
-    da = p * (1.f + g * (1.f - p));
-  } else {
-    const float e = FAST ? __expf(-0.5f * g * g) : expf(-0.5f * g * g);
-    float p;
-    if (FAST) {
-      const float z = fabsf(g) * 0.70710678f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
-      const float q = 0.5f * e * t *
-                      fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
-                           0.254829592f);
-      p = g < 0.f ? q : 1.f - q;
-    } else {
-      p = 0.5f * erfcf(-g * 0.70710678f);
-    }
+    da = FAST ? fmaf(a, 1.f - p, p) : p * (1.f + g * (1.f - p));
+  } else if (FAST) {
+    const float e = exp2_fast(g * g * -0.72134752f), t = rcp_fast(fmaf(0.231641888f, fabsf(g), 1.f));
+    const float q = e * t *
+                    fmaf(t, fmaf(t, fmaf(t, fmaf(t, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f),
+                         0.127414796f);
+    const float p = g < 0.f ? q : 1.f - q;
     a = g * p;
     da = fmaf(g * 0.39894228f, e, p);
+  } else {
+    const float p = 0.5f * erfcf(-g * 0.70710678f);
+    a = g * p;
+    da = fmaf(g * 0.39894228f, expf(-0.5f * g * g), p);
   }
 }
 
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
-  return uint32_t(__bfloat16_as_ushort(a)) | uint32_t(__bfloat16_as_ushort(b)) << 16;
-}
-__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
-  return uint32_t(__half_as_ushort(a)) | uint32_t(__half_as_ushort(b)) << 16;
+// two values rounded to 16 bits, the first in the lower half
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
 }
 __device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                : "memory");
 }
-// 16 neighbours of a row, those of them that lie before column `cols`.
+// 16 columns of 32 rows, a row a lane, those that lie inside rows x cols. Whole chunks of rows that start on 16 or 32 bytes
+// go straight out. The rest goes through 32 x 17 floats of shared memory and out again with 16 lanes to a row: element by
+// element with a row a lane, a product with 333 columns took 130 us of which 95 were its stores.
+constexpr int kStageRow = 17, kStageFloats = 32 * kStageRow;
 template <typename T>
-__device__ __forceinline__ void emit(T* base, int64_t ld, int64_t row, int64_t col, int64_t cols, int align,
-                                     const T (&v)[16]) {
-  T* p = base + row * ld + col;
+__device__ __forceinline__ void emit(T* base, int64_t ld, int64_t row0, int64_t col, int64_t rows, int64_t cols, int align,
+                                     const float (&v)[16], float* stage) {
+  const int lane = threadIdx.x % 32;
+  if (col >= cols) return;  // the same for all lanes, like the next
   if (col + 16 <= cols && align >= 16) {
+    const int64_t row = row0 + lane;
+    if (row >= rows || !LNCC_IN(row * ld + col, 16, (rows - 1) * ld + cols)) return;
+    T* p = base + row * ld + col;
     constexpr int WORDS = 16 * int(sizeof(T)) / 4;
     uint32_t w[WORDS];
 #pragma unroll
     for (int i = 0; i < WORDS; i++) {
       if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
-      else w[i] = pack2(v[2 * i], v[2 * i + 1]);
+      else w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
     }
     if (align >= 32) {
 #pragma unroll
@@ -130,8 +149,16 @@ __device__ __forceinline__ void emit(T* base, int64_t ld, int64_t row, int64_t c
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; i++)
-      if (col + i < cols) p[i] = v[i];
+    for (int i = 0; i < 16; i++) stage[lane * kStageRow + i] = v[i];
+    __syncwarp();
+    const int c = lane % 16;
+    T* p = base + (row0 + lane / 16) * ld + col + c;
+    if (col + c < cols) {
+#pragma unroll 4
+      for (int r = lane / 16; r < 32; r += 2, p += 2 * ld)
+        if (row0 + r < rows && LNCC_IN((row0 + r) * ld + col + c, 1, (rows - 1) * ld + cols)) *p = from_f<T>(stage[r * kStageRow + c]);
+    }
+    __syncwarp();
   }
 }
 // fp32 as three bf16 numbers that add up to it. The first is cut, not rounded, so that it stays finite; all 24 bits are held.
@@ -142,22 +169,24 @@ __device__ __forceinline__ void take_apart(float v, __nv_bfloat16& hi, __nv_bflo
   mid = __float2bfloat16_rn(fine ? r : 0.f);
   lo = __float2bfloat16_rn(fine ? r - __bfloat162float(mid) : 0.f);
 }
-// Hidden results: of the type, or taken apart for fp32.
+// Hidden results: of the type, or taken apart for fp32 (each part is a bf16 number, which the rounding leaves as it is).
 template <typename T>
-__device__ __forceinline__ void emit_hidden(void* base, const Gemm& g, int64_t row, int64_t col, const float (&v)[16]) {
-  if (row >= g.rows || col >= g.cols || !LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) return;
+__device__ __forceinline__ void emit_hidden(void* base, const Gemm& g, int64_t row0, int64_t col, const float (&v)[16],
+                                            float* stage) {
   if constexpr (sizeof(T) == 2) {
-    T o[16];
-#pragma unroll
-    for (int i = 0; i < 16; i++) o[i] = from_f<T>(v[i]);
-    emit<T>(static_cast<T*>(base), g.ld, row, col, g.cols, g.align, o);
+    emit<T>(static_cast<T*>(base), g.ld, row0, col, g.rows, g.cols, g.align, v, stage);
   } else {
-    __nv_bfloat16 o[3][16];
+    float part[3][16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) take_apart(v[i], o[0][i], o[1][i], o[2][i]);
+    for (int i = 0; i < 16; i++) {
+      __nv_bfloat16 hi, mid, lo;
+      take_apart(v[i], hi, mid, lo);
+      part[0][i] = to_f(hi), part[1][i] = to_f(mid), part[2][i] = to_f(lo);
+    }
 #pragma unroll
     for (int k = 0; k < 3; k++)
-      emit<__nv_bfloat16>(static_cast<__nv_bfloat16*>(base) + k * g.plane, g.ld, row, col, g.cols, g.align, o[k]);
+      emit<__nv_bfloat16>(static_cast<__nv_bfloat16*>(base) + k * g.plane, g.ld, row0, col, g.rows, g.cols, g.align, part[k],
+                          stage);
   }
 }
 
@@ -317,60 +346,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     // ---- epilogue: lanes are rows; two warps share a row, half of the columns each
     const int sub = warp & 3, half = (warp - 4) / 4;
     constexpr int COLS = gated(KIND) ? HALF / 2 : HALF;  // columns of a result that a warp takes
-    const float nan = __int_as_float(0x7fffffff);
+    float* const stage = reinterpret_cast<float*>(smem + STAGES * (kATile + BT) + 256) + (warp - 4) * kStageFloats;
+    constexpr uint32_t kNaN = 0x7fffffff;  // what a tile gets whose products were given up
     int turn = 0;
     for (int t = blockIdx.x / 2; t < tiles; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
-      const int64_t row = int64_t(w.m) * 256 + rank * 128 + sub * 32 + lane;
+      const int64_t row0 = int64_t(w.m) * 256 + rank * 128 + sub * 32;
       const int64_t col0 = int64_t(w.n) * (gated(KIND) ? HALF : BN) + half * COLS;
 
-      // 16 columns: v0 (g, or the product), v1 (u), v2 (dh) as fp32
+      // 16 columns: v0 (g, or the product), v1 (u), v2 (dh) as fp32; all lanes of the warp together
       const auto finish = [&](int64_t col, const float (&v0)[16], const float (&v1)[16], const float (&v2)[16]) {
-        if (row >= g.rows || col >= g.cols) return;
-        if constexpr (KIND == UP || KIND == HIDDEN) {
-          float h[16], dg[16], du[16];
+        if (row0 >= g.rows || col >= g.cols) return;
+        if constexpr (KIND == UP) {
+          float h[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
             float a, da;
             activate<ACT, !F32>(v0[i], a, da);
             h[i] = a * v1[i];
-            dg[i] = v2[i] * v1[i] * da;
-            du[i] = v2[i] * a;
           }
-          if (KIND == HIDDEN) {
-            emit_hidden<T>(g.out0, g, row, col, dg);
-            emit_hidden<T>(g.out1, g, row, col, du);
-            emit_hidden<T>(g.out2, g, row, col, h);
-          } else {
-            emit_hidden<T>(g.out0, g, row, col, h);
-          }
-        } else if constexpr (KIND == DH) {
+          emit_hidden<T>(g.out0, g, row0, col, h, stage);
+        } else if constexpr (KIND == HIDDEN || KIND == DH) {
           float h[16], dg[16], du[16];
+          float4 gates[4], ups[4];
+          if (KIND == DH) {  // rows of g and u are padded to whole chunks
+            const int64_t at = min(row0 + lane, g.rows - 1) * g.ld + col;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              gates[i] = reinterpret_cast<const float4*>(g.gate + at)[i];
+              ups[i] = reinterpret_cast<const float4*>(g.up + at)[i];
+            }
+          }
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            const bool in = col + i < g.cols;
-            const float gate = in ? g.gate[row * g.ld + col + i] : 0.f, up = in ? g.up[row * g.ld + col + i] : 0.f;
+            const float gate = KIND == DH ? reinterpret_cast<const float*>(gates)[i] : v0[i];
+            const float up = KIND == DH ? reinterpret_cast<const float*>(ups)[i] : v1[i], dh = KIND == DH ? v0[i] : v2[i];
             float a, da;
             activate<ACT, !F32>(gate, a, da);
             h[i] = a * up;
-            dg[i] = v0[i] * up * da;
-            du[i] = v0[i] * a;
+            dg[i] = dh * up * da;
+            du[i] = dh * a;
           }
-          emit_hidden<T>(g.out0, g, row, col, dg);
-          emit_hidden<T>(g.out1, g, row, col, du);
-          emit_hidden<T>(g.out2, g, row, col, h);
+          emit_hidden<T>(g.out0, g, row0, col, dg, stage);
+          emit_hidden<T>(g.out1, g, row0, col, du, stage);
+          emit_hidden<T>(g.out2, g, row0, col, h, stage);
         } else if constexpr (KIND == GATES) {
-          if (!LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) return;
-          emit<float>(static_cast<float*>(g.out0), g.ld, row, col, g.cols, g.align, v0);
-          emit<float>(static_cast<float*>(g.out1), g.ld, row, col, g.cols, g.align, v1);
+          emit<float>(static_cast<float*>(g.out0), g.ld, row0, col, g.rows, g.cols, g.align, v0, stage);
+          emit<float>(static_cast<float*>(g.out1), g.ld, row0, col, g.rows, g.cols, g.align, v1, stage);
         } else if (g.splits > 1) {
           const int64_t ld = (g.cols + 3) / 4 * 4;
-          emit<float>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row, col, ld, 16, v0);
-        } else if (LNCC_IN(row * g.ld + col, 1, g.rows * g.ld)) {
-          T o[16];
-#pragma unroll
-          for (int i = 0; i < 16; i++) o[i] = from_f<T>(v0[i]);
-          emit<T>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row, col, g.cols, g.align, o);
+          emit<float>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row0, col, g.rows, ld, 16, v0, stage);
+        } else {
+          emit<T>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, v0, stage);
         }
       };
       const auto done = [&](int acc) {  // this warp has read the accumulator
@@ -393,9 +420,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             if (ok) {
               tmem_load(d + (gated(KIND) ? i / 2 * HALF + i % 2 * 16 : i * 16), v);
               wait_ld(v);
+            } else {
+              for (int j = 0; j < 16; j++) v[j] = kNaN;
             }
 #pragma unroll
-            for (int j = 0; j < 16; j++) sum[i][j] += ok ? __uint_as_float(v[j]) : nan;
+            for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
           }
           done(turn & 1);
         }
@@ -423,14 +452,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             wait_ld(v[0]);
             if (gated(KIND)) wait_ld(v[1]);
             if (KIND == HIDDEN) wait_ld(v[2]);
+          } else {
+            for (int i = 0; i < 16; i++) v[0][i] = v[1][i] = v[2][i] = kNaN;
           }
           if (c + 16 == COLS) done(acc);
           float f[3][16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            f[0][i] = ok ? __uint_as_float(v[0][i]) : nan;
-            f[1][i] = ok ? __uint_as_float(v[gated(KIND) ? 1 : 0][i]) : nan;
-            f[2][i] = ok ? __uint_as_float(v[KIND == HIDDEN ? 2 : 0][i]) : nan;
+            f[0][i] = __uint_as_float(v[0][i]);
+            f[1][i] = __uint_as_float(v[gated(KIND) ? 1 : 0][i]);
+            f[2][i] = __uint_as_float(v[KIND == HIDDEN ? 2 : 0][i]);
           }
           finish(col0 + c, f[0], f[1], f[2]);
         }
@@ -546,6 +577,121 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ x, 
     }
 }
 
+// ---- a few tokens ----------------------------------------------------------------------------------------------------
+// Up to eight tokens need each weight once and little else: a warp reads rows of the weights, 16 bytes a lane, and multiplies
+// them with the tokens, which wait in shared memory in fp32. h stays fp32 between the two kernels. Measured for one token,
+// 1024 x 2816 bf16 (17 MB of weights, 2.7 us at the copy rate): the tensor kernels' pair tiles took 14 + 10 + 3 us.
+constexpr int kFewTokens = 8, kFewBytes = 64 * 1024;  // of fp32 tokens in shared memory, K or F wide
+constexpr int kRowWarps = 4;                         // warps that share a row of Wd
+
+template <typename T, int V> __device__ __forceinline__ void to_floats(const Vec<T, V>& v, float (&f)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i++) f[i] = to_f(v.e[i]);
+}
+// acc[m] += sum over this lane's V elements of w[at] x[m][at]
+template <int V, int MT>
+__device__ __forceinline__ void multiply(const float (&w)[V], const float* x, int64_t width, int64_t at, float (&acc)[MT]) {
+#pragma unroll
+  for (int m = 0; m < MT; m++) {
+    const Vec<float, V> t = *reinterpret_cast<const Vec<float, V>*>(x + m * width + at);
+#pragma unroll
+    for (int i = 0; i < V; i++) acc[m] = fmaf(w[i], t.e[i], acc[m]);
+  }
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// h[m][f], one f a warp at a time. V: weights of a lane's load.
+template <typename T, int V, int MT, int ACT>
+__global__ void __launch_bounds__(256) few_up_kernel(const T* __restrict__ x, int64_t x_stride, const T* __restrict__ wg,
+                                                     const T* __restrict__ wu, float* __restrict__ h, int64_t M, int64_t K,
+                                                     int64_t F, unsigned* abort_word) {
+  extern __shared__ __align__(128) float tokens[];  // [MT][width], zeros past M and K
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (blockIdx.x == 0 && threadIdx.x == 0) *abort_word = 0u;  // these kernels wait for nothing
+  const int64_t width = (K + 32 * V - 1) / (32 * V) * (32 * V);
+  for (int64_t i = threadIdx.x; i < MT * width; i += 256) {
+    const int64_t m = i / width, k = i % width;
+    tokens[i] = m < M && k < K ? to_f(x[m * x_stride + k]) : 0.f;
+  }
+  __syncthreads();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  for (int64_t f = int64_t(blockIdx.x) * 8 + warp; f < F; f += int64_t(gridDim.x) * 8) {
+    float ag[MT] = {}, au[MT] = {};
+#pragma unroll 4
+    for (int64_t k = lane * V; k < K; k += 32 * V) {  // K is a multiple of V
+      float g[V], u[V];
+      to_floats(*reinterpret_cast<const Vec<T, V>*>(wg + f * K + k), g);
+      to_floats(*reinterpret_cast<const Vec<T, V>*>(wu + f * K + k), u);
+      multiply<V, MT>(g, tokens, width, k, ag);
+      multiply<V, MT>(u, tokens, width, k, au);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      const float g = warp_sum(ag[m]), u = warp_sum(au[m]);
+      float a, da;
+      activate<ACT, sizeof(T) == 2>(g, a, da);
+      if (lane == 0 && m < M && LNCC_IN(m * F + f, 1, M * F)) h[m * F + f] = a * u;
+    }
+  }
+}
+
+// y[m][n]: kRowWarps warps share a row of Wd, whose first loads are under way before h is waited for.
+template <typename T, int V, int MT>
+__global__ void __launch_bounds__(256) few_down_kernel(const float* __restrict__ h, const T* __restrict__ wd,
+                                                       T* __restrict__ y, int64_t M, int64_t F, int64_t N) {
+  extern __shared__ __align__(128) float tokens[];  // [MT][width], zeros past M and F
+  __shared__ float meet[8][MT];
+  constexpr int ROWS = 8 / kRowWarps, STEP = 32 * V * kRowWarps, HELD = 4;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, mine = warp % kRowWarps;
+  const int64_t width = (F + STEP - 1) / STEP * STEP, first = (mine * 32 + lane) * V;
+  typedef Vec<T, V> W;
+  W held[HELD];
+  const auto load = [&](int64_t n, int64_t from) {
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+      if (n < N && from + i * STEP < F) held[i] = *reinterpret_cast<const W*>(wd + n * F + from + i * STEP);
+  };
+  int64_t n = int64_t(blockIdx.x) * ROWS + warp / kRowWarps;
+  load(n, first);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int64_t i = threadIdx.x; i < MT * width; i += 256) {
+    const int64_t m = i / width, f = i % width;
+    tokens[i] = m < M && f < F ? h[m * F + f] : 0.f;
+  }
+  __syncthreads();
+  for (int64_t n0 = int64_t(blockIdx.x) * ROWS; n0 < N; n0 += int64_t(gridDim.x) * ROWS) {
+    float acc[MT] = {};
+    for (int64_t from = first; from < F; from += HELD * STEP) {
+      if (from != first || n0 != int64_t(blockIdx.x) * ROWS) load(n, from);
+#pragma unroll
+      for (int i = 0; i < HELD; i++) {
+        if (n < N && from + i * STEP < F) {
+          float w[V];
+          to_floats(held[i], w);
+          multiply<V, MT>(w, tokens, width, from + i * STEP, acc);
+        }
+      }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; m++) {
+      const float s = warp_sum(acc[m]);
+      if (lane == 0) meet[warp][m] = s;
+    }
+    __syncthreads();
+    if (mine == 0 && lane < M && n < N && LNCC_IN(lane * N + n, 1, M * N)) {
+      float s = 0.f;
+      for (int i = 0; i < kRowWarps; i++) s += meet[warp + i][lane];
+      y[lane * N + n] = from_f<T>(s);
+    }
+    __syncthreads();
+    n += int64_t(gridDim.x) * ROWS;
+  }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------------
 struct Args {
   const void *x, *wg, *wu, *wd, *dy;
@@ -595,8 +741,13 @@ static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int
   return c.splits > 1 ? size_t(c.splits) * whichs * rows * ((cols + 3) / 4 * 4) * 4 : 0;
 }
 static int64_t k_steps(int64_t k) { return ceil_div(k, 64); }
+static bool few(const Args& a);
 static Plan plan_for(const Args& a, bool backward) {
   Plan p = {};
+  if (!backward && few(a)) {
+    p.total = kHeader + round_up(size_t(a.M) * a.F * 4);
+    return p;
+  }
   p.planes = a.dtype == LNCC_F32 ? 3 : 1;
   p.ldf = lead(a.F);
   size_t at = kHeader;
@@ -749,7 +900,57 @@ struct Call {
   }
 };
 
+static int tokens_of(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
+static bool few(const Args& a) {
+  const int64_t widest = (a.K > a.F ? a.K : a.F) + 1024;  // rounded up to a block's step
+  return a.M <= kFewTokens && tokens_of(a.M) * widest * 4 <= kFewBytes;
+}
+template <typename T, int V, int MT> static int few_run(const Args& a, float* h, cudaStream_t st) {
+  const auto up = a.act == LNCC_ACT_SILU ? few_up_kernel<T, V, MT, LNCC_ACT_SILU>
+                  : a.act == LNCC_ACT_GELU ? few_up_kernel<T, V, MT, LNCC_ACT_GELU> : few_up_kernel<T, V, MT, LNCC_ACT_RELU>;
+  const auto down = few_down_kernel<T, V, MT>;
+  const int up_smem = int(MT * ceil_div(a.K, 32 * V) * 32 * V * 4), step = 32 * V * kRowWarps;
+  const int down_smem = int(MT * ceil_div(a.F, step) * step * 4);
+  if (up_smem > 48 * 1024 && cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, up_smem) != cudaSuccess)
+    return LNCC_ERR_SMEM;
+  if (down_smem > 48 * 1024 && cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, down_smem) != cudaSuccess)
+    return LNCC_ERR_SMEM;
+  const int64_t most = int64_t(sm_count()) * 4, up_blocks = ceil_div(a.F, 8), down_blocks = ceil_div(a.N, 8 / kRowWarps);
+  up<<<unsigned(up_blocks < most ? up_blocks : most), 256, up_smem, st>>>(
+      static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.wg), static_cast<const T*>(a.wu), h, a.M, a.K, a.F,
+      reinterpret_cast<unsigned*>(reinterpret_cast<char*>(h) - kHeader));
+  cudaLaunchAttribute early = {};  // begins while the first kernel ends
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(down_blocks < most ? down_blocks : most)), cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = down_smem, cfg.stream = st, cfg.attrs = &early, cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, down, static_cast<const float*>(h), static_cast<const T*>(a.wd),
+                                           static_cast<T*>(a.y), a.M, a.F, a.N);
+  return e == cudaSuccess ? LNCC_OK : LNCC_ERR_LAUNCH;
+}
+template <typename T, int V> static int few_tokens(const Args& a, float* h, cudaStream_t st) {
+  switch (tokens_of(a.M)) {
+    case 1: return few_run<T, V, 1>(a, h, st);
+    case 2: return few_run<T, V, 2>(a, h, st);
+    case 4: return few_run<T, V, 4>(a, h, st);
+    default: return few_run<T, V, 8>(a, h, st);
+  }
+}
+template <typename T> static int few_forward(const Args& a, void* scratch, cudaStream_t st) {
+  constexpr int V = 16 / int(sizeof(T));
+  float* h = reinterpret_cast<float*>(static_cast<char*>(scratch) + kHeader);
+  if (a.K % V == 0 && a.F % V == 0 && aligned(a.wg, 16) && aligned(a.wu, 16) && aligned(a.wd, 16))
+    return few_tokens<T, V>(a, h, st);
+  return few_tokens<T, 1>(a, h, st);
+}
+
 static int forward(const Args& a, void* scratch, cudaStream_t stream) {
+  if (few(a)) {
+    if (a.dtype == LNCC_F32) return few_forward<float>(a, scratch, stream);
+    if (a.dtype == LNCC_BF16) return few_forward<__nv_bfloat16>(a, scratch, stream);
+    return few_forward<__half>(a, scratch, stream);
+  }
   Call c = {a, plan_for(a, false), static_cast<char*>(scratch), stream, LNCC_OK, true};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg),
                wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu), wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd),
