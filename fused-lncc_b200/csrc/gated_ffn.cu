@@ -35,9 +35,12 @@ namespace ffn {
 using namespace blk;
 using namespace tc;
 
+constexpr uint32_t kNaN = 0x7fffffff;  // what a tile gets whose products were given up
+
 enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
 
-constexpr int kThreads = 384;              // warps 0 TMA, 1 products, 4 - 11 epilogue
+constexpr int kEpilogueWarps = 16;         // of a CTA: four for each quarter of the lanes of tensor memory
+constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0 TMA, 1 products, 4 - 19 epilogue
 constexpr int kATile = 128 * 64 * 2;       // bytes of a CTA's share of A in a stage
 constexpr int kChunk = 4;                  // blocks of 64 that an accumulator of fp32 takes
 
@@ -46,7 +49,7 @@ __host__ __device__ constexpr bool b_mn(int kind) { return kind == DH || kind ==
 __host__ __device__ constexpr bool gated(int kind) { return kind == UP || kind == GATES || kind == HIDDEN; }
 __host__ __device__ constexpr int b_tile(int bn) { return bn / 2 * 64 * 2; }  // a CTA's share of B
 __host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 6 : 8; }
-__host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256 + 8 * 32 * 17 * 4; }
+__host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256 + kEpilogueWarps * 32 * 9 * 4; }
 
 // Planes of the six products of operands that are taken apart, smallest first.
 __device__ __constant__ const int8_t kPlaneA[6] = {2, 1, 0, 1, 0, 0}, kPlaneB[6] = {0, 1, 2, 0, 1, 0};
@@ -56,7 +59,7 @@ struct Gemm {
   int64_t rows, cols;        // of a result
   int m_tiles, n_tiles, whichs, splits;
   int k_steps, k_steps2;     // blocks of 64 of the inner axis (HIDDEN: of g and u, and of dh)
-  int blocks;                // of a tile: k_steps times the products summed into it (DX: 2)
+  int blocks, per_split;     // of a tile: k_steps times the products summed into it (DX: 2); those of a split
   int bf16;
   void *out0, *out1, *out2;  // results (DW_UP: of which = 0, 1; HIDDEN, DH: dg, du, h; GATES: g, u)
   int64_t ld, plane;         // of the results; plane for hidden results taken apart
@@ -111,52 +114,39 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
   else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-__device__ __forceinline__ void store32(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-               "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-// 16 columns of 32 rows, a row a lane, those that lie inside rows x cols. Whole chunks of rows that start on 16 or 32 bytes
-// go straight out. The rest goes through 32 x 17 floats of shared memory and out again with 16 lanes to a row: element by
-// element with a row a lane, a product with 333 columns took 130 us of which 95 were its stores.
-constexpr int kStageRow = 17, kStageFloats = 32 * kStageRow;
-template <typename T>
+// NW words (16 or 32 bytes) of 32 rows, a row a lane, from column col on: what lies inside rows x cols. Whole pieces of rows
+// that start on 16 or 32 bytes go straight out. The rest goes through shared memory and out again with the lanes side by
+// side along a row: element by element with a row a lane, a product with 333 columns took 130 us of which 95 were its stores.
+constexpr int kStageWords = 32 * 9;
+template <typename T, int NW>
 __device__ __forceinline__ void emit(T* base, int64_t ld, int64_t row0, int64_t col, int64_t rows, int64_t cols, int align,
-                                     const float (&v)[16], float* stage) {
+                                     const uint32_t (&w)[NW], uint32_t* stage) {
+  constexpr int N = NW * 4 / int(sizeof(T)), PITCH = NW + 1;  // elements; words from row to row of the stage
   const int lane = threadIdx.x % 32;
   if (col >= cols) return;  // the same for all lanes, like the next
-  if (col + 16 <= cols && align >= 16) {
+  if (col + N <= cols && align >= 16) {
     const int64_t row = row0 + lane;
-    if (row >= rows || !LNCC_IN(row * ld + col, 16, (rows - 1) * ld + cols)) return;
-    T* p = base + row * ld + col;
-    constexpr int WORDS = 16 * int(sizeof(T)) / 4;
-    uint32_t w[WORDS];
-#pragma unroll
-    for (int i = 0; i < WORDS; i++) {
-      if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
-      else w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    }
-    if (align >= 32) {
-#pragma unroll
-      for (int i = 0; i < WORDS; i += 8) {
-        const uint32_t u[8] = {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
-        store32(reinterpret_cast<uint32_t*>(p) + i, u);
-      }
+    if (row >= rows || !LNCC_IN(row * ld + col, N, (rows - 1) * ld + cols)) return;
+    uint32_t* p = reinterpret_cast<uint32_t*>(base + row * ld + col);
+    if (NW == 8 && align >= 32) {
+      asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                   "r"(w[4 % NW]), "r"(w[5 % NW]), "r"(w[6 % NW]), "r"(w[7 % NW])
+                   : "memory");
     } else {
 #pragma unroll
-      for (int i = 0; i < WORDS; i += 4)
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(p) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      for (int i = 0; i < NW; i += 4) *reinterpret_cast<uint4*>(p + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; i++) stage[lane * kStageRow + i] = v[i];
+    for (int i = 0; i < NW; i++) stage[lane * PITCH + i] = w[i];
     __syncwarp();
-    const int c = lane % 16;
-    T* p = base + (row0 + lane / 16) * ld + col + c;
+    const int c = lane % N, per_turn = 32 / N;
+    T* p = base + (row0 + lane / N) * ld + col + c;
     if (col + c < cols) {
 #pragma unroll 4
-      for (int r = lane / 16; r < 32; r += 2, p += 2 * ld)
-        if (row0 + r < rows && LNCC_IN((row0 + r) * ld + col + c, 1, (rows - 1) * ld + cols)) *p = from_f<T>(stage[r * kStageRow + c]);
+      for (int r = lane / N; r < 32; r += per_turn, p += per_turn * ld)
+        if (row0 + r < rows && LNCC_IN((row0 + r) * ld + col + c, 1, (rows - 1) * ld + cols))
+          *p = reinterpret_cast<const T*>(stage + r * PITCH)[c];
     }
     __syncwarp();
   }
@@ -169,39 +159,40 @@ __device__ __forceinline__ void take_apart(float v, __nv_bfloat16& hi, __nv_bflo
   mid = __float2bfloat16_rn(fine ? r : 0.f);
   lo = __float2bfloat16_rn(fine ? r - __bfloat162float(mid) : 0.f);
 }
-// Hidden results: of the type, or taken apart for fp32 (each part is a bf16 number, which the rounding leaves as it is).
-template <typename T>
-__device__ __forceinline__ void emit_hidden(void* base, const Gemm& g, int64_t row0, int64_t col, const float (&v)[16],
-                                            float* stage) {
-  if constexpr (sizeof(T) == 2) {
-    emit<T>(static_cast<T*>(base), g.ld, row0, col, g.rows, g.cols, g.align, v, stage);
-  } else {
-    float part[3][16];
+// Eight hidden results of a row in fp32, as the three bf16 matrices that hold them.
+__device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t row0, int64_t col, const float (&v)[8],
+                                           uint32_t* stage) {
+  float part[3][8];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      __nv_bfloat16 hi, mid, lo;
-      take_apart(v[i], hi, mid, lo);
-      part[0][i] = to_f(hi), part[1][i] = to_f(mid), part[2][i] = to_f(lo);
-    }
+  for (int i = 0; i < 8; i++) {
+    __nv_bfloat16 hi, mid, lo;
+    take_apart(v[i], hi, mid, lo);
+    part[0][i] = to_f(hi), part[1][i] = to_f(mid), part[2][i] = to_f(lo);
+  }
 #pragma unroll
-    for (int k = 0; k < 3; k++)
-      emit<__nv_bfloat16>(static_cast<__nv_bfloat16*>(base) + k * g.plane, g.ld, row0, col, g.rows, g.cols, g.align, part[k],
-                          stage);
+  for (int k = 0; k < 3; k++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = pack2<__nv_bfloat16>(part[k][2 * i], part[k][2 * i + 1]);
+    emit<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(base) + k * g.plane, g.ld, row0, col, g.rows, g.cols, g.align, w, stage);
   }
 }
 
-// One tile: 256 rows m, columns n, one of the results, blocks [from, to) of its inner axis.
+// One tile: 256 rows m, columns n, one of the results, blocks [from, to) of its inner axis. One division where nothing is
+// split: the thread that issues the products works this out between tiles, and the tensor cores wait for it (five
+// divisions, two of them of 64 bits, cost UP 24 of 198 us).
 struct Tile {
   int n, m, which, split, from, to;
 };
 __device__ __forceinline__ Tile tile_of(const Gemm& g, int t) {
   Tile r;
-  r.n = t % g.n_tiles, t /= g.n_tiles;
-  r.m = t % g.m_tiles, t /= g.m_tiles;
-  r.which = t % g.whichs;
-  r.split = t / g.whichs;
-  r.from = int(int64_t(g.blocks) * r.split / g.splits);
-  r.to = int(int64_t(g.blocks) * (r.split + 1) / g.splits);
+  r.m = t / g.n_tiles, r.n = t - r.m * g.n_tiles, r.which = r.split = 0, r.from = 0, r.to = g.blocks;
+  if (g.whichs * g.splits > 1) {
+    t = r.m;
+    r.split = t / (g.m_tiles * g.whichs), t -= r.split * g.m_tiles * g.whichs;
+    r.which = t / g.m_tiles, r.m = t - r.which * g.m_tiles;
+    r.from = r.split * g.per_split, r.to = min(g.blocks, r.from + g.per_split);
+  }
   return r;
 }
 
@@ -215,7 +206,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   constexpr int PARTS = F32 ? 6 : 1;                   // products of parts of the operands
   constexpr int CHUNK = F32 ? kChunk : 1 << 30;        // blocks that one accumulator takes
   static_assert(KIND != HIDDEN || (BN == 256 && !F32), "dh's share of B is one block of 64 columns a CTA");
-  static_assert(!F32 || BN == 128, "the epilogue's sums of fp32 take 64 registers");
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
   const uint32_t tiles_at = smem_addr(smem);
@@ -236,7 +226,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     }
     for (int i = 0; i < 2; i++) {
       mbar_init(acc_full + 8 * i, 1);
-      mbar_init(acc_empty + 8 * i, 16);  // eight epilogue warps of each CTA
+      mbar_init(acc_empty + 8 * i, 2 * kEpilogueWarps);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -343,127 +333,167 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       }
     }
   } else if (warp >= 4) {
-    // ---- epilogue: lanes are rows; two warps share a row, half of the columns each
-    const int sub = warp & 3, half = (warp - 4) / 4;
-    constexpr int COLS = gated(KIND) ? HALF / 2 : HALF;  // columns of a result that a warp takes
-    float* const stage = reinterpret_cast<float*>(smem + STAGES * (kATile + BT) + 256) + (warp - 4) * kStageFloats;
-    constexpr uint32_t kNaN = 0x7fffffff;  // what a tile gets whose products were given up
+    // ---- epilogue: lanes are rows; four warps share a row, a quarter of the columns each
+    const int sub = warp & 3, quarter = (warp - 4) / 4;
+    constexpr int COLS = gated(KIND) ? HALF / 4 : BN / 4;  // columns of a result that a warp takes
+    uint32_t* const stage = reinterpret_cast<uint32_t*>(smem + STAGES * (kATile + BT) + 256) + (warp - 4) * kStageWords;
     int turn = 0;
     for (int t = blockIdx.x / 2; t < tiles; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
       const int64_t row0 = int64_t(w.m) * 256 + rank * 128 + sub * 32;
-      const int64_t col0 = int64_t(w.n) * (gated(KIND) ? HALF : BN) + half * COLS;
-
-      // 16 columns: v0 (g, or the product), v1 (u), v2 (dh) as fp32; all lanes of the warp together
-      const auto finish = [&](int64_t col, const float (&v0)[16], const float (&v1)[16], const float (&v2)[16]) {
-        if (row0 >= g.rows || col >= g.cols) return;
-        if constexpr (KIND == UP) {
-          float h[16];
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            float a, da;
-            activate<ACT, !F32>(v0[i], a, da);
-            h[i] = a * v1[i];
-          }
-          emit_hidden<T>(g.out0, g, row0, col, h, stage);
-        } else if constexpr (KIND == HIDDEN || KIND == DH) {
-          float h[16], dg[16], du[16];
-          float4 gates[4], ups[4];
-          if (KIND == DH) {  // rows of g and u are padded to whole chunks
-            const int64_t at = min(row0 + lane, g.rows - 1) * g.ld + col;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              gates[i] = reinterpret_cast<const float4*>(g.gate + at)[i];
-              ups[i] = reinterpret_cast<const float4*>(g.up + at)[i];
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float gate = KIND == DH ? reinterpret_cast<const float*>(gates)[i] : v0[i];
-            const float up = KIND == DH ? reinterpret_cast<const float*>(ups)[i] : v1[i], dh = KIND == DH ? v0[i] : v2[i];
-            float a, da;
-            activate<ACT, !F32>(gate, a, da);
-            h[i] = a * up;
-            dg[i] = dh * up * da;
-            du[i] = dh * a;
-          }
-          emit_hidden<T>(g.out0, g, row0, col, dg, stage);
-          emit_hidden<T>(g.out1, g, row0, col, du, stage);
-          emit_hidden<T>(g.out2, g, row0, col, h, stage);
-        } else if constexpr (KIND == GATES) {
-          emit<float>(static_cast<float*>(g.out0), g.ld, row0, col, g.rows, g.cols, g.align, v0, stage);
-          emit<float>(static_cast<float*>(g.out1), g.ld, row0, col, g.rows, g.cols, g.align, v1, stage);
-        } else if (g.splits > 1) {
-          const int64_t ld = (g.cols + 3) / 4 * 4;
-          emit<float>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row0, col, g.rows, ld, 16, v0, stage);
-        } else {
-          emit<T>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, v0, stage);
-        }
-      };
+      const int64_t col0 = int64_t(w.n) * (gated(KIND) ? HALF : BN) + quarter * COLS;
+      const bool rows_here = row0 < g.rows;
       const auto done = [&](int acc) {  // this warp has read the accumulator
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty + 8 * acc, 0));
       };
+      // where an ordinary result of this tile goes: its type, or partial sums in fp32
+      const auto put = [&](int64_t col, const float (&v)[16]) {
+        if (g.splits > 1 || sizeof(T) == 4) {
+          const int64_t ld = (g.cols + 3) / 4 * 4;
+          float* to = g.splits > 1 ? g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld
+                                   : static_cast<float*>(w.which ? g.out1 : g.out0);
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = __float_as_uint(v[i + j]);
+            emit<float, 8>(to, g.splits > 1 ? ld : g.ld, row0, col + i, g.rows, g.splits > 1 ? ld : g.cols,
+                           g.splits > 1 ? 16 : g.align, o, stage);
+          }
+        } else if constexpr (sizeof(T) == 2) {
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; i++) o[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+          emit<T, 8>(static_cast<T*>(w.which ? g.out1 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, o, stage);
+        }
+      };
 
       if constexpr (F32) {
-        float sum[4][16];
+        constexpr int SUMS = gated(KIND) ? 2 * COLS : COLS;  // gated: columns of g, then of u
+        float sum[SUMS];
 #pragma unroll
-        for (int i = 0; i < 64; i++) sum[i / 16][i % 16] = 0.f;
+        for (int i = 0; i < SUMS; i++) sum[i] = 0.f;
         for (int c = w.from; c < w.to; c += CHUNK, turn++) {
           const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * (turn & 1), (turn >> 1) & 1, gave_up));
           fence_after();
-          const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (turn & 1) * 256 + half * COLS;
+          const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (turn & 1) * 256 + quarter * COLS;
 #pragma unroll
-          for (int i = 0; i < 4; i++) {  // gated: 32 columns of g and 32 of u, else 64 of the product
+          for (int i = 0; i < SUMS; i += 16) {
             uint32_t v[16];
             if (ok) {
-              tmem_load(d + (gated(KIND) ? i / 2 * HALF + i % 2 * 16 : i * 16), v);
+              tmem_load(d + (gated(KIND) && i >= COLS ? HALF + i - COLS : i), v);
               wait_ld(v);
             } else {
               for (int j = 0; j < 16; j++) v[j] = kNaN;
             }
 #pragma unroll
-            for (int j = 0; j < 16; j++) sum[i][j] += __uint_as_float(v[j]);
+            for (int j = 0; j < 16; j++) sum[i + j] += __uint_as_float(v[j]);
           }
           done(turn & 1);
         }
-        if (gated(KIND)) {
-          finish(col0, sum[0], sum[2], sum[2]);
-          finish(col0 + 16, sum[1], sum[3], sum[3]);
+        if (!rows_here) continue;
+        if constexpr (KIND == UP || KIND == DH) {
+#pragma unroll
+          for (int c = 0; c < COLS; c += 8) {
+            const int64_t col = col0 + c;
+            if (col >= g.cols) break;
+            float h[8], dg[8], du[8], gate[8], up[8];
+            if (KIND == DH) {  // rows of g and u are padded to whole pieces
+              const int64_t at = min(row0 + lane, g.rows - 1) * g.ld + col;
+              load_vec<float, 4>(g.gate + at, reinterpret_cast<float(&)[4]>(gate[0]));
+              load_vec<float, 4>(g.gate + at + 4, reinterpret_cast<float(&)[4]>(gate[4]));
+              load_vec<float, 4>(g.up + at, reinterpret_cast<float(&)[4]>(up[0]));
+              load_vec<float, 4>(g.up + at + 4, reinterpret_cast<float(&)[4]>(up[4]));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+              const float u = KIND == DH ? up[i] : sum[(COLS + c + i) % SUMS], dh = sum[c + i];
+              float a, da;
+              activate<ACT, false>(KIND == DH ? gate[i] : sum[c + i], a, da);
+              h[i] = a * u;
+              dg[i] = dh * u * da;
+              du[i] = dh * a;
+            }
+            if (KIND == DH) {
+              emit_parts(g.out0, g, row0, col, dg, stage);
+              emit_parts(g.out1, g, row0, col, du, stage);
+            }
+            emit_parts(KIND == DH ? g.out2 : g.out0, g, row0, col, h, stage);
+          }
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; i++) finish(col0 + i * 16, sum[i], sum[i], sum[i]);
+          for (int c = 0; c < SUMS; c += 8) {
+            uint32_t o[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = __float_as_uint(sum[c + j]);
+            const bool second = KIND == GATES && c >= COLS;
+            const int64_t col = col0 + (second ? c - COLS : c), ld = (g.cols + 3) / 4 * 4;
+            if (KIND != GATES && g.splits > 1)
+              emit<float, 8>(g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld, ld, row0, col, g.rows, ld, 16, o, stage);
+            else
+              emit<float, 8>(static_cast<float*>(second || w.which ? g.out1 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, o, stage);
+          }
         }
       } else {
         const int acc = ACCS == 2 ? turn & 1 : 0;
         const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
         const bool ok = __all_sync(0xffffffffu, mbar_wait(acc_full + 8 * acc, acc_phase, gave_up));
         fence_after();
-        const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (ACCS == 2 ? acc * 256 : 0) + half * COLS;
+        const uint32_t d = tmem + (uint32_t(sub * 32) << 16) + (ACCS == 2 ? acc * 256 : 0) + quarter * COLS;
 #pragma unroll 1
         for (int c = 0; c < COLS; c += 16) {
           __syncwarp();
-          uint32_t v[3][16];
-          if (ok) {
-            tmem_load(d + c, v[0]);
-            if (gated(KIND)) tmem_load(d + HALF + c, v[1]);
-            if (KIND == HIDDEN) tmem_load(d + BN + (turn & 1) * HALF + c, v[2]);
-            wait_ld(v[0]);
-            if (gated(KIND)) wait_ld(v[1]);
-            if (KIND == HIDDEN) wait_ld(v[2]);
-          } else {
-            for (int i = 0; i < 16; i++) v[0][i] = v[1][i] = v[2][i] = kNaN;
-          }
-          if (c + 16 == COLS) done(acc);
-          float f[3][16];
+          const int64_t col = col0 + c;
+          if constexpr (gated(KIND)) {
+            uint32_t h[8], dg[8], du[8];
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            f[0][i] = __uint_as_float(v[0][i]);
-            f[1][i] = __uint_as_float(v[gated(KIND) ? 1 : 0][i]);
-            f[2][i] = __uint_as_float(v[KIND == HIDDEN ? 2 : 0][i]);
+            for (int half = 0; half < 2; half++) {  // eight columns at a time: 640 threads leave 102 registers each
+              uint32_t v[3][8];
+              const uint32_t at = d + c + half * 8;
+              if (ok) {
+                tmem_load(at, v[0]);
+                tmem_load(at + HALF, v[1]);
+                if (KIND == HIDDEN) tmem_load(at + BN + (turn & 1) * HALF, v[2]);
+                wait_ld(v[0]);
+                wait_ld(v[1]);
+                if (KIND == HIDDEN) wait_ld(v[2]);
+              } else {
+                for (int i = 0; i < 8; i++) v[0][i] = v[1][i] = v[2][i] = kNaN;
+              }
+#pragma unroll
+              for (int i = 0; i < 8; i += 2) {
+                float a[2], da[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++) activate<ACT, true>(__uint_as_float(v[0][i + j]), a[j], da[j]);
+                const float u0 = __uint_as_float(v[1][i]), u1 = __uint_as_float(v[1][i + 1]);
+                h[half * 4 + i / 2] = pack2<T>(a[0] * u0, a[1] * u1);
+                if (KIND == HIDDEN) {
+                  const float d0 = __uint_as_float(v[2][i]), d1 = __uint_as_float(v[2][i + 1]);
+                  dg[half * 4 + i / 2] = pack2<T>(d0 * u0 * da[0], d1 * u1 * da[1]);
+                  du[half * 4 + i / 2] = pack2<T>(d0 * a[0], d1 * a[1]);
+                }
+              }
+            }
+            if (c + 16 == COLS) done(acc);
+            if (!rows_here) continue;
+            if (KIND == HIDDEN) {
+              emit<T, 8>(static_cast<T*>(g.out0), g.ld, row0, col, g.rows, g.cols, g.align, dg, stage);
+              emit<T, 8>(static_cast<T*>(g.out1), g.ld, row0, col, g.rows, g.cols, g.align, du, stage);
+            }
+            emit<T, 8>(static_cast<T*>(KIND == HIDDEN ? g.out2 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, h, stage);
+          } else {
+            uint32_t v[16];
+            if (ok) {
+              tmem_load(d + c, v);
+              wait_ld(v);
+            } else {
+              for (int i = 0; i < 16; i++) v[i] = kNaN;
+            }
+            if (c + 16 == COLS) done(acc);
+            if (rows_here) put(col, reinterpret_cast<const float(&)[16]>(v));
           }
-          finish(col0 + c, f[0], f[1], f[2]);
         }
         turn++;
       }
@@ -581,7 +611,7 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ x, 
 // Up to eight tokens need each weight once and little else: a warp reads rows of the weights, 16 bytes a lane, and multiplies
 // them with the tokens, which wait in shared memory in fp32. h stays fp32 between the two kernels. Measured for one token,
 // 1024 x 2816 bf16 (17 MB of weights, 2.7 us at the copy rate): the tensor kernels' pair tiles took 14 + 10 + 3 us.
-constexpr int kFewTokens = 8, kFewBytes = 64 * 1024;  // of fp32 tokens in shared memory, K or F wide
+constexpr int kFewTokens = 8, kFewBytes = 96 * 1024;  // of fp32 tokens in shared memory, K or F wide
 constexpr int kRowWarps = 4;                         // warps that share a row of Wd
 
 template <typename T, int V> __device__ __forceinline__ void to_floats(const Vec<T, V>& v, float (&f)[V]) {
@@ -704,30 +734,34 @@ constexpr size_t kHeader = 256;  // the abort word, as in the loss's workspace
 inline size_t round_up(size_t n) { return (n + 255) / 256 * 256; }
 inline int64_t lead(int64_t cols) { return (cols + 15) / 16 * 16; }  // rows of hidden and packed matrices: 32-byte starts
 
-// How a product is cut into tiles: 256 columns, or 128 where that would leave pairs of SMs without work or columns
-// empty, and then the inner axis over the pairs that are still free.
+// How a product is cut into tiles and its inner axis into splits: the cheapest by a model of the time in clocks. A block of
+// 64 of a tile of 256 columns takes 590 and one of 128 columns 515 (measured; the tensor cores then wait for A's share of
+// shared memory, not for products), a tile 1500 around them; partial sums are written and read at 2200 bytes a clock, and
+// their join costs a launch. Of equal ones the fewest splits.
 struct Cut {
-  int bn, m_tiles, n_tiles, splits;
+  int bn, m_tiles, n_tiles, splits, per_split;
 };
 static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
-  const int pairs = sm_count() / 2;
-  Cut c;
-  c.m_tiles = int(ceil_div(rows, 256));
-  c.bn = 256;
-  c.n_tiles = int(ceil_div(cols, gated(kind) ? 128 : 256));
-  if (dtype == LNCC_F32 ||
-      (kind != HIDDEN && (int64_t(c.m_tiles) * c.n_tiles * whichs < pairs || cols <= (gated(kind) ? 64 : 128)))) {
-    c.bn = 128;
-    c.n_tiles = int(ceil_div(cols, gated(kind) ? 64 : 128));
+  const int pairs = sm_count() / 2, parts = dtype == LNCC_F32 ? 6 : 1;
+  Cut best = {};
+  double least = 0;
+  for (int bn = 256; bn >= 128; bn -= 128) {
+    if (kind == HIDDEN && bn == 128) break;
+    const int width = gated(kind) ? bn / 2 : bn;
+    const int64_t m_tiles = ceil_div(rows, 256), n_tiles = ceil_div(cols, width), tiles = m_tiles * n_tiles * whichs;
+    for (int want = 1; want <= 64; want++) {
+      if (want > 1 && (gated(kind) || kind == DH || blocks < 4 * want)) break;
+      const int64_t per = ceil_div(blocks, want), splits = ceil_div(blocks, per);
+      if (splits != want) continue;
+      double t = double(ceil_div(tiles * splits, pairs)) * (double(per) * parts * (bn == 256 ? 590 : 515) + 1500);
+      if (splits > 1) t += 6000 + 8.0 * double(splits) * whichs * double(rows) * double(cols) / 2200;
+      if (best.bn == 0 || t < 0.98 * least) {
+        best = {bn, int(m_tiles), int(n_tiles), int(splits), int(per)};
+        least = t;
+      }
+    }
   }
-  c.splits = 1;
-  const int64_t tiles = int64_t(c.m_tiles) * c.n_tiles * whichs;
-  if (!gated(kind) && kind != DH && tiles <= pairs / 2) {  // at least 8 blocks for each split
-    const int64_t want = pairs / tiles, most = blocks / 8;
-    c.splits = int(want < most ? want : most);
-    if (c.splits < 1) c.splits = 1;
-  }
-  return c;
+  return best;
 }
 
 // Scratch of a call, laid out in one place for its size and its use.
@@ -856,7 +890,7 @@ struct Call {
     g.k_steps2 = int(k_steps(inner2));
     g.blocks = KIND == DX ? 2 * g.k_steps : KIND == HIDDEN ? g.k_steps + g.k_steps2 : g.k_steps;
     const Cut c = cut_for(KIND, a.dtype, rows, cols, whichs, g.blocks);
-    g.m_tiles = c.m_tiles, g.n_tiles = c.n_tiles, g.splits = c.splits, g.whichs = whichs;
+    g.m_tiles = c.m_tiles, g.n_tiles = c.n_tiles, g.splits = c.splits, g.whichs = whichs, g.per_split = c.per_split;
     const int a_box = a_mn(KIND) ? 64 : 128, b_box = b_mn(KIND) ? 64 : c.bn / 2;
     if (!make_map(&g.a0, a0, a_box) || !make_map(&g.a1, a1, a_box) || !make_map(&g.b0, b0, b_box) ||
         !make_map(&g.b1, b1, b_box) || !make_map(&g.b2, b2, 64)) {
@@ -876,9 +910,9 @@ struct Call {
     g.clear_abort = first;
     first = false;
     if constexpr (KIND == GATES || KIND == DH) {
-      launch_act<KIND, 128, float>(g);
+      launch_type<KIND, float>(g, c.bn);
     } else if (a.dtype == LNCC_F32) {
-      if constexpr (KIND != HIDDEN) launch_act<KIND, 128, float>(g);
+      if constexpr (KIND != HIDDEN) launch_type<KIND, float>(g, c.bn);
     } else if (a.dtype == LNCC_BF16) {
       launch_type<KIND, __nv_bfloat16>(g, c.bn);
     } else {
