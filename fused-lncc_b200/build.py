@@ -112,7 +112,9 @@ def build_torch_ops(force=False, verbose=False):
     cuda = os.path.dirname(os.path.dirname(nvcc_path())) or "/usr/local/cuda"
     includes = [INCLUDE, os.path.join(torch_dir, "include"),
                 os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+    # not $CXX: a compiler that links its own libstdc++ statically gives the library a second one beside torch's, and the
+    # first number printed into an error message crashes
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in includes),
            "-o", out + ".tmp", src, f"-L{LIB_DIR}", f"-l:{os.path.basename(lib)}", f"-L{os.path.join(torch_dir, 'lib')}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]

@@ -6,7 +6,7 @@
 //
 // Every product runs on the tensor cores, in one kernel whose epilogue does what follows it: UP forms g and u side by side
 // in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h (for fp32 GATES
-// writes g and u, and DH forms dh and reads them); the others write a result or, where a long inner axis is split over
+// writes g and u, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is split over
 // the GPU, fp32 partial sums that a last kernel adds in order.
 //
 // A pair of CTAs takes a tile of 256 rows by up to 256 columns (cta_group::2): each loads its 128 rows of A and half the
@@ -61,11 +61,10 @@ struct Gemm {
   int k_steps, k_steps2;     // blocks of 64 of the inner axis (HIDDEN: of g and u, and of dh)
   int blocks, per_split;     // of a tile: k_steps times the products summed into it (DX: 2); those of a split
   int bf16;
-  void *out0, *out1, *out2;  // results (DW_UP: of which = 0, 1; HIDDEN, DH: dg, du, h; GATES: g, u)
-  int64_t ld, plane;         // of the results; plane for hidden results taken apart
+  void *out0, *out1, *out2;  // results (DW_UP: of which = 0, 1; HIDDEN: dg, du, h; GATES: g, u)
+  int64_t ld, plane;         // of the results; plane for h taken apart
   int align;                 // bytes on which every row of the results starts: 32, 16 or the element's
   float* partial;            // [splits][whichs][rows][cols rounded up to 4], where splits > 1
-  const float *gate, *up;    // DH: g and u, rows ld apart
   unsigned* abort_word;
   int clear_abort;
 };
@@ -159,7 +158,7 @@ __device__ __forceinline__ void take_apart(float v, __nv_bfloat16& hi, __nv_bflo
   mid = __float2bfloat16_rn(fine ? r : 0.f);
   lo = __float2bfloat16_rn(fine ? r - __bfloat162float(mid) : 0.f);
 }
-// Eight hidden results of a row in fp32, as the three bf16 matrices that hold them.
+// Eight results of a row in fp32, as the three bf16 matrices that hold them.
 __device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t row0, int64_t col, const float (&v)[8],
                                            uint32_t* stage) {
   float part[3][8];
@@ -197,7 +196,7 @@ __device__ __forceinline__ Tile tile_of(const Gemm& g, int t) {
 }
 
 // T: type of the results (for float, bf16 operands taken apart). KIND, BN: see above; gated kinds hold BN/2 columns of g
-// and of u, HIDDEN BN/2 of dh beside them. ACT: the activation of UP, HIDDEN and DH.
+// and of u, HIDDEN BN/2 of dh beside them. ACT: the activation of UP and HIDDEN.
 template <int KIND, int BN, int ACT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Gemm g) {
   constexpr int STAGES = stages(BN), BT = b_tile(BN), HALF = BN / 2;
@@ -394,33 +393,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           done(turn & 1);
         }
         if (!rows_here) continue;
-        if constexpr (KIND == UP || KIND == DH) {
+        if constexpr (KIND == UP) {
 #pragma unroll
           for (int c = 0; c < COLS; c += 8) {
-            const int64_t col = col0 + c;
-            if (col >= g.cols) break;
-            float h[8], dg[8], du[8], gate[8], up[8];
-            if (KIND == DH) {  // rows of g and u are padded to whole pieces
-              const int64_t at = min(row0 + lane, g.rows - 1) * g.ld + col;
-              load_vec<float, 4>(g.gate + at, reinterpret_cast<float(&)[4]>(gate[0]));
-              load_vec<float, 4>(g.gate + at + 4, reinterpret_cast<float(&)[4]>(gate[4]));
-              load_vec<float, 4>(g.up + at, reinterpret_cast<float(&)[4]>(up[0]));
-              load_vec<float, 4>(g.up + at + 4, reinterpret_cast<float(&)[4]>(up[4]));
-            }
+            if (col0 + c >= g.cols) break;
+            float h[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
-              const float u = KIND == DH ? up[i] : sum[(COLS + c + i) % SUMS], dh = sum[c + i];
               float a, da;
-              activate<ACT, false>(KIND == DH ? gate[i] : sum[c + i], a, da);
-              h[i] = a * u;
-              dg[i] = dh * u * da;
-              du[i] = dh * a;
+              activate<ACT, false>(sum[c + i], a, da);
+              h[i] = a * sum[(COLS + c + i) % SUMS];
             }
-            if (KIND == DH) {
-              emit_parts(g.out0, g, row0, col, dg, stage);
-              emit_parts(g.out1, g, row0, col, du, stage);
-            }
-            emit_parts(KIND == DH ? g.out2 : g.out0, g, row0, col, h, stage);
+            emit_parts(g.out0, g, row0, col0 + c, h, stage);
           }
         } else {
 #pragma unroll
@@ -506,35 +490,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
 }
 
-// Partial sums of the splits: eight strands of splits for each 32 quads of columns, then the strands, each in order.
-template <typename T>
+// Partial sums of the splits, added in order: a thread a quad of columns, or, for many splits of few columns, STRANDS threads
+// with every STRANDS-th split each, whose sums are then added in order.
+constexpr int kManySplits = 16;
+template <typename T, int STRANDS>
 __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, int splits, int whichs, int64_t rows,
                                                    int64_t cols, T* out0, T* out1) {
-  __shared__ float4 meet[8][32];
-  const int strand = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int64_t ld = (cols + 3) / 4 * 4, quads = whichs * rows * (ld / 4), q = int64_t(blockIdx.x) * 32 + lane;
+  constexpr int LANES = 256 / STRANDS;
+  __shared__ float4 meet[STRANDS][LANES];
+  const int strand = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+  const int64_t ld = (cols + 3) / 4 * 4, quads = whichs * rows * (ld / 4), q = int64_t(blockIdx.x) * LANES + lane;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (q < quads) {
 #pragma unroll 4
-    for (int i = strand; i < splits; i += 8) {
+    for (int i = strand; i < splits; i += STRANDS) {
       const float4 v = reinterpret_cast<const float4*>(partial)[i * quads + q];
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
   }
-  meet[strand][lane] = s;
-  __syncthreads();
-  if (strand != 0 || q >= quads) return;
-  for (int i = 1; i < 8; i++) {
-    const float4 v = meet[i][lane];
-    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  if (STRANDS > 1) {
+    meet[strand][lane] = s;
+    __syncthreads();
+    if (strand != 0) return;
+    for (int i = 1; i < STRANDS; i++) {
+      const float4 v = meet[i][lane];
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
   }
-  const int64_t row = q / (ld / 4) % rows, col = q % (ld / 4) * 4;
-  T* out = q / (ld / 4) / rows ? out1 : out0;
-  if (out == nullptr) return;
+  if (q >= quads) return;
+  const uint32_t per_row = uint32_t(ld / 4);
+  const int64_t r = q / per_row, row = r < rows ? r : r - rows, col = (q - r * per_row) * 4;
+  T* out = r < rows ? out0 : out1;
   const float v[4] = {s.x, s.y, s.z, s.w};
+  T* to = out + row * cols + col;
+  if (cols % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(T)) == 0) {
+    if (LNCC_IN(row * cols + col, 4, rows * cols)) store_vec<T, 4>(to, v);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; i++)
-    if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) out[row * cols + col + i] = from_f<T>(v[i]);
+    if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) to[i] = from_f<T>(v[i]);
 }
 
 // A matrix that TMA cannot read as it lies (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows.
@@ -555,6 +550,40 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, in
 #pragma unroll
     for (int k = 0; k < (sizeof(T) == 4 ? 3 : 1); k++)
       *reinterpret_cast<Vec<TO, 8>*>(dst + k * plane + row * ld + col) = o[k];
+  }
+}
+
+// fp32: dg, du and h, taken apart, from g, u and dh (rows ld apart, like the results). Eight neighbours a thread.
+template <int ACT>
+__global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g, const float* __restrict__ u,
+                                                    const float* __restrict__ dh, __nv_bfloat16* dg, __nv_bfloat16* du,
+                                                    __nv_bfloat16* h, int64_t n, int64_t plane) {
+  for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += int64_t(gridDim.x) * 256 * 8) {
+    float vg[8], vu[8], vd[8], o[3][8];
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      load_vec<float, 4>(g + i + k, reinterpret_cast<float(&)[4]>(vg[k]));
+      load_vec<float, 4>(u + i + k, reinterpret_cast<float(&)[4]>(vu[k]));
+      load_vec<float, 4>(dh + i + k, reinterpret_cast<float(&)[4]>(vd[k]));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      float a, da;
+      activate<ACT, false>(vg[k], a, da);
+      o[0][k] = vd[k] * vu[k] * da;
+      o[1][k] = vd[k] * a;
+      o[2][k] = a * vu[k];
+    }
+#pragma unroll
+    for (int r = 0; r < 3; r++) {
+      Vec<__nv_bfloat16, 8> part[3];
+#pragma unroll
+      for (int k = 0; k < 8; k++) take_apart(o[r][k], part[0].e[k], part[1].e[k], part[2].e[k]);
+      __nv_bfloat16* to = (r == 0 ? dg : r == 1 ? du : h) + i;
+#pragma unroll
+      for (int k = 0; k < 3; k++)
+        if (LNCC_IN(i, 8, n)) *reinterpret_cast<Vec<__nv_bfloat16, 8>*>(to + k * plane) = part[k];
+    }
   }
 }
 
@@ -767,7 +796,7 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
 // Scratch of a call, laid out in one place for its size and its use.
 struct Plan {
   int planes;
-  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, partial, total;
+  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, dh, partial, total;
   int64_t ldf;
 };
 static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
@@ -804,6 +833,7 @@ static Plan plan_for(const Args& a, bool backward) {
     if (a.dtype == LNCC_F32) {
       p.gate = at, at += round_up(size_t(a.M) * p.ldf * 4);
       p.up = at, at += round_up(size_t(a.M) * p.ldf * 4);
+      p.dh = at, at += round_up(size_t(a.M) * p.ldf * 4);
     }
     partial(partial_bytes(DX, a.dtype, a.M, a.K, 1, 2 * k_steps(a.F)));
     partial(partial_bytes(DW_UP, a.dtype, a.F, a.K, 2, k_steps(a.M)));
@@ -865,7 +895,7 @@ struct Call {
     product_kernel<KIND, BN, ACT, T><<<unsigned(2 * (tiles < pairs ? tiles : pairs)), kThreads, smem, stream>>>(g);
   }
   template <int KIND, int BN, typename T> void launch_act(Gemm& g) {
-    if constexpr (KIND == UP || KIND == HIDDEN || KIND == DH) {
+    if constexpr (KIND == UP || KIND == HIDDEN) {
       if (a.act == LNCC_ACT_SILU) launch<KIND, BN, LNCC_ACT_SILU, T>(g);
       else if (a.act == LNCC_ACT_GELU) launch<KIND, BN, LNCC_ACT_GELU, T>(g);
       else launch<KIND, BN, LNCC_ACT_RELU, T>(g);
@@ -877,6 +907,15 @@ struct Call {
     if constexpr (KIND == HIDDEN) launch_act<KIND, 256, T>(g);
     else if (bn == 256) launch_act<KIND, 256, T>(g);
     else launch_act<KIND, 128, T>(g);
+  }
+
+  template <typename T> void join(const Gemm& g) {
+    const int64_t quads = g.whichs * g.rows * ceil_div(g.cols, 4);
+    T *out0 = static_cast<T*>(g.out0), *out1 = static_cast<T*>(g.out1);
+    if (g.splits < kManySplits)
+      join_kernel<T, 1><<<unsigned(ceil_div(quads, 256)), 256, 0, stream>>>(g.partial, g.splits, g.whichs, g.rows, g.cols, out0, out1);
+    else
+      join_kernel<T, 8><<<unsigned(ceil_div(quads, 32)), 256, 0, stream>>>(g.partial, g.splits, g.whichs, g.rows, g.cols, out0, out1);
   }
 
   // One product: A (a0, a1) and B (b0, b1, b2) as the kind takes them, results out (rows x cols, ld apart).
@@ -899,13 +938,11 @@ struct Call {
     }
     g.rows = rows, g.cols = cols, g.bf16 = a0.bf16;
     g.out0 = out0, g.out1 = out1, g.out2 = out2, g.ld = ld, g.plane = plane;
-    const int es = KIND == UP || KIND == HIDDEN || KIND == DH ? 2 : elem_size(a.dtype);
+    const int es = KIND == UP || KIND == HIDDEN ? 2 : elem_size(a.dtype);
     g.align = es;
     for (int al = 16; al <= 32; al *= 2)
       if (aligned(out0, al) && aligned(out1, al) && aligned(out2, al) && ld * es % al == 0) g.align = al;
     g.partial = reinterpret_cast<float*>(scratch + plan.partial);
-    g.gate = reinterpret_cast<const float*>(scratch + plan.gate);
-    g.up = reinterpret_cast<const float*>(scratch + plan.up);
     g.abort_word = reinterpret_cast<unsigned*>(scratch);
     g.clear_abort = first;
     first = false;
@@ -919,16 +956,9 @@ struct Call {
       launch_type<KIND, __half>(g, c.bn);
     }
     if (g.splits > 1 && status == LNCC_OK) {
-      const unsigned grid = unsigned(ceil_div(whichs * rows * ceil_div(cols, 4), 32));
-      if (a.dtype == LNCC_F32)
-        join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<float*>(out0),
-                                              static_cast<float*>(out1));
-      else if (a.dtype == LNCC_BF16)
-        join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<__nv_bfloat16*>(out0),
-                                              static_cast<__nv_bfloat16*>(out1));
-      else
-        join_kernel<<<grid, 256, 0, stream>>>(g.partial, g.splits, whichs, rows, cols, static_cast<__half*>(out0),
-                                              static_cast<__half*>(out1));
+      if (a.dtype == LNCC_F32) join<float>(g);
+      else if (a.dtype == LNCC_BF16) join<__nv_bfloat16>(g);
+      else join<__half>(g);
     }
     if (cudaPeekAtLastError() != cudaSuccess) status = LNCC_ERR_LAUNCH;
   }
@@ -945,9 +975,10 @@ template <typename T, int V, int MT> static int few_run(const Args& a, float* h,
   const auto down = few_down_kernel<T, V, MT>;
   const int up_smem = int(MT * ceil_div(a.K, 32 * V) * 32 * V * 4), step = 32 * V * kRowWarps;
   const int down_smem = int(MT * ceil_div(a.F, step) * step * 4);
-  if (up_smem > 48 * 1024 && cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, up_smem) != cudaSuccess)
+  constexpr int kFree = 40 * 1024;  // dynamic shared memory that any kernel may have beside its static
+  if (up_smem > kFree && cudaFuncSetAttribute(up, cudaFuncAttributeMaxDynamicSharedMemorySize, up_smem) != cudaSuccess)
     return LNCC_ERR_SMEM;
-  if (down_smem > 48 * 1024 && cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, down_smem) != cudaSuccess)
+  if (down_smem > kFree && cudaFuncSetAttribute(down, cudaFuncAttributeMaxDynamicSharedMemorySize, down_smem) != cudaSuccess)
     return LNCC_ERR_SMEM;
   const int64_t most = int64_t(sm_count()) * 4, up_blocks = ceil_div(a.F, 8), down_blocks = ceil_div(a.N, 8 / kRowWarps);
   up<<<unsigned(up_blocks < most ? up_blocks : most), 256, up_smem, st>>>(
@@ -1006,7 +1037,13 @@ static int backward(const Args& a, void* scratch, cudaStream_t stream) {
     if (a.act == LNCC_ACT_RELU)
       gate_kernel<<<dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, stream>>>(
           static_cast<const float*>(a.x), a.x_stride, static_cast<const float*>(a.wg), gate, h.ld, a.M, a.F, a.K);
-    c.product<DH>(dy, dy, wd, wd, wd, a.M, a.F, 1, a.N, 0, dg.p, du.p, h.p, h.ld, h.plane);
+    float *const up = reinterpret_cast<float*>(c.scratch + c.plan.up), *const dhp = reinterpret_cast<float*>(c.scratch + c.plan.dh);
+    c.product<DH>(dy, dy, wd, wd, wd, a.M, a.F, 1, a.N, 0, dhp, nullptr, nullptr, h.ld, 0);
+    const auto parts = a.act == LNCC_ACT_SILU ? parts_kernel<LNCC_ACT_SILU>
+                       : a.act == LNCC_ACT_GELU ? parts_kernel<LNCC_ACT_GELU> : parts_kernel<LNCC_ACT_RELU>;
+    const int64_t n = a.M * h.ld, blocks = ceil_div(n, 2048), most = int64_t(sm_count()) * 8;
+    parts<<<unsigned(blocks < most ? blocks : most), 256, 0, stream>>>(
+        gate, up, dhp, static_cast<__nv_bfloat16*>(dg.p), static_cast<__nv_bfloat16*>(du.p), static_cast<__nv_bfloat16*>(h.p), n, h.plane);
   } else {
     c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
   }

@@ -65,6 +65,35 @@ def test_refusals_without_gpu():
         fused_lncc.fused_gated_ffn(x, x, x, x, activation="tanh")
 
 
+def test_refusals_of_fake_cuda_tensors():
+    """Every check of shapes, types and devices, without a GPU: fake tensors that say they are on one."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    ln, scan, ffn = fused_lncc.fused_layer_norm, fused_lncc.fused_gated_scan, fused_lncc.fused_gated_ffn
+    with FakeTensorMode():
+        x, w, d = (torch.zeros(s, device="cuda") for s in ((4, 8), (16, 8), (8, 16)))
+        half = torch.zeros(8, device="cuda", dtype=torch.float16)
+        for call, why in ((lambda: ln(x.double()), "float32"), (lambda: ln(x, torch.zeros(7, device="cuda")), r"\(7\)"),
+                          (lambda: ln(x, torch.zeros(8)), "CUDA"), (lambda: ln(x, half), "Half"),
+                          (lambda: ln(x.half(), torch.zeros(8, device="cuda"), half), "one type"),
+                          (lambda: ln(x[:, :0]), "C >= 1"), (lambda: scan(x, x), r"\(B, T, C\)"),
+                          (lambda: scan(x[None], x[None].half()), "Half"), (lambda: scan(x[None], x[None, :3]), r"\(1, 3, 8\)"),
+                          (lambda: scan(x[None], x[None], x), r"\(4, 8\)"), (lambda: ffn(x, w, w, w), r"w_down \(N, F\)"),
+                          (lambda: ffn(x, w, w[:8], d), r"\(8, 8\)"), (lambda: ffn(x.half(), w, w, d), "Half"),
+                          (lambda: ffn(x, w[0], w, d), "matrix"), (lambda: ffn(x, w, w, d.cpu()), "CUDA")):
+            with pytest.raises(RuntimeError, match=why):
+                call()
+
+
+def test_torch_library_brings_no_second_libstdcxx():
+    """One that defines std::ostream itself crashes on the first number in an error message."""
+    import subprocess
+
+    from fused_lncc import _native
+    _native.load()
+    out = subprocess.run(["nm", "-D", "--defined-only", _native.OPS_PATH], capture_output=True, text=True, check=True).stdout
+    assert "_ZNSo9_M_insert" not in out
+
+
 def test_custom_ops_registered():
     for name in ("layer_norm", "layer_norm_backward", "gated_scan", "gated_scan_backward", "gated_ffn",
                  "gated_ffn_backward"):

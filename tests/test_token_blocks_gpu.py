@@ -302,7 +302,7 @@ def _ffn_tensors(M, K, F, N, dtype, seed, act="silu"):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("M,K,F,N,act", [
     (1, 64, 128, 64, "silu"), (1, 33, 51, 27, "gelu"), (2, 256, 512, 256, "relu"), (5, 96, 264, 96, "silu"),
-    (8, 128, 384, 128, "gelu"), (9, 200, 504, 200, "silu"), (16, 1024, 640, 72, "silu"), (17, 40, 1001, 8, "gelu"),
+    (8, 128, 384, 128, "gelu"), (4, 1024, 2816, 1024, "silu"), (3, 1000, 3001, 500, "silu"), (8, 2040, 1024, 96, "gelu"), (9, 200, 504, 200, "silu"), (16, 1024, 640, 72, "silu"), (17, 40, 1001, 8, "gelu"),
     (63, 96, 256, 96, "gelu"), (127, 64, 64, 64, "silu"), (128, 128, 128, 128, "relu"), (129, 136, 200, 136, "silu"),
     (300, 389, 1037, 389, "gelu"), (1000, 96, 256, 96, "gelu"), (513, 768, 1000, 768, "silu"), (700, 8, 16, 1000, "relu"),
     (2049, 72, 88, 104, "silu"), (260, 520, 260, 515, "silu")])
