@@ -637,24 +637,33 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ x, 
 }
 
 // ---- a few tokens ----------------------------------------------------------------------------------------------------
-// Up to eight tokens need each weight once and little else: a warp reads rows of the weights, 16 bytes a lane, and multiplies
-// them with the tokens, which wait in shared memory in fp32. h stays fp32 between the two kernels. Measured for one token,
+// Up to four tokens need each weight once and little else: a warp reads rows of the weights, 16 bytes a lane, and multiplies
+// them with the tokens, which wait in shared memory in fp32 (of each eight the first four in one half of the row and the last
+// four in the other, so that lanes read 16 bytes side by side). h stays fp32 between the two kernels. Measured for one token,
 // 1024 x 2816 bf16 (17 MB of weights, 2.7 us at the copy rate): the tensor kernels' pair tiles took 14 + 10 + 3 us.
-constexpr int kFewTokens = 8, kFewBytes = 96 * 1024;  // of fp32 tokens in shared memory, K or F wide
+constexpr int kFewTokens = 4, kFewBytes = 96 * 1024;  // of fp32 tokens in shared memory, K or F wide
 constexpr int kRowWarps = 4;                         // warps that share a row of Wd
 
 template <typename T, int V> __device__ __forceinline__ void to_floats(const Vec<T, V>& v, float (&f)[V]) {
 #pragma unroll
   for (int i = 0; i < V; i++) f[i] = to_f(v.e[i]);
 }
+// where element k of a token lies in its row of `width`
+template <int V> __device__ __forceinline__ int token_place(int k, int width) {
+  return V == 8 ? k / 8 * 4 + k % 4 + (k & 4 ? width / 2 : 0) : k;
+}
 // acc[m] += sum over this lane's V elements of w[at] x[m][at]
 template <int V, int MT>
-__device__ __forceinline__ void multiply(const float (&w)[V], const float* x, int64_t width, int64_t at, float (&acc)[MT]) {
+__device__ __forceinline__ void multiply(const float (&w)[V], const float* x, int width, int at, float (&acc)[MT]) {
+  constexpr int PIECE = V == 8 ? 4 : V;
 #pragma unroll
   for (int m = 0; m < MT; m++) {
-    const Vec<float, V> t = *reinterpret_cast<const Vec<float, V>*>(x + m * width + at);
 #pragma unroll
-    for (int i = 0; i < V; i++) acc[m] = fmaf(w[i], t.e[i], acc[m]);
+    for (int j = 0; j < V; j += PIECE) {
+      const Vec<float, PIECE> t = *reinterpret_cast<const Vec<float, PIECE>*>(x + m * width + token_place<V>(at + j, width));
+#pragma unroll
+      for (int i = 0; i < PIECE; i++) acc[m] = fmaf(w[j + i], t.e[i], acc[m]);
+    }
   }
 }
 __device__ __forceinline__ float warp_sum(float v) {
@@ -671,22 +680,41 @@ __global__ void __launch_bounds__(256) few_up_kernel(const T* __restrict__ x, in
   extern __shared__ __align__(128) float tokens[];  // [MT][width], zeros past M and K
   asm volatile("griddepcontrol.launch_dependents;");
   if (blockIdx.x == 0 && threadIdx.x == 0) *abort_word = 0u;  // these kernels wait for nothing
-  const int64_t width = (K + 32 * V - 1) / (32 * V) * (32 * V);
-  for (int64_t i = threadIdx.x; i < MT * width; i += 256) {
-    const int64_t m = i / width, k = i % width;
-    tokens[i] = m < M && k < K ? to_f(x[m * x_stride + k]) : 0.f;
-  }
-  __syncthreads();
+  const int width = int((K + 32 * V - 1) / (32 * V) * (32 * V));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  for (int64_t f = int64_t(blockIdx.x) * 8 + warp; f < F; f += int64_t(gridDim.x) * 8) {
+  constexpr int HELD = 4, STEP = 32 * V;  // loads of each matrix under way at once; the first ones before the tokens are here
+  typedef Vec<T, V> W;
+  W held_g[HELD], held_u[HELD];
+  const auto load = [&](int64_t f, int from) {
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+      if (f < F && from + i * STEP < K) {  // K is a multiple of V
+        held_g[i] = *reinterpret_cast<const W*>(wg + f * K + from + i * STEP);
+        held_u[i] = *reinterpret_cast<const W*>(wu + f * K + from + i * STEP);
+      }
+    }
+  };
+  const int64_t first_f = int64_t(blockIdx.x) * 8 + warp;
+  const int first = lane * V;
+  load(first_f, first);
+  for (int m = 0; m < MT; m++)
+    for (int k = threadIdx.x; k < width; k += 256)
+      tokens[m * width + token_place<V>(k, width)] = m < M && k < K ? to_f(x[m * x_stride + k]) : 0.f;
+  __syncthreads();
+  for (int64_t f = first_f; f < F; f += int64_t(gridDim.x) * 8) {
     float ag[MT] = {}, au[MT] = {};
-#pragma unroll 4
-    for (int64_t k = lane * V; k < K; k += 32 * V) {  // K is a multiple of V
-      float g[V], u[V];
-      to_floats(*reinterpret_cast<const Vec<T, V>*>(wg + f * K + k), g);
-      to_floats(*reinterpret_cast<const Vec<T, V>*>(wu + f * K + k), u);
-      multiply<V, MT>(g, tokens, width, k, ag);
-      multiply<V, MT>(u, tokens, width, k, au);
+    for (int from = first; from < K; from += HELD * STEP) {
+      if (from != first || f != first_f) load(f, from);
+#pragma unroll
+      for (int i = 0; i < HELD; i++) {
+        if (from + i * STEP < K) {
+          float g[V], u[V];
+          to_floats(held_g[i], g);
+          to_floats(held_u[i], u);
+          multiply<V, MT>(g, tokens, width, from + i * STEP, ag);
+          multiply<V, MT>(u, tokens, width, from + i * STEP, au);
+        }
+      }
     }
 #pragma unroll
     for (int m = 0; m < MT; m++) {
@@ -706,10 +734,10 @@ __global__ void __launch_bounds__(256) few_down_kernel(const float* __restrict__
   __shared__ float meet[8][MT];
   constexpr int ROWS = 8 / kRowWarps, STEP = 32 * V * kRowWarps, HELD = 4;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, mine = warp % kRowWarps;
-  const int64_t width = (F + STEP - 1) / STEP * STEP, first = (mine * 32 + lane) * V;
+  const int width = int((F + STEP - 1) / STEP * STEP), first = (mine * 32 + lane) * V;
   typedef Vec<T, V> W;
   W held[HELD];
-  const auto load = [&](int64_t n, int64_t from) {
+  const auto load = [&](int64_t n, int from) {
 #pragma unroll
     for (int i = 0; i < HELD; i++)
       if (n < N && from + i * STEP < F) held[i] = *reinterpret_cast<const W*>(wd + n * F + from + i * STEP);
@@ -717,14 +745,13 @@ __global__ void __launch_bounds__(256) few_down_kernel(const float* __restrict__
   int64_t n = int64_t(blockIdx.x) * ROWS + warp / kRowWarps;
   load(n, first);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int64_t i = threadIdx.x; i < MT * width; i += 256) {
-    const int64_t m = i / width, f = i % width;
-    tokens[i] = m < M && f < F ? h[m * F + f] : 0.f;
-  }
+  for (int m = 0; m < MT; m++)
+    for (int f = threadIdx.x; f < width; f += 256)
+      tokens[m * width + token_place<V>(f, width)] = m < M && f < F ? h[m * F + f] : 0.f;
   __syncthreads();
   for (int64_t n0 = int64_t(blockIdx.x) * ROWS; n0 < N; n0 += int64_t(gridDim.x) * ROWS) {
     float acc[MT] = {};
-    for (int64_t from = first; from < F; from += HELD * STEP) {
+    for (int from = first; from < F; from += HELD * STEP) {
       if (from != first || n0 != int64_t(blockIdx.x) * ROWS) load(n, from);
 #pragma unroll
       for (int i = 0; i < HELD; i++) {
@@ -964,7 +991,7 @@ struct Call {
   }
 };
 
-static int tokens_of(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : M <= 4 ? 4 : 8; }
+static int tokens_of(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : 4; }
 static bool few(const Args& a) {
   const int64_t widest = (a.K > a.F ? a.K : a.F) + 1024;  // rounded up to a block's step
   return a.M <= kFewTokens && tokens_of(a.M) * widest * 4 <= kFewBytes;
@@ -998,8 +1025,7 @@ template <typename T, int V> static int few_tokens(const Args& a, float* h, cuda
   switch (tokens_of(a.M)) {
     case 1: return few_run<T, V, 1>(a, h, st);
     case 2: return few_run<T, V, 2>(a, h, st);
-    case 4: return few_run<T, V, 4>(a, h, st);
-    default: return few_run<T, V, 8>(a, h, st);
+    default: return few_run<T, V, 4>(a, h, st);
   }
 }
 template <typename T> static int few_forward(const Args& a, void* scratch, cudaStream_t st) {
