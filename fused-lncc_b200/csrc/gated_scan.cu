@@ -40,26 +40,61 @@ struct Args {
   int runs, run_blocks;    // runs of a sequence; blocks of them
 };
 
-// a = sigmoid(g) and keep = 1 - a = sigmoid(-g), each to a few u32 of itself (1 - a would cancel for open gates):
-// e = exp(-|g|) by the exponential of 2, for fp32 with the rounding of |g| log2 e carried along, and 1 / (1 + e), for fp32
-// with one step of Newton's. 16-bit types take both as they come: e is off by |g| u32 at most, far below their own u.
-template <bool EXACT> __device__ __forceinline__ void gates(float g, float& a, float& keep) {
-  const float z = -fabsf(g);
-  float t = z * 1.4426950408889634f, e, r;
-  if (EXACT) {
-    const float lost = fmaf(z, 1.4426950408889634f, -t) + z * 1.925963033e-8f;  // log2 e = 1.44269502162933 + 1.93e-8
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-    e = z > -126.f ? fmaf(e, lost * 0.69314718f, e) : 0.f;
+// V channels' products and sums; two channels as one packed instruction.
+template <int V> __device__ __forceinline__ void mul(const float (&a)[V], const float (&b)[V], float (&d)[V]) {
+  if constexpr (V == 2)
+    asm("{\n\t.reg .b64 A, B;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmul.rn.f32x2 A, A, B;\n\tmov.b64 {%0, %1}, A;\n\t}"
+        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+  else
+    for (int v = 0; v < V; v++) d[v] = a[v] * b[v];
+}
+template <int V> __device__ __forceinline__ void fma(const float (&a)[V], const float (&b)[V], const float (&c)[V], float (&d)[V]) {
+  if constexpr (V == 2)
+    asm("{\n\t.reg .b64 A, B, C;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmov.b64 C, {%6, %7};\n\tfma.rn.f32x2 A, A, B, C;\n\t"
+        "mov.b64 {%0, %1}, A;\n\t}"
+        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+  else
+    for (int v = 0; v < V; v++) d[v] = fmaf(a[v], b[v], c[v]);
+}
+
+// a = sigmoid(g) and keep = 1 - a = sigmoid(-g), each to a few u32 of itself (1 - a would cancel for open gates).
+// fp32: e = exp(-|g|) by the exponential of 2, with the rounding of |g| log2 e carried along, and 1 / (1 + e) with one step of
+// Newton's; gates of -inf and +inf give exactly 0 and 1. 16-bit types: e = exp(-g), held below 2^126 so that its reciprocal
+// stays a normal number (a then is 1e-38 where it should be less), a = 1 / (1 + e), keep = e a: e is off by |g| u32 at
+// most, far below their own u. The two special functions of each gate, at 16 an SM and clock, are what bounds 16-bit scans
+// next to their bytes: at 16.8M gates 7.5 us a pass over them.
+template <bool EXACT, int V> __device__ __forceinline__ void gates(const float (&g)[V], float (&a)[V], float (&keep)[V]) {
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      const float z = -fabsf(g[v]), t = z * 1.4426950408889634f;
+      const float lost = fmaf(z, 1.4426950408889634f, -t) + z * 1.925963033e-8f;  // log2 e = 1.44269502162933 + 1.93e-8
+      float e, r;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+      e = z > -126.f ? fmaf(e, lost * 0.69314718f, e) : 0.f;
+      const float d = 1.f + e;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+      r = fmaf(r, fmaf(-d, r, 1.f), r);
+      const float er = e * r;
+      a[v] = g[v] >= 0.f ? r : er;
+      keep[v] = g[v] >= 0.f ? er : r;
+      if (g[v] != g[v]) a[v] = keep[v] = g[v];
+    }
   } else {
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    float t[V], e[V], d[V], minus_log2e[V], one[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) minus_log2e[v] = -1.44269504f, one[v] = 1.f;
+    mul<V>(g, minus_log2e, t);
+#pragma unroll
+    for (int v = 0; v < V; v++) {
+      asm("min.NaN.f32 %0, %1, 0f42FB0000;" : "=f"(t[v]) : "f"(t[v]));  // 125.5
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e[v]) : "f"(t[v]));
+    }
+    fma<V>(e, one, one, d);
+#pragma unroll
+    for (int v = 0; v < V; v++) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a[v]) : "f"(d[v]));
+    mul<V>(e, a, keep);
   }
-  const float d = 1.f + e;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  if (EXACT) r = fmaf(r, fmaf(-d, r, 1.f), r);
-  const float er = e * r;
-  a = g >= 0.f ? r : er;
-  keep = g >= 0.f ? er : r;
-  if (EXACT && g != g) a = keep = g;
 }
 
 // A register's worth of channels.
@@ -184,7 +219,10 @@ template <typename T, int V> struct Steps {
   // The empty statement keeps the arithmetic on step i from moving ahead of the step before it: done for all steps at
   // once it would take hundreds of registers.
   __device__ __forceinline__ void open(int i) { Word<sizeof(T) * V>::pin(e[i]); }
-  __device__ __forceinline__ float get(int i, int v) const { return to_f(reinterpret_cast<const Vec<T, V>&>(e[i]).e[v]); }
+  __device__ __forceinline__ void get(int i, float (&f)[V]) const {
+#pragma unroll
+    for (int v = 0; v < V; v++) f[v] = to_f(reinterpret_cast<const Vec<T, V>&>(e[i]).e[v]);
+  }
 };
 
 // the kernel's launch may begin before the one ahead of it in the stream has ended; what that one wrote is read after this
@@ -209,13 +247,12 @@ template <typename T, int V, int LANES> __global__ void __launch_bounds__(kThrea
       for (int i = 0; i < kKeep; i++) {
         if (!FULL && t + i >= at.to) break;
         sg.open(i), sx.open(i);
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-          float a, keep;
-          gates<sizeof(T) == 4>(sg.get(i, v), a, keep);
-          S[v] = fmaf(a, S[v], keep * sx.get(i, v));
-          A[v] *= a;
-        }
+        float g[V], x_t[V], a[V], keep[V];
+        sg.get(i, g), sx.get(i, x_t);
+        gates<sizeof(T) == 4, V>(g, a, keep);
+        mul<V>(keep, x_t, keep);
+        fma<V>(a, S, keep, S);
+        mul<V>(A, a, A);
       }
     };
     int64_t t = at.from;
@@ -251,12 +288,11 @@ template <typename T, int V, int LANES, bool SPLIT> __global__ void __launch_bou
     for (int i = 0; i < kKeep; i++, to += p.out_t) {
       if (!FULL && t + i >= at.to) break;
       sg.open(i), sx.open(i);
-#pragma unroll
-      for (int v = 0; v < V; v++) {
-        float a, keep;
-        gates<sizeof(T) == 4>(sg.get(i, v), a, keep);
-        h[v] = fmaf(a, h[v], keep * sx.get(i, v));
-      }
+      float g[V], x_t[V], a[V], keep[V];
+      sg.get(i, g), sx.get(i, x_t);
+      gates<sizeof(T) == 4, V>(g, a, keep);
+      mul<V>(keep, x_t, keep);
+      fma<V>(a, h, keep, h);
       store_vec<T, V>(to, h);
     }
   };
@@ -285,13 +321,13 @@ template <typename T, int V, int LANES> __global__ void __launch_bounds__(kThrea
       for (int i = kKeep - 1; i >= 0; i--) {
         if (!FULL && t + i >= at.to) continue;
         sg.open(i), sd.open(i);
+        float g[V], d[V], a[V], keep[V];
+        sg.get(i, g), sd.get(i, d);
+        gates<sizeof(T) == 4, V>(g, a, keep);
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-          float a, keep;
-          gates<sizeof(T) == 4>(sg.get(i, v), a, keep);
-          S[v] = a * (S[v] + sd.get(i, v));
-          A[v] *= a;
-        }
+        for (int v = 0; v < V; v++) d[v] += S[v];
+        mul<V>(a, d, S);
+        mul<V>(A, a, A);
       }
     };
     int64_t t = (at.to - 1) / kKeep * kKeep;
@@ -327,29 +363,30 @@ template <typename T, int V, int LANES, bool SPLIT> __global__ void __launch_bou
     for (int i = 0; i < kKeep; i++) {
       if (!FULL && t + i >= at.to) break;
       sg.open(i), sx.open(i);
+      float g[V], x_t[V], a[V], keep[V];
+      sg.get(i, g), sx.get(i, x_t);
+      gates<sizeof(T) == 4, V>(g, a, keep);
 #pragma unroll
-      for (int v = 0; v < V; v++) {
-        float a, keep;
-        gates<sizeof(T) == 4>(sg.get(i, v), a, keep);
-        apart[i][v] = h[v] - sx.get(i, v);
-        h[v] = fmaf(a, h[v], keep * sx.get(i, v));
-      }
+      for (int v = 0; v < V; v++) apart[i][v] = h[v] - x_t[v];
+      mul<V>(keep, x_t, keep);
+      fma<V>(a, h, keep, h);
     }
     T *to_x = dx + (t + kKeep - 1) * p.out_t, *to_gate = dgate + (t + kKeep - 1) * p.out_t;
 #pragma unroll
     for (int i = kKeep - 1; i >= 0; i--, to_x -= p.out_t, to_gate -= p.out_t) {
       if (!FULL && t + i >= at.to) continue;
       sg.open(i), sd.open(i);
-      float ox[V], og[V];
+      float g[V], d[V], a[V], keep[V], ox[V], og[V], aq[V];
+      sg.get(i, g), sd.get(i, d);
+      gates<sizeof(T) == 4, V>(g, a, keep);
 #pragma unroll
-      for (int v = 0; v < V; v++) {
-        float a, keep;
-        gates<sizeof(T) == 4>(sg.get(i, v), a, keep);
-        q[v] += sd.get(i, v);
-        ox[v] = keep * q[v];
-        og[v] = q[v] * apart[i][v] * (a * keep);
-        q[v] *= a;
-      }
+      for (int v = 0; v < V; v++) q[v] += d[v];
+      mul<V>(keep, q, ox);
+      mul<V>(a, q, aq);
+      mul<V>(ox, apart[i], og);
+      mul<V>(og, a, og);
+#pragma unroll
+      for (int v = 0; v < V; v++) q[v] = aq[v];
       store_vec<T, V>(to_x, ox);
       store_vec<T, V>(to_gate, og);
     }
