@@ -6,7 +6,7 @@
 //
 // Every product runs on the tensor cores, in one kernel whose epilogue does what follows it: UP forms g and u side by side
 // in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h (for fp32 GATES
-// writes g and u, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is split over
+// writes g and u, or ONE_GATE u alone, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is split over
 // the GPU, fp32 partial sums that a last kernel adds in order.
 //
 // A pair of CTAs takes a tile of 256 rows by up to 256 columns (cta_group::2): each loads its 128 rows of A and half the
@@ -37,7 +37,7 @@ using namespace tc;
 
 constexpr uint32_t kNaN = 0x7fffffff;  // what a tile gets whose products were given up
 
-enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
+enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN, ONE_GATE };
 
 constexpr int kEpilogueWarps = 16;         // of a CTA: four for each quarter of the lanes of tensor memory
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0 TMA, 1 products, 4 - 19 epilogue
@@ -177,6 +177,13 @@ __device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t ro
   }
 }
 
+// A call's kernels but the first are launched before the one ahead has ended. Each lets the next begin at once and waits here
+// before it touches memory, so that one kernel's set-up hides behind the other's end.
+__device__ __forceinline__ void begin_after_previous() {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // One tile: 256 rows m, columns n, one of the results, blocks [from, to) of its inner axis. One division where nothing is
 // split: the thread that issues the products works this out between tiles, and the tensor cores wait for it (five
 // divisions, two of them of 64 bits, cost UP 24 of 198 us).
@@ -216,7 +223,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cta_rank();
 
-  if (g.clear_abort && blockIdx.x == 0 && threadIdx.x == 0) *g.abort_word = 0u;  // waits give up seconds later
   if (threadIdx.x == 0) {
     gave_up_flag = 0;
     for (int i = 0; i < STAGES; i++) {
@@ -237,7 +243,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   __syncthreads();
   cluster_sync();
   fence_after();
+  begin_after_previous();  // all of the above runs while the kernel before this one ends
   const uint32_t tmem = tmem_at;
+  if (g.clear_abort && blockIdx.x == 0 && threadIdx.x == 0) *g.abort_word = 0u;  // waits give up seconds later
   const int pairs_at_work = gridDim.x / 2, tiles = g.n_tiles * g.m_tiles * g.whichs * g.splits;
 
   if (warp == 0 && lane == 0) {
@@ -498,6 +506,7 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
                                                    int64_t cols, T* out0, T* out1) {
   constexpr int LANES = 256 / STRANDS;
   __shared__ float4 meet[STRANDS][LANES];
+  begin_after_previous();
   const int strand = threadIdx.x / LANES, lane = threadIdx.x % LANES;
   const int64_t ld = (cols + 3) / 4 * 4, quads = whichs * rows * (ld / 4), q = int64_t(blockIdx.x) * LANES + lane;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -532,24 +541,40 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) to[i] = from_f<T>(v[i]);
 }
 
-// A matrix that TMA cannot read as it lies (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows.
-template <typename T, typename TO>
-__global__ void __launch_bounds__(256) pack_kernel(const T* __restrict__ src, int64_t stride, int64_t rows, int64_t cols,
-                                                   TO* dst, int64_t ld, int64_t plane) {
-  const int64_t eights = rows * (ld / 8);
-  for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < eights; q += int64_t(gridDim.x) * 256) {
-    const int64_t row = q / (ld / 8), col = q % (ld / 8) * 8;
+// Matrices that TMA cannot read as they lie (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows: up to
+// five in one launch, each with blocks of its own.
+struct Pack {
+  const void* src;
+  void* dst;
+  int64_t stride, rows, cols, ld, plane;
+  int first_block;
+};
+struct Packs {
+  Pack job[5];
+  int jobs, blocks;
+};
+template <typename T, typename TO> __global__ void __launch_bounds__(256) pack_kernel(const Packs p) {
+  begin_after_previous();
+  int j = 0;
+  while (j + 1 < p.jobs && int(blockIdx.x) >= p.job[j + 1].first_block) j++;
+  const Pack& m = p.job[j];
+  const T* src = static_cast<const T*>(m.src);
+  TO* dst = static_cast<TO*>(m.dst);
+  const uint32_t per_row = uint32_t(m.ld / 8), blocks = (j + 1 < p.jobs ? p.job[j + 1].first_block : p.blocks) - m.first_block;
+  const int64_t eights = m.rows * per_row;
+  for (int64_t q = int64_t(blockIdx.x - m.first_block) * 256 + threadIdx.x; q < eights; q += int64_t(blocks) * 256) {
+    const int64_t row = q / per_row, col = (q - row * per_row) * 8;
     Vec<TO, 8> o[3];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const T v = col + i < cols && LNCC_IN(row * stride + col + i, 1, (rows - 1) * stride + cols) ? src[row * stride + col + i]
-                                                                                                  : from_f<T>(0.f);
+      const T v = col + i < m.cols && LNCC_IN(row * m.stride + col + i, 1, (m.rows - 1) * m.stride + m.cols)
+                      ? src[row * m.stride + col + i] : from_f<T>(0.f);
       if constexpr (sizeof(T) == 4) take_apart(v, o[0].e[i], o[1].e[i], o[2].e[i]);
       else o[0].e[i] = v;
     }
 #pragma unroll
     for (int k = 0; k < (sizeof(T) == 4 ? 3 : 1); k++)
-      *reinterpret_cast<Vec<TO, 8>*>(dst + k * plane + row * ld + col) = o[k];
+      *reinterpret_cast<Vec<TO, 8>*>(dst + k * m.plane + row * m.ld + col) = o[k];
   }
 }
 
@@ -558,6 +583,7 @@ template <int ACT>
 __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g, const float* __restrict__ u,
                                                     const float* __restrict__ dh, __nv_bfloat16* dg, __nv_bfloat16* du,
                                                     __nv_bfloat16* h, int64_t n, int64_t plane) {
+  begin_after_previous();
   for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += int64_t(gridDim.x) * 256 * 8) {
     float vg[8], vu[8], vd[8], o[3][8];
 #pragma unroll
@@ -589,15 +615,17 @@ __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g,
 
 // g = x Wg^T by fp32 multiply-adds in the order of k, for the backward pass of ReLU in fp32 alone: the derivative jumps at
 // g = 0, where the last bit of g decides, so g is the plain fp32 sum there. A block takes 128 x 128, a thread 8 x 8 of it,
-// 16 of k at a time through shared memory; the next 16 are loaded while these are summed.
+// two columns a packed multiply-add, 16 of k at a time through two buffers of shared memory.
 constexpr int kTile = 128, kInner = 16;
-__global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ x, int64_t x_stride,
-                                                   const float* __restrict__ w, float* out, int64_t ld, int64_t M, int64_t N,
-                                                   int64_t K) {
-  __shared__ __align__(16) float sa[kInner][kTile + 4], sb[kInner][kTile + 4];
+__global__ void __launch_bounds__(256, 2) gate_kernel(const float* __restrict__ x, int64_t x_stride,
+                                                      const float* __restrict__ w, float* out, int64_t ld, int64_t M, int64_t N,
+                                                      int64_t K) {
+  begin_after_previous();
+  __shared__ __align__(16) float sa[2][kInner][kTile + 4], sb[2][kInner][kTile + 4];
   const int64_t m0 = int64_t(blockIdx.x) * kTile, n0 = int64_t(blockIdx.y) * kTile;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // also: column of k, and first row, of the thread's loads
-  float acc[8][8] = {}, la[8], lb[8];
+  uint64_t acc[8][4] = {};  // pairs of columns
+  float la[8], lb[8];
   const auto load = [&](int64_t k) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -606,33 +634,50 @@ __global__ void __launch_bounds__(256) gate_kernel(const float* __restrict__ x, 
       lb[i] = n0 + r < N && k + tx < K ? w[(n0 + r) * K + k + tx] : 0.f;
     }
   };
-  load(0);
-  for (int64_t k0 = 0; k0 < K; k0 += kInner) {
-    __syncthreads();
+  const auto put = [&](int buffer) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) sa[tx][ty + 16 * i] = la[i], sb[tx][ty + 16 * i] = lb[i];
-    __syncthreads();
+    for (int i = 0; i < 8; i++) sa[buffer][tx][ty + 16 * i] = la[i], sb[buffer][tx][ty + 16 * i] = lb[i];
+  };
+  load(0);
+  put(0);
+  __syncthreads();
+  int buffer = 0;
+  for (int64_t k0 = 0; k0 < K; k0 += kInner, buffer ^= 1) {
     load(k0 + kInner);
 #pragma unroll
     for (int k = 0; k < kInner; k++) {
-      float a[8], b[8];
+      float a[8];
+      ulonglong2 b[2];
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        *reinterpret_cast<float4*>(a + i) = *reinterpret_cast<const float4*>(&sa[k][ty * 4 + i * 16]);
-        *reinterpret_cast<float4*>(b + i) = *reinterpret_cast<const float4*>(&sb[k][tx * 4 + i * 16]);
+      for (int i = 0; i < 2; i++) {
+        *reinterpret_cast<float4*>(a + 4 * i) = *reinterpret_cast<const float4*>(&sa[buffer][k][ty * 4 + i * 64]);
+        b[i] = *reinterpret_cast<const ulonglong2*>(&sb[buffer][k][tx * 4 + i * 64]);
       }
 #pragma unroll
-      for (int i = 0; i < 8; i++)
+      for (int i = 0; i < 8; i++) {
+        uint64_t both;
+        asm("mov.b64 %0, {%1, %1};" : "=l"(both) : "f"(a[i]));
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < 4; j++) {
+          const uint64_t pair = j % 2 ? b[j / 2].y : b[j / 2].x;
+          asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(both), "l"(pair));
+        }
+      }
     }
+    put(buffer ^ 1);
+    __syncthreads();
   }
 #pragma unroll
   for (int i = 0; i < 8; i++)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int64_t m = m0 + ty * 4 + i % 4 + i / 4 * 64, n = n0 + tx * 4 + j % 4 + j / 4 * 64;
-      if (m < M && n < N && LNCC_IN(m * ld + n, 1, M * ld)) out[m * ld + n] = acc[i][j];
+    for (int j = 0; j < 4; j++) {
+      float v[2];
+      asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(acc[i][j]));
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int64_t m = m0 + ty * 4 + i % 4 + i / 4 * 64, n = n0 + tx * 4 + j % 2 * 2 + e + j / 2 * 64;
+        if (m < M && n < N && LNCC_IN(m * ld + n, 1, M * ld)) out[m * ld + n] = v[e];
+      }
     }
 }
 
@@ -806,7 +851,7 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
     const int width = gated(kind) ? bn / 2 : bn;
     const int64_t m_tiles = ceil_div(rows, 256), n_tiles = ceil_div(cols, width), tiles = m_tiles * n_tiles * whichs;
     for (int want = 1; want <= 64; want++) {
-      if (want > 1 && (gated(kind) || kind == DH || blocks < 4 * want)) break;
+      if (want > 1 && (gated(kind) || kind == DH || kind == ONE_GATE || blocks < 4 * want)) break;
       const int64_t per = ceil_div(blocks, want), splits = ceil_div(blocks, per);
       if (splits != want) continue;
       double t = double(ceil_div(tiles * splits, pairs)) * (double(per) * parts * (bn == 256 ? 590 : 515) + 1500);
@@ -880,9 +925,23 @@ struct Call {
   char* scratch;
   cudaStream_t stream;
   int status;
-  bool first;  // the next product kernel is the call's first
+  bool first = true;      // the next product kernel is the call's first
+  bool launched = false;  // a kernel of this call is in the stream
+  Packs packs = {};
 
-  // src as TMA reads it: in place, or packed to `to`
+  // every kernel of a call but its first may be launched while the one before it ends (begin_after_previous)
+  template <typename K, typename... A> void run(K kernel, dim3 grid, int threads, int smem, const A&... args) {
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid, cfg.blockDim = dim3(unsigned(threads)), cfg.dynamicSmemBytes = size_t(smem), cfg.stream = stream;
+    cfg.attrs = &early, cfg.numAttrs = launched ? 1 : 0;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) != cudaSuccess) status = LNCC_ERR_LAUNCH;
+    launched = true;
+  }
+
+  // src as TMA reads it: in place, or packed to `to` by pack()
   Matrix operand(const void* src, int64_t rows, int64_t cols, int64_t stride, size_t to) {
     Matrix m = {const_cast<void*>(src), rows, cols, stride, 0, 1, a.dtype != LNCC_F16};
     if (a.dtype != LNCC_F32 && aligned(src, 16) && (stride % 8 == 0 || rows == 1)) {
@@ -894,17 +953,16 @@ struct Call {
     m.plane = rows * m.ld;
     m.planes = plan.planes;
     const int64_t blocks = ceil_div(rows * (m.ld / 8), 256), most = int64_t(sm_count()) * 8;
-    const unsigned grid = unsigned(blocks < most ? blocks : most);
-    if (a.dtype == LNCC_F32)
-      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(src), stride, rows, cols,
-                                            static_cast<__nv_bfloat16*>(m.p), m.ld, m.plane);
-    else if (a.dtype == LNCC_BF16)
-      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(src), stride, rows, cols,
-                                            static_cast<__nv_bfloat16*>(m.p), m.ld, m.plane);
-    else
-      pack_kernel<<<grid, 256, 0, stream>>>(static_cast<const __half*>(src), stride, rows, cols, static_cast<__half*>(m.p),
-                                            m.ld, m.plane);
+    packs.job[packs.jobs++] = {src, m.p, stride, rows, cols, m.ld, m.plane, packs.blocks};
+    packs.blocks += int(blocks < most ? blocks : most);
     return m;
+  }
+  void pack() {
+    if (packs.jobs == 0) return;
+    const dim3 grid = dim3(unsigned(packs.blocks));
+    if (a.dtype == LNCC_F32) run(pack_kernel<float, __nv_bfloat16>, grid, 256, 0, packs);
+    else if (a.dtype == LNCC_BF16) run(pack_kernel<__nv_bfloat16, __nv_bfloat16>, grid, 256, 0, packs);
+    else run(pack_kernel<__half, __half>, grid, 256, 0, packs);
   }
   Matrix hidden(size_t at) const {
     return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.planes, a.dtype != LNCC_F16};
@@ -919,7 +977,7 @@ struct Call {
       return;
     }
     const int64_t tiles = int64_t(g.m_tiles) * g.n_tiles * g.whichs * g.splits;
-    product_kernel<KIND, BN, ACT, T><<<unsigned(2 * (tiles < pairs ? tiles : pairs)), kThreads, smem, stream>>>(g);
+    run(product_kernel<KIND, BN, ACT, T>, dim3(unsigned(2 * (tiles < pairs ? tiles : pairs))), kThreads, smem, g);
   }
   template <int KIND, int BN, typename T> void launch_act(Gemm& g) {
     if constexpr (KIND == UP || KIND == HIDDEN) {
@@ -940,9 +998,11 @@ struct Call {
     const int64_t quads = g.whichs * g.rows * ceil_div(g.cols, 4);
     T *out0 = static_cast<T*>(g.out0), *out1 = static_cast<T*>(g.out1);
     if (g.splits < kManySplits)
-      join_kernel<T, 1><<<unsigned(ceil_div(quads, 256)), 256, 0, stream>>>(g.partial, g.splits, g.whichs, g.rows, g.cols, out0, out1);
+      run(join_kernel<T, 1>, dim3(unsigned(ceil_div(quads, 256))), 256, 0, static_cast<const float*>(g.partial), g.splits,
+          g.whichs, g.rows, g.cols, out0, out1);
     else
-      join_kernel<T, 8><<<unsigned(ceil_div(quads, 32)), 256, 0, stream>>>(g.partial, g.splits, g.whichs, g.rows, g.cols, out0, out1);
+      run(join_kernel<T, 8>, dim3(unsigned(ceil_div(quads, 32))), 256, 0, static_cast<const float*>(g.partial), g.splits,
+          g.whichs, g.rows, g.cols, out0, out1);
   }
 
   // One product: A (a0, a1) and B (b0, b1, b2) as the kind takes them, results out (rows x cols, ld apart).
@@ -973,7 +1033,7 @@ struct Call {
     g.abort_word = reinterpret_cast<unsigned*>(scratch);
     g.clear_abort = first;
     first = false;
-    if constexpr (KIND == GATES || KIND == DH) {
+    if constexpr (KIND == GATES || KIND == DH || KIND == ONE_GATE) {
       launch_type<KIND, float>(g, c.bn);
     } else if (a.dtype == LNCC_F32) {
       if constexpr (KIND != HIDDEN) launch_type<KIND, float>(g, c.bn);
@@ -987,7 +1047,6 @@ struct Call {
       else if (a.dtype == LNCC_BF16) join<__nv_bfloat16>(g);
       else join<__half>(g);
     }
-    if (cudaPeekAtLastError() != cudaSuccess) status = LNCC_ERR_LAUNCH;
   }
 };
 
@@ -1042,34 +1101,40 @@ static int forward(const Args& a, void* scratch, cudaStream_t stream) {
     if (a.dtype == LNCC_BF16) return few_forward<__nv_bfloat16>(a, scratch, stream);
     return few_forward<__half>(a, scratch, stream);
   }
-  Call c = {a, plan_for(a, false), static_cast<char*>(scratch), stream, LNCC_OK, true};
+  Call c = {a, plan_for(a, false), static_cast<char*>(scratch), stream, LNCC_OK};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg),
                wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu), wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd),
                h = c.hidden(c.plan.h);
+  c.pack();
   c.product<UP>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, h.p, nullptr, nullptr, h.ld, h.plane);
   c.product<DOWN>(h, h, wd, wd, wd, a.M, a.N, 1, a.F, 0, a.y, nullptr, nullptr, a.N, 0);
   return c.status;
 }
 
 static int backward(const Args& a, void* scratch, cudaStream_t stream) {
-  Call c = {a, plan_for(a, true), static_cast<char*>(scratch), stream, LNCC_OK, true};
+  Call c = {a, plan_for(a, true), static_cast<char*>(scratch), stream, LNCC_OK};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), dy = c.operand(a.dy, a.M, a.N, a.dy_stride, c.plan.dy),
                wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg), wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu),
                wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd);
   const Matrix h = c.hidden(c.plan.h), dg = c.hidden(c.plan.dg), du = c.hidden(c.plan.du);
+  c.pack();
   if (a.dtype == LNCC_F32) {
-    float* const gate = reinterpret_cast<float*>(c.scratch + c.plan.gate);
-    c.product<GATES>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, gate, c.scratch + c.plan.up, nullptr, h.ld, 0);
-    if (a.act == LNCC_ACT_RELU)
-      gate_kernel<<<dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, stream>>>(
-          static_cast<const float*>(a.x), a.x_stride, static_cast<const float*>(a.wg), gate, h.ld, a.M, a.F, a.K);
-    float *const up = reinterpret_cast<float*>(c.scratch + c.plan.up), *const dhp = reinterpret_cast<float*>(c.scratch + c.plan.dh);
-    c.product<DH>(dy, dy, wd, wd, wd, a.M, a.F, 1, a.N, 0, dhp, nullptr, nullptr, h.ld, 0);
+    float *const gate = reinterpret_cast<float*>(c.scratch + c.plan.gate), *const up = reinterpret_cast<float*>(c.scratch + c.plan.up),
+                *const dh = reinterpret_cast<float*>(c.scratch + c.plan.dh);
+    if (a.act == LNCC_ACT_RELU) {
+      c.run(gate_kernel, dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, static_cast<const float*>(a.x),
+            a.x_stride, static_cast<const float*>(a.wg), gate, h.ld, a.M, a.F, a.K);
+      c.product<ONE_GATE>(x, x, wu, wu, wu, a.M, a.F, 1, a.K, 0, up, nullptr, nullptr, h.ld, 0);
+    } else {
+      c.product<GATES>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, gate, up, nullptr, h.ld, 0);
+    }
+    c.product<DH>(dy, dy, wd, wd, wd, a.M, a.F, 1, a.N, 0, dh, nullptr, nullptr, h.ld, 0);
     const auto parts = a.act == LNCC_ACT_SILU ? parts_kernel<LNCC_ACT_SILU>
                        : a.act == LNCC_ACT_GELU ? parts_kernel<LNCC_ACT_GELU> : parts_kernel<LNCC_ACT_RELU>;
     const int64_t n = a.M * h.ld, blocks = ceil_div(n, 2048), most = int64_t(sm_count()) * 8;
-    parts<<<unsigned(blocks < most ? blocks : most), 256, 0, stream>>>(
-        gate, up, dhp, static_cast<__nv_bfloat16*>(dg.p), static_cast<__nv_bfloat16*>(du.p), static_cast<__nv_bfloat16*>(h.p), n, h.plane);
+    c.run(parts, dim3(unsigned(blocks < most ? blocks : most)), 256, 0, static_cast<const float*>(gate), static_cast<const float*>(up),
+          static_cast<const float*>(dh), static_cast<__nv_bfloat16*>(dg.p), static_cast<__nv_bfloat16*>(du.p),
+          static_cast<__nv_bfloat16*>(h.p), n, h.plane);
   } else {
     c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
   }
