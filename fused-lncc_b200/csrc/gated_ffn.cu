@@ -6,7 +6,7 @@
 //
 // Every product runs on the tensor cores, in one kernel whose epilogue does what follows it: UP forms g and u side by side
 // in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h (for fp32 GATES
-// writes g and u, or ONE_GATE u alone, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is split over
+// writes g and u, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is split over
 // the GPU, fp32 partial sums that a last kernel adds in order.
 //
 // A pair of CTAs takes a tile of 256 rows by up to 256 columns (cta_group::2): each loads its 128 rows of A and half the
@@ -37,7 +37,7 @@ using namespace tc;
 
 constexpr uint32_t kNaN = 0x7fffffff;  // what a tile gets whose products were given up
 
-enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN, ONE_GATE };
+enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
 
 constexpr int kEpilogueWarps = 16;         // of a CTA: four for each quarter of the lanes of tensor memory
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0 TMA, 1 products, 4 - 19 epilogue
@@ -578,20 +578,82 @@ template <typename T, typename TO> __global__ void __launch_bounds__(256) pack_k
   }
 }
 
+// Euclidean norms of the rows of x and then of Wg, a warp a row.
+__global__ void __launch_bounds__(256) norms_kernel(const float* __restrict__ x, int64_t x_stride, const float* __restrict__ w,
+                                                    float* norms, int64_t M, int64_t F, int64_t K) {
+  begin_after_previous();
+  const int64_t row = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
+  if (row >= M + F) return;
+  const float* p = row < M ? x + row * x_stride : w + (row - M) * K;
+  float s = 0.f;
+  for (int64_t k = threadIdx.x % 32; k < K; k += 32) s = fmaf(p[k], p[k], s);
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (threadIdx.x % 32 == 0 && LNCC_IN(row, 1, M + F)) norms[row] = sqrtf(s);
+}
+struct NearZero {  // what a gate of ReLU is formed again from
+  const float *x, *w, *norms;
+  int64_t x_stride, M, F, K, ld;
+};
+// A gate of ReLU by fp32 multiply-adds in the order of k, by a whole warp: it loads 128 of k side by side, and every lane
+// adds them up.
+__device__ __noinline__ float gate_in_order(const NearZero& z, int64_t row, int64_t col, float2* stage) {
+  const float *x = z.x + row * z.x_stride, *w = z.w + col * z.K;
+  const int lane = threadIdx.x % 32;
+  float s = 0.f;
+  for (int64_t k0 = 0; k0 < z.K; k0 += 128) {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int64_t k = k0 + i * 32 + lane;
+      stage[i * 32 + lane] = k < z.K ? make_float2(x[k], w[k]) : make_float2(0.f, 0.f);  // adding 0 * 0 changes nothing
+    }
+    __syncwarp();
+#pragma unroll 16
+    for (int i = 0; i < 128; i++) s = fmaf(stage[i].x, stage[i].y, s);
+  }
+  return s;
+}
+
 // fp32: dg, du and h, taken apart, from g, u and dh (rows ld apart, like the results). Eight neighbours a thread.
+// ReLU's derivative jumps at g = 0, where the last bits of g decide and one element that falls the other way is off by all of
+// its gradient. The sum of the tensor cores and the plain fp32 sum in the order of k are each within (K + 64) 2^-24 |x| |w|
+// of the exact one; where g is closer to 0 than both together, it is formed again as the plain sum (about one gate in
+// 2500 at K = 389; forming all of them so took 100 us of 413 at 4093 x 389 x 1037).
 template <int ACT>
 __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g, const float* __restrict__ u,
                                                     const float* __restrict__ dh, __nv_bfloat16* dg, __nv_bfloat16* du,
-                                                    __nv_bfloat16* h, int64_t n, int64_t plane) {
+                                                    __nv_bfloat16* h, int64_t n, int64_t plane, const NearZero z) {
   begin_after_previous();
-  for (int64_t i = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8; i < n; i += int64_t(gridDim.x) * 256 * 8) {
+  __shared__ float2 stages[ACT == LNCC_ACT_RELU ? 8 : 1][128];
+  const int lane = threadIdx.x % 32;
+  // a warp's lanes take the same number of turns
+  for (int64_t i0 = (int64_t(blockIdx.x) * 256 + threadIdx.x - lane) * 8; i0 < n; i0 += int64_t(gridDim.x) * 256 * 8) {
+    const int64_t i = i0 + lane * 8;
+    const bool here = i < n;
     float vg[8], vu[8], vd[8], o[3][8];
+    if (here) {
 #pragma unroll
-    for (int k = 0; k < 8; k += 4) {
-      load_vec<float, 4>(g + i + k, reinterpret_cast<float(&)[4]>(vg[k]));
-      load_vec<float, 4>(u + i + k, reinterpret_cast<float(&)[4]>(vu[k]));
-      load_vec<float, 4>(dh + i + k, reinterpret_cast<float(&)[4]>(vd[k]));
+      for (int k = 0; k < 8; k += 4) {
+        load_vec<float, 4>(g + i + k, reinterpret_cast<float(&)[4]>(vg[k]));
+        load_vec<float, 4>(u + i + k, reinterpret_cast<float(&)[4]>(vu[k]));
+        load_vec<float, 4>(dh + i + k, reinterpret_cast<float(&)[4]>(vd[k]));
+      }
     }
+    if (ACT == LNCC_ACT_RELU) {
+      const int64_t row = i / z.ld, col = i - row * z.ld;
+      const float near = here ? z.norms[row] * (float(z.K + 64) * 1.1920929e-7f) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        const bool again = here && col + k < z.F && !(fabsf(vg[k]) > near * z.norms[z.M + col + k]);
+        for (unsigned rest = __ballot_sync(0xffffffffu, again); rest; rest &= rest - 1) {
+          const int who = __ffs(rest) - 1;
+          const float v = gate_in_order(z, __shfl_sync(0xffffffffu, row, who), __shfl_sync(0xffffffffu, col, who) + k, stages[threadIdx.x / 32]);
+          if (lane == who) vg[k] = v;
+        }
+      }
+    }
+    if (!here) continue;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
       float a, da;
@@ -611,74 +673,6 @@ __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g,
         if (LNCC_IN(i, 8, n)) *reinterpret_cast<Vec<__nv_bfloat16, 8>*>(to + k * plane) = part[k];
     }
   }
-}
-
-// g = x Wg^T by fp32 multiply-adds in the order of k, for the backward pass of ReLU in fp32 alone: the derivative jumps at
-// g = 0, where the last bit of g decides, so g is the plain fp32 sum there. A block takes 128 x 128, a thread 8 x 8 of it,
-// two columns a packed multiply-add, 16 of k at a time through two buffers of shared memory.
-constexpr int kTile = 128, kInner = 16;
-__global__ void __launch_bounds__(256, 2) gate_kernel(const float* __restrict__ x, int64_t x_stride,
-                                                      const float* __restrict__ w, float* out, int64_t ld, int64_t M, int64_t N,
-                                                      int64_t K) {
-  begin_after_previous();
-  __shared__ __align__(16) float sa[2][kInner][kTile + 4], sb[2][kInner][kTile + 4];
-  const int64_t m0 = int64_t(blockIdx.x) * kTile, n0 = int64_t(blockIdx.y) * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;  // also: column of k, and first row, of the thread's loads
-  uint64_t acc[8][4] = {};  // pairs of columns
-  float la[8], lb[8];
-  const auto load = [&](int64_t k) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int64_t r = ty + 16 * i;
-      la[i] = m0 + r < M && k + tx < K ? x[(m0 + r) * x_stride + k + tx] : 0.f;
-      lb[i] = n0 + r < N && k + tx < K ? w[(n0 + r) * K + k + tx] : 0.f;
-    }
-  };
-  const auto put = [&](int buffer) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) sa[buffer][tx][ty + 16 * i] = la[i], sb[buffer][tx][ty + 16 * i] = lb[i];
-  };
-  load(0);
-  put(0);
-  __syncthreads();
-  int buffer = 0;
-  for (int64_t k0 = 0; k0 < K; k0 += kInner, buffer ^= 1) {
-    load(k0 + kInner);
-#pragma unroll
-    for (int k = 0; k < kInner; k++) {
-      float a[8];
-      ulonglong2 b[2];
-#pragma unroll
-      for (int i = 0; i < 2; i++) {
-        *reinterpret_cast<float4*>(a + 4 * i) = *reinterpret_cast<const float4*>(&sa[buffer][k][ty * 4 + i * 64]);
-        b[i] = *reinterpret_cast<const ulonglong2*>(&sb[buffer][k][tx * 4 + i * 64]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        uint64_t both;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(both) : "f"(a[i]));
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const uint64_t pair = j % 2 ? b[j / 2].y : b[j / 2].x;
-          asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[i][j]) : "l"(both), "l"(pair));
-        }
-      }
-    }
-    put(buffer ^ 1);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 8; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      float v[2];
-      asm("mov.b64 {%0, %1}, %2;" : "=f"(v[0]), "=f"(v[1]) : "l"(acc[i][j]));
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const int64_t m = m0 + ty * 4 + i % 4 + i / 4 * 64, n = n0 + tx * 4 + j % 2 * 2 + e + j / 2 * 64;
-        if (m < M && n < N && LNCC_IN(m * ld + n, 1, M * ld)) out[m * ld + n] = v[e];
-      }
-    }
 }
 
 // ---- a few tokens ----------------------------------------------------------------------------------------------------
@@ -851,7 +845,7 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
     const int width = gated(kind) ? bn / 2 : bn;
     const int64_t m_tiles = ceil_div(rows, 256), n_tiles = ceil_div(cols, width), tiles = m_tiles * n_tiles * whichs;
     for (int want = 1; want <= 64; want++) {
-      if (want > 1 && (gated(kind) || kind == DH || kind == ONE_GATE || blocks < 4 * want)) break;
+      if (want > 1 && (gated(kind) || kind == DH || blocks < 4 * want)) break;
       const int64_t per = ceil_div(blocks, want), splits = ceil_div(blocks, per);
       if (splits != want) continue;
       double t = double(ceil_div(tiles * splits, pairs)) * (double(per) * parts * (bn == 256 ? 590 : 515) + 1500);
@@ -868,7 +862,7 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
 // Scratch of a call, laid out in one place for its size and its use.
 struct Plan {
   int planes;
-  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, dh, partial, total;
+  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, dh, norms, partial, total;
   int64_t ldf;
 };
 static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
@@ -906,6 +900,7 @@ static Plan plan_for(const Args& a, bool backward) {
       p.gate = at, at += round_up(size_t(a.M) * p.ldf * 4);
       p.up = at, at += round_up(size_t(a.M) * p.ldf * 4);
       p.dh = at, at += round_up(size_t(a.M) * p.ldf * 4);
+      p.norms = at, at += round_up(size_t(a.M + a.F) * 4);
     }
     partial(partial_bytes(DX, a.dtype, a.M, a.K, 1, 2 * k_steps(a.F)));
     partial(partial_bytes(DW_UP, a.dtype, a.F, a.K, 2, k_steps(a.M)));
@@ -1033,7 +1028,7 @@ struct Call {
     g.abort_word = reinterpret_cast<unsigned*>(scratch);
     g.clear_abort = first;
     first = false;
-    if constexpr (KIND == GATES || KIND == DH || KIND == ONE_GATE) {
+    if constexpr (KIND == GATES || KIND == DH) {
       launch_type<KIND, float>(g, c.bn);
     } else if (a.dtype == LNCC_F32) {
       if constexpr (KIND != HIDDEN) launch_type<KIND, float>(g, c.bn);
@@ -1121,20 +1116,18 @@ static int backward(const Args& a, void* scratch, cudaStream_t stream) {
   if (a.dtype == LNCC_F32) {
     float *const gate = reinterpret_cast<float*>(c.scratch + c.plan.gate), *const up = reinterpret_cast<float*>(c.scratch + c.plan.up),
                 *const dh = reinterpret_cast<float*>(c.scratch + c.plan.dh);
-    if (a.act == LNCC_ACT_RELU) {
-      c.run(gate_kernel, dim3(unsigned(ceil_div(a.M, kTile)), unsigned(ceil_div(a.F, kTile))), 256, 0, static_cast<const float*>(a.x),
-            a.x_stride, static_cast<const float*>(a.wg), gate, h.ld, a.M, a.F, a.K);
-      c.product<ONE_GATE>(x, x, wu, wu, wu, a.M, a.F, 1, a.K, 0, up, nullptr, nullptr, h.ld, 0);
-    } else {
-      c.product<GATES>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, gate, up, nullptr, h.ld, 0);
-    }
+    const NearZero z = {static_cast<const float*>(a.x), static_cast<const float*>(a.wg),
+                        reinterpret_cast<const float*>(c.scratch + c.plan.norms), a.x_stride, a.M, a.F, a.K, h.ld};
+    if (a.act == LNCC_ACT_RELU)
+      c.run(norms_kernel, dim3(unsigned(ceil_div(a.M + a.F, 8))), 256, 0, z.x, a.x_stride, z.w, const_cast<float*>(z.norms), a.M, a.F, a.K);
+    c.product<GATES>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, gate, up, nullptr, h.ld, 0);
     c.product<DH>(dy, dy, wd, wd, wd, a.M, a.F, 1, a.N, 0, dh, nullptr, nullptr, h.ld, 0);
     const auto parts = a.act == LNCC_ACT_SILU ? parts_kernel<LNCC_ACT_SILU>
                        : a.act == LNCC_ACT_GELU ? parts_kernel<LNCC_ACT_GELU> : parts_kernel<LNCC_ACT_RELU>;
     const int64_t n = a.M * h.ld, blocks = ceil_div(n, 2048), most = int64_t(sm_count()) * 8;
     c.run(parts, dim3(unsigned(blocks < most ? blocks : most)), 256, 0, static_cast<const float*>(gate), static_cast<const float*>(up),
           static_cast<const float*>(dh), static_cast<__nv_bfloat16*>(dg.p), static_cast<__nv_bfloat16*>(du.p),
-          static_cast<__nv_bfloat16*>(h.p), n, h.plane);
+          static_cast<__nv_bfloat16*>(h.p), n, h.plane, z);
   } else {
     c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
   }
