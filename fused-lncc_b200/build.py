@@ -18,6 +18,7 @@ import os
 import re
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG_ROOT = os.path.dirname(os.path.abspath(__file__))
@@ -111,13 +112,14 @@ def build_torch_ops(force=False, verbose=False):
     torch_dir = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(nvcc_path())) or "/usr/local/cuda"
     includes = [INCLUDE, os.path.join(torch_dir, "include"),
-                os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include")]
+                os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), os.path.join(cuda, "include"),
+                sysconfig.get_paths()["include"]]
     # not $CXX: a compiler that links its own libstdc++ statically gives the library a second one beside torch's, and the
     # first number printed into an error message crashes
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in includes),
            "-o", out + ".tmp", src, f"-L{LIB_DIR}", f"-l:{os.path.basename(lib)}", f"-L{os.path.join(torch_dir, 'lib')}",
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     _run(cmd, out, verbose)
     os.replace(out + ".tmp", out)
     return out

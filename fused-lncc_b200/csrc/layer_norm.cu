@@ -381,7 +381,11 @@ template <typename T, int VEC, int LANES> static void launch_lanes(const Args& a
   constexpr int threads = threads_of<LANES>();
   const int ring = Rows<T, LANES, VEC, threads>::smem(), smem = backward ? 2 * ring : ring;
   const auto kernel = backward ? backward_kernel<T, LANES, VEC> : forward_kernel<T, LANES, VEC>;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static uint64_t asked[2];  // devices that were asked for this kernel's shared memory; asking twice does no harm
+  int dev = 0;
+  if (smem > 40 * 1024 && cudaGetDevice(&dev) == cudaSuccess && dev < 64 && !(asked[backward] >> dev & 1)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) asked[backward] |= 1ull << dev;
+  }
   kernel<<<grid, threads, smem, st>>>(a);
 }
 template <typename T, int VEC> static void launch(const Args& a, bool backward, cudaStream_t st) {

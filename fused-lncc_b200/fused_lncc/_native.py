@@ -1,5 +1,6 @@
 """Loads libfused_lncc_torch.so, which gives torch the token-block operators (csrc/torch_ops.cpp), and tells torch.compile
 their shapes. Like the C library it is built in-tree once where it is missing, and there is no fallback."""
+import importlib.machinery
 import importlib.util
 import os
 import threading
@@ -12,7 +13,7 @@ OPS_PATH = os.path.join(os.path.dirname(_lib.LIB_PATH), "libfused_lncc_torch.so"
 KEEP = 16  # steps of the gated scan from one kept state to the next (lncc_gated_scan_kept_bytes)
 
 _lock = threading.Lock()
-_loaded = False
+_module = None
 
 
 def _build():
@@ -28,18 +29,21 @@ def kept_numel(B, T, C):
 
 
 def load():
-    """torch.ops.fused_lncc with the token-block operators in it."""
-    global _loaded
-    if not _loaded:
+    """The library as a module: layer_norm, gated_scan and gated_ffn for eager calls. torch.ops.fused_lncc has the operators
+    once it is loaded."""
+    global _module
+    if _module is None:
         with _lock:
-            if not _loaded:
+            if _module is None:
                 if not os.path.exists(OPS_PATH):
                     _build()
                 _lib.load()
-                torch.ops.load_library(OPS_PATH)
+                loader = importlib.machinery.ExtensionFileLoader("libfused_lncc_torch", OPS_PATH)
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+                loader.exec_module(module)
                 _register_fakes()
-                _loaded = True
-    return torch.ops.fused_lncc
+                _module = module
+    return _module
 
 
 def _register_fakes():

@@ -7,6 +7,8 @@
 x: (..., K); w_gate, w_up: (F, K); w_down: (N, F), as torch.nn.Linear lays its weights out; all of one type, float32,
 bfloat16 or float16. Sums are fp32. Nothing of the hidden layer is saved for the backward pass: it forms g, u and h again.
 """
+import torch
+
 from . import _native
 
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
@@ -21,4 +23,7 @@ def fused_gated_ffn(x, w_gate, w_up, w_down, activation="silu"):
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"fused_lncc: gated_ffn: activation must be 'silu', 'gelu' or 'relu', got {activation!r}")
-    return _native.load().fused_gated_ffn(x, w_gate, w_up, w_down, act)
+    module = _native.load()
+    if torch.compiler.is_compiling():
+        return torch.ops.fused_lncc.fused_gated_ffn(x, w_gate, w_up, w_down, act)
+    return module.gated_ffn(x, w_gate, w_up, w_down, act)

@@ -9,6 +9,8 @@ pieces, down to single tokens, by handing each call the state that the one befor
 throughout; h is rounded to x's type as it is written, and no rounded value is carried on. The backward pass forms h
 again from fp32 states that the forward pass kept, so nothing of h is saved.
 """
+import torch
+
 from . import _native
 
 
@@ -20,4 +22,7 @@ def fused_gated_scan(x, gate, state=None, reverse=False):
     the last step taken. Gradients flow to x, gate and state from both results.
     A gate of +inf keeps the state and ignores x_t, one of -inf forgets the state (x_t and the state have to be finite
     all the same: the formula multiplies them by zero). RuntimeError for wrong shapes, types or devices."""
-    return _native.load().fused_gated_scan(x, gate, state, reverse)
+    module = _native.load()
+    if torch.compiler.is_compiling():
+        return torch.ops.fused_lncc.fused_gated_scan(x, gate, state, reverse)
+    return module.gated_scan(x, gate, state, reverse)
