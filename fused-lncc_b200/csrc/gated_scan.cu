@@ -42,19 +42,20 @@ struct Args {
 
 // V channels' products and sums; two channels as one packed instruction.
 template <int V> __device__ __forceinline__ void mul(const float (&a)[V], const float (&b)[V], float (&d)[V]) {
-  if constexpr (V == 2)
-    asm("{\n\t.reg .b64 A, B;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmul.rn.f32x2 A, A, B;\n\tmov.b64 {%0, %1}, A;\n\t}"
-        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
-  else
+  if constexpr (V == 2) {
+    const float2 r = mul2(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+    d[0] = r.x, d[1] = r.y;
+  } else {
     for (int v = 0; v < V; v++) d[v] = a[v] * b[v];
+  }
 }
 template <int V> __device__ __forceinline__ void fma(const float (&a)[V], const float (&b)[V], const float (&c)[V], float (&d)[V]) {
-  if constexpr (V == 2)
-    asm("{\n\t.reg .b64 A, B, C;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmov.b64 C, {%6, %7};\n\tfma.rn.f32x2 A, A, B, C;\n\t"
-        "mov.b64 {%0, %1}, A;\n\t}"
-        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
-  else
+  if constexpr (V == 2) {
+    const float2 r = fma2(make_float2(a[0], a[1]), make_float2(b[0], b[1]), make_float2(c[0], c[1]));
+    d[0] = r.x, d[1] = r.y;
+  } else {
     for (int v = 0; v < V; v++) d[v] = fmaf(a[v], b[v], c[v]);
+  }
 }
 
 // a = sigmoid(g) and keep = 1 - a = sigmoid(-g), each to a few u32 of itself (1 - a would cancel for open gates).

@@ -3,10 +3,11 @@
 //   mu = mean(x), v = mean((x - mu)^2), r = 1/sqrt(v + eps), n = (x - mu) r, y = n w + b
 //   g = dy w, dx = r (g - mean(g) - n mean(g n)), dw = sum over rows of dy n, db = sum over rows of dy
 //
-// A row lives in the registers of LANES threads, 16 elements each, from its one load to its one store: the mean and
+// A row lives in the registers of LANES threads, E = 12 or 16 elements each, from its one load to its one store: the mean and
 // then the centred squares are summed in fp32 without a second read (the two-step variance does not cancel). LANES is
-// the smallest power of two whose registers hold the row, so a warp takes 8 rows of 64 or one of 512, and a block one of
-// up to 8192. Both directions are bound by their bytes; thread blocks stay and walk over the rows, so that the weight
+// a power of two and E the smaller one that holds the row, so a warp takes 8 rows of 64 or one of 384 or 512, and a block one
+// of up to 8192. Arithmetic is packed, two elements an instruction: at 107520 x 384 the kernels were bound by issuing 257
+// instructions a row forward and 391 backward. Both directions are bound by their bytes; thread blocks stay and walk over the rows, so that the weight
 // is loaded once and, backward, each thread keeps the fp32 sums of dw and db of its own columns. The next three rows are
 // under way meanwhile, copied asynchronously into shared memory that only the thread itself reads (so no barrier waits for
 // them): with one row ahead in registers 24 KB an SM were in flight, and the forward pass took 60 us where its bytes
@@ -22,7 +23,7 @@ namespace norm {
 
 using namespace blk;
 
-constexpr int kElems = 16;       // elements of a row that one thread holds
+constexpr int kElems = 16;       // the most elements of a row that one thread holds
 constexpr int kThreads = 256;    // threads of a block (LANES where that is more)
 constexpr int kMaxWidth = 8192;  // widest row that 512 threads hold
 
@@ -68,10 +69,10 @@ template <int LANES> __device__ __forceinline__ float row_sum(float v, float* re
 }
 
 // One thread's shares of the rows to come: NV vectors of VEC elements each, vector v at column (v*LANES + lane)*VEC. A ring
-// of rows in shared memory, filled by asynchronous copies of 4 or 16 bytes; single 16-bit elements, which have
+// of rows in shared memory, filled by asynchronous copies of 4 to 16 bytes; single 16-bit elements, which have
 // none, wait in registers instead, one row ahead.
-template <typename T, int LANES, int VEC, int THREADS> struct Rows {
-  static constexpr int NV = kElems / VEC, BYTES = VEC * int(sizeof(T));
+template <typename T, int LANES, int VEC, int E, int THREADS> struct Rows {
+  static constexpr int NV = E / VEC, BYTES = VEC * int(sizeof(T));
   static constexpr int kStages = sizeof(T) == 4 ? 3 : 4;  // at most 48 KB a ring for 256 threads
   static constexpr bool ASYNC = BYTES >= 4;
   typedef Vec<T, VEC> V;
@@ -98,7 +99,9 @@ template <typename T, int LANES, int VEC, int THREADS> struct Rows {
         const uint32_t dst = uint32_t(__cvta_generic_to_shared(ring + (in * NV + v) * THREADS));
         const T* src = live ? from + c : base;
         const int bytes = live ? BYTES : 0;  // what is not copied is zero
-        if constexpr (BYTES == 16)
+        if constexpr (BYTES == 8)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+        else if constexpr (BYTES == 16)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
         else
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -109,8 +112,9 @@ template <typename T, int LANES, int VEC, int THREADS> struct Rows {
     }
     in = in + 1 == kStages ? 0 : in + 1;
   }
-  // the oldest row fetched, as floats
-  __device__ __forceinline__ void take(float (&f)[kElems]) {
+  // the oldest row fetched, as pairs of floats
+  __device__ __forceinline__ void take(float2 (&pairs)[E / 2]) {
+    float f[E];
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       V r;
@@ -119,6 +123,8 @@ template <typename T, int LANES, int VEC, int THREADS> struct Rows {
 #pragma unroll
       for (int i = 0; i < VEC; i++) f[v * VEC + i] = to_f(r.e[i]);
     }
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) pairs[i] = make_float2(f[2 * i], f[2 * i + 1]);
     out = out + 1 == kStages ? 0 : out + 1;
   }
 };
@@ -127,11 +133,15 @@ template <int LATER> __device__ __forceinline__ void wait_fetch() { asm volatile
 
 template <int LANES> __host__ __device__ constexpr int threads_of() { return LANES > kThreads ? LANES : kThreads; }
 
-template <typename T, int LANES, int VEC>
+// column of element e of a lane
+template <int LANES, int VEC> __device__ __forceinline__ int column(int e, int lane) { return (e / VEC * LANES + lane) * VEC + e % VEC; }
+__device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
+
+template <typename T, int LANES, int VEC, int E>
 __global__ void __launch_bounds__(threads_of<LANES>(), LANES > kThreads ? 1 : VEC * sizeof(T) >= 4 ? 3 : 2) forward_kernel(const Args a) {
   constexpr int THREADS = LANES > kThreads ? LANES : kThreads;
-  constexpr int ROWS = THREADS / LANES, NV = kElems / VEC;
-  typedef Rows<T, LANES, VEC, THREADS> R;
+  constexpr int ROWS = THREADS / LANES, NV = E / VEC;
+  typedef Rows<T, LANES, VEC, E, THREADS> R;
   constexpr int AHEAD = R::ASYNC ? R::kStages - 1 : 1;
   extern __shared__ __align__(16) unsigned char stage[];
   __shared__ float red[2][THREADS / 32];
@@ -145,54 +155,62 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES > kThreads ? 1 : VE
     rows.fetch(row + i * step);
     close_fetch();
   }
-  float w[kElems], b[kElems];
+  float2 w[E / 2], b[E / 2];
 #pragma unroll
-  for (int e = 0; e < kElems; e++) {
-    const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
-    w[e] = a.w && c < a.width ? load_param(a.w, a.wdtype, c) : 1.f;
-    b[e] = a.b && c < a.width ? load_param(a.b, a.wdtype, c) : 0.f;
+  for (int e = 0; e < E; e++) {
+    const int c = column<LANES, VEC>(e, lane);
+    (e % 2 ? w[e / 2].y : w[e / 2].x) = a.w && c < a.width ? load_param(a.w, a.wdtype, c) : 1.f;
+    (e % 2 ? b[e / 2].y : b[e / 2].x) = a.b && c < a.width ? load_param(a.b, a.wdtype, c) : 0.f;
   }
   const float inv = 1.f / float(a.width);
   // every group of the block takes the same number of turns: the row sums hold barriers
   for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += step, row += step) {
-    float x[kElems];
+    float2 x[E / 2];
     if (R::ASYNC) wait_fetch<AHEAD - 1>();
     rows.take(x);
     rows.fetch(row + AHEAD * step);
     close_fetch();
-    float s = 0.f;
+    float2 s = x[0];
 #pragma unroll
-    for (int e = 0; e < kElems; e++) s += x[e];
-    const float mu = row_sum<LANES>(s, red[0]) * inv;
-    float q = 0.f;
+    for (int i = 1; i < E / 2; i++) s = add2(s, x[i]);
+    const float mu = row_sum<LANES>(sum2(s), red[0]) * inv;
+    float2 q = both(0.f);
 #pragma unroll
-    for (int e = 0; e < kElems; e++) {
-      const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
-      x[e] -= mu;
-      if (c < a.width) q += x[e] * x[e];
+    for (int i = 0; i < E / 2; i++) {
+      x[i] = add2(x[i], both(-mu));
+      // past the row's end nothing is summed (vectors end where rows do; single elements are looked at one by one)
+      if (VEC > 1) {
+        if (column<LANES, VEC>(2 * i, lane) < a.width) q = fma2(x[i], x[i], q);
+      } else {
+        if (column<LANES, VEC>(2 * i, lane) < a.width) q.x = fmaf(x[i].x, x[i].x, q.x);
+        if (column<LANES, VEC>(2 * i + 1, lane) < a.width) q.y = fmaf(x[i].y, x[i].y, q.y);
+      }
     }
-    const float rs = rsqrtf(row_sum<LANES>(q, red[1]) * inv + a.eps);
+    const float rs = rsqrtf(row_sum<LANES>(sum2(q), red[1]) * inv + a.eps);
     if (row >= a.rows) continue;
     if (lane == 0 && a.mean && LNCC_IN(row, 1, a.rows)) {
       a.mean[row] = mu;
       a.rstd[row] = rs;
     }
 #pragma unroll
+    for (int i = 0; i < E / 2; i++) x[i] = fma2(mul2(x[i], both(rs)), w[i], b[i]);
+#pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = (v * LANES + lane) * VEC;
       float o[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; i++) o[i] = x[v * VEC + i] * rs * w[v * VEC + i] + b[v * VEC + i];
+      for (int i = 0; i < VEC; i++) o[i] = (v * VEC + i) % 2 ? x[(v * VEC + i) / 2].y : x[(v * VEC + i) / 2].x;
       if (c < a.width && LNCC_IN(row * a.width + c, VEC, a.rows * a.width)) store_vec<T, VEC>(y + row * a.width + c, o);
     }
   }
+  if (R::ASYNC) wait_fetch<0>();  // nothing is under way to shared memory any more
 }
 
-template <typename T, int LANES, int VEC>
+template <typename T, int LANES, int VEC, int E>
 __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= kThreads && VEC * sizeof(T) >= 4 ? 2 : 1) backward_kernel(const Args a) {
   constexpr int THREADS = LANES > kThreads ? LANES : kThreads;
-  constexpr int ROWS = THREADS / LANES, NV = kElems / VEC;
-  typedef Rows<T, LANES, VEC, THREADS> R;
+  constexpr int ROWS = THREADS / LANES, NV = E / VEC;
+  typedef Rows<T, LANES, VEC, E, THREADS> R;
   constexpr int AHEAD = R::ASYNC ? R::kStages - 1 : 1;
   extern __shared__ __align__(16) unsigned char stage[];
   __shared__ float red[2][THREADS / 32];
@@ -207,17 +225,17 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= kThreads && VEC 
     rows_dy.fetch(row + i * step);
     close_fetch();
   }
-  float w[kElems], dw[kElems], db[kElems];
+  float2 w[E / 2], dw[E / 2], db[E / 2];
 #pragma unroll
-  for (int e = 0; e < kElems; e++) {
-    const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
-    w[e] = a.w && c < a.width ? load_param(a.w, a.wdtype, c) : 1.f;
-    dw[e] = db[e] = 0.f;
+  for (int e = 0; e < E; e++) {
+    const int c = column<LANES, VEC>(e, lane);
+    (e % 2 ? w[e / 2].y : w[e / 2].x) = a.w && c < a.width ? load_param(a.w, a.wdtype, c) : 1.f;
+    dw[e / 2] = db[e / 2] = both(0.f);
   }
   const float inv = 1.f / float(a.width);
   float mu_next = row < a.rows ? a.mean[row] : 0.f, rs_next = row < a.rows ? a.rstd[row] : 0.f;
   for (int64_t first = int64_t(blockIdx.x) * ROWS; first < a.rows; first += step, row += step) {
-    float n[kElems], d[kElems];
+    float2 n[E / 2], d[E / 2];
     const float mu = mu_next, rs = rs_next;
     mu_next = row + step < a.rows ? a.mean[row + step] : 0.f;
     rs_next = row + step < a.rows ? a.rstd[row + step] : 0.f;
@@ -227,39 +245,42 @@ __global__ void __launch_bounds__(threads_of<LANES>(), LANES <= kThreads && VEC 
     rows_x.fetch(row + AHEAD * step);
     rows_dy.fetch(row + AHEAD * step);
     close_fetch();
-    float s1 = 0.f, s2 = 0.f;
+    float2 s1 = both(0.f), s2 = both(0.f);
 #pragma unroll
-    for (int e = 0; e < kElems; e++) {  // past the row's end dy is 0, and with it every term
-      n[e] = (n[e] - mu) * rs;
-      db[e] += d[e];
-      dw[e] += d[e] * n[e];
-      d[e] *= w[e];
-      s1 += d[e];
-      s2 += d[e] * n[e];
+    for (int i = 0; i < E / 2; i++) {  // past the row's end dy is 0, and with it every term
+      n[i] = mul2(add2(n[i], both(-mu)), both(rs));
+      db[i] = add2(db[i], d[i]);
+      dw[i] = fma2(d[i], n[i], dw[i]);
+      d[i] = mul2(d[i], w[i]);
+      s1 = add2(s1, d[i]);
+      s2 = fma2(d[i], n[i], s2);
     }
     if (a.y == nullptr) continue;  // the same for every thread
-    const float m1 = row_sum<LANES>(s1, red[0]) * inv, m2 = row_sum<LANES>(s2, red[1]) * inv;
+    const float m1 = row_sum<LANES>(sum2(s1), red[0]) * inv, m2 = row_sum<LANES>(sum2(s2), red[1]) * inv;
     if (row >= a.rows) continue;
+#pragma unroll
+    for (int i = 0; i < E / 2; i++) d[i] = fma2(n[i], both(-m2 * rs), mul2(add2(d[i], both(-m1)), both(rs)));
 #pragma unroll
     for (int v = 0; v < NV; v++) {
       const int c = (v * LANES + lane) * VEC;
       float o[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; i++) o[i] = rs * (d[v * VEC + i] - m1 - n[v * VEC + i] * m2);
+      for (int i = 0; i < VEC; i++) o[i] = (v * VEC + i) % 2 ? d[(v * VEC + i) / 2].y : d[(v * VEC + i) / 2].x;
       if (c < a.width && LNCC_IN(row * a.width + c, VEC, a.rows * a.width)) store_vec<T, VEC>(dx + row * a.width + c, o);
     }
   }
-  if (R::ASYNC) wait_fetch<0>();  // nothing is under way to shared memory any more
+  if (R::ASYNC) wait_fetch<0>();
   if (a.partial == nullptr) return;
   // the block's rows meet: thread t < LANES adds the other groups' sums to its own, group by group
   float* out = a.partial + int64_t(blockIdx.x) * 2 * a.width;
   __shared__ float meet[ROWS > 1 ? THREADS : 1];
 #pragma unroll
-  for (int e = 0; e < kElems; e++) {
-    const int c = (e / VEC * LANES + lane) * VEC + e % VEC;
+  for (int e = 0; e < E; e++) {
+    const int c = column<LANES, VEC>(e, lane);
 #pragma unroll
     for (int which = 0; which < 2; which++) {
-      float v = which ? db[e] : dw[e];
+      const float2 pair = which ? db[e / 2] : dw[e / 2];
+      float v = e % 2 ? pair.y : pair.x;
       if (ROWS > 1) {
         __syncthreads();
         meet[threadIdx.x] = v;
@@ -357,11 +378,16 @@ template <typename T> __global__ void __launch_bounds__(kThreads) wide_columns_k
   out[a.width + c] = db;
 }
 
-static int lanes_for(int64_t width) {
-  int lanes = 4;
-  while (int64_t(lanes) * kElems < width) lanes *= 2;
-  return lanes;
+// Elements of a thread and threads of a row: the smallest product that holds it, of 12 or 16 by a power of two from 4.
+struct Shape {
+  int lanes, elems;
+};
+static Shape shape_for(int64_t width) {
+  for (int lanes = 4;; lanes *= 2)
+    for (int elems = 12; elems <= kElems; elems += 4)
+      if (int64_t(lanes) * elems >= width) return {lanes, elems};
 }
+static int lanes_for(int64_t width) { return shape_for(width).lanes; }
 
 // Thread blocks of a call: as many as have rows, at most what the GPU holds at once (three of 256 threads an SM forward, two
 // backward, whose sums take 120 registers; one of 512).
@@ -377,10 +403,10 @@ static int strands_for(int64_t rows, int64_t width) {
   return int(rows < 64 ? rows : 64);
 }
 
-template <typename T, int VEC, int LANES> static void launch_lanes(const Args& a, bool backward, int grid, cudaStream_t st) {
+template <typename T, int VEC, int E, int LANES> static void launch_lanes(const Args& a, bool backward, int grid, cudaStream_t st) {
   constexpr int threads = threads_of<LANES>();
-  const int ring = Rows<T, LANES, VEC, threads>::smem(), smem = backward ? 2 * ring : ring;
-  const auto kernel = backward ? backward_kernel<T, LANES, VEC> : forward_kernel<T, LANES, VEC>;
+  const int ring = Rows<T, LANES, VEC, E, threads>::smem(), smem = backward ? 2 * ring : ring;
+  const auto kernel = backward ? backward_kernel<T, LANES, VEC, E> : forward_kernel<T, LANES, VEC, E>;
   static uint64_t asked[2];  // devices that were asked for this kernel's shared memory; asking twice does no harm
   int dev = 0;
   if (smem > 40 * 1024 && cudaGetDevice(&dev) == cudaSuccess && dev < 64 && !(asked[backward] >> dev & 1)) {
@@ -388,21 +414,22 @@ template <typename T, int VEC, int LANES> static void launch_lanes(const Args& a
   }
   kernel<<<grid, threads, smem, st>>>(a);
 }
-template <typename T, int VEC> static void launch(const Args& a, bool backward, cudaStream_t st) {
+template <typename T, int VEC, int E> static void launch(const Args& a, bool backward, cudaStream_t st) {
   const int grid = blocks_for(a.rows, a.width, backward);
   switch (lanes_for(a.width)) {
-    case 4: launch_lanes<T, VEC, 4>(a, backward, grid, st); break;
-    case 8: launch_lanes<T, VEC, 8>(a, backward, grid, st); break;
-    case 16: launch_lanes<T, VEC, 16>(a, backward, grid, st); break;
-    case 32: launch_lanes<T, VEC, 32>(a, backward, grid, st); break;
-    case 64: launch_lanes<T, VEC, 64>(a, backward, grid, st); break;
-    case 128: launch_lanes<T, VEC, 128>(a, backward, grid, st); break;
-    case 256: launch_lanes<T, VEC, 256>(a, backward, grid, st); break;
-    default: launch_lanes<T, VEC, 512>(a, backward, grid, st); break;
+    case 4: launch_lanes<T, VEC, E, 4>(a, backward, grid, st); break;
+    case 8: launch_lanes<T, VEC, E, 8>(a, backward, grid, st); break;
+    case 16: launch_lanes<T, VEC, E, 16>(a, backward, grid, st); break;
+    case 32: launch_lanes<T, VEC, E, 32>(a, backward, grid, st); break;
+    case 64: launch_lanes<T, VEC, E, 64>(a, backward, grid, st); break;
+    case 128: launch_lanes<T, VEC, E, 128>(a, backward, grid, st); break;
+    case 256: launch_lanes<T, VEC, E, 256>(a, backward, grid, st); break;
+    default: launch_lanes<T, VEC, E, 512>(a, backward, grid, st); break;
   }
 }
 
-// 16-byte accesses where every row of every array starts on a 16-byte boundary, else single elements.
+// 16-byte accesses (8 for 12 elements of 16 bits) where every row of every array starts on a 16-byte boundary, else single
+// elements.
 template <typename T> static void run(const Args& a, bool backward, cudaStream_t st) {
   constexpr int VEC = 16 / int(sizeof(T));
   const bool vec = a.width % VEC == 0 && a.x_stride % VEC == 0 && aligned(a.x, 16) && (!a.y || aligned(a.y, 16)) &&
@@ -418,8 +445,11 @@ template <typename T> static void run(const Args& a, bool backward, cudaStream_t
       wide_columns_kernel<T><<<dim3(unsigned(ceil_div(a.width, kThreads)), strands_for(a.rows, a.width)), kThreads, 0, st>>>(a);
     return;
   }
-  if (vec) launch<T, VEC>(a, backward, st);
-  else launch<T, 1>(a, backward, st);
+  const bool twelve = shape_for(a.width).elems == 12;
+  if (vec && twelve) launch<T, 4, 12>(a, backward, st);
+  else if (vec) launch<T, VEC, 16>(a, backward, st);
+  else if (twelve) launch<T, 1, 12>(a, backward, st);
+  else launch<T, 1, 16>(a, backward, st);
 }
 
 static void dispatch(const Args& a, int dtype, bool backward, cudaStream_t st) {

@@ -38,6 +38,28 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, con
   *reinterpret_cast<Vec<T, V>*>(p) = v;
 }
 
+// two fp32 numbers a packed instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 A, B;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tadd.rn.f32x2 A, A, B;\n\tmov.b64 {%0, %1}, A;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 A, B;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmul.rn.f32x2 A, A, B;\n\tmov.b64 {%0, %1}, A;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 A, B, C;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmov.b64 C, {%6, %7};\n\tfma.rn.f32x2 A, A, B, C;\n\t"
+      "mov.b64 {%0, %1}, A;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 inline bool valid_dtype(int dtype) { return dtype == LNCC_F32 || dtype == LNCC_BF16 || dtype == LNCC_F16; }
 inline int elem_size(int dtype) { return dtype == LNCC_F32 ? 4 : 2; }
 inline bool aligned(const void* p, uintptr_t n) { return uintptr_t(p) % n == 0; }
