@@ -965,11 +965,16 @@ struct Call {
 
   template <int KIND, int BN, int ACT, typename T> void launch(Gemm& g) {
     const int smem = smem_bytes(BN), pairs = sm_count() / 2;
-    if (cudaFuncSetAttribute(product_kernel<KIND, BN, ACT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
-        cudaSuccess) {
-      cudaGetLastError();
-      status = LNCC_ERR_SMEM;
-      return;
+    static uint64_t asked;  // devices that were asked for this kernel's shared memory; asking twice does no harm
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !(asked >> dev & 1)) {
+      if (cudaFuncSetAttribute(product_kernel<KIND, BN, ACT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+          cudaSuccess) {
+        cudaGetLastError();
+        status = LNCC_ERR_SMEM;
+        return;
+      }
+      if (dev < 64) asked |= 1ull << dev;
     }
     const int64_t tiles = int64_t(g.m_tiles) * g.n_tiles * g.whichs * g.splits;
     run(product_kernel<KIND, BN, ACT, T>, dim3(unsigned(2 * (tiles < pairs ? tiles : pairs))), kThreads, smem, g);
@@ -1013,8 +1018,9 @@ struct Call {
     const Cut c = cut_for(KIND, a.dtype, rows, cols, whichs, g.blocks);
     g.m_tiles = c.m_tiles, g.n_tiles = c.n_tiles, g.splits = c.splits, g.whichs = whichs, g.per_split = c.per_split;
     const int a_box = a_mn(KIND) ? 64 : 128, b_box = b_mn(KIND) ? 64 : c.bn / 2;
-    if (!make_map(&g.a0, a0, a_box) || !make_map(&g.a1, a1, a_box) || !make_map(&g.b0, b0, b_box) ||
-        !make_map(&g.b1, b1, b_box) || !make_map(&g.b2, b2, 64)) {
+    constexpr bool second_a = KIND == HIDDEN || KIND == DX || KIND == DW_UP, second_b = gated(KIND) || KIND == DX;
+    if (!make_map(&g.a0, a0, a_box) || (second_a && !make_map(&g.a1, a1, a_box)) || !make_map(&g.b0, b0, b_box) ||
+        (second_b && !make_map(&g.b1, b1, b_box)) || (KIND == HIDDEN && !make_map(&g.b2, b2, 64))) {
       status = LNCC_ERR_CUDA;
       return;
     }

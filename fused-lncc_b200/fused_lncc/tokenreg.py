@@ -11,7 +11,7 @@ volume, 107520 for 160 x 192 x 224. A head turns each token into a displacement,
 resolution, warps the moving volume, and is trained under LNCC + lam * diffusion. The projections in and out
 and the head are ordinary torch products.
 
-    python -m fused_lncc.tokenreg --size 64 --iters 200
+    python -m fused_lncc.tokenreg --size 64
 """
 import argparse
 import json
@@ -98,7 +98,7 @@ def train(net, pairs, base, iters=60, lr=2e-3, lam=0.5, kernel_size=7):
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--size", type=int, default=64)
-    ap.add_argument("--iters", type=int, default=200)
+    ap.add_argument("--iters", type=int, default=600)
     ap.add_argument("--width", type=int, default=96)
     ap.add_argument("--hidden", type=int, default=256)
     ap.add_argument("--depth", type=int, default=2)

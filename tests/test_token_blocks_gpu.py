@@ -163,13 +163,27 @@ def _scan_check(x, gate, state, reverse, dh, dlast):
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("B,T,C", [(1, 1, 1), (2, 1, 40), (3, 2, 33), (1, 15, 8), (2, 16, 3), (1, 17, 96), (2, 63, 130),
                                    (1, 64, 64), (3, 65, 31), (1, 127, 256), (2, 129, 16), (1, 1000, 24), (2, 1023, 7),
-                                   (1, 4097, 66), (5, 300, 97), (1, 9001, 16)])
+                                   (1, 4097, 66), (5, 300, 97), (1, 9001, 16), (40, 33, 1500),
+                                   (2, 20, 80000)])
 def test_scan(B, T, C, dtype):
     seed = B + T + C
     reverse = seed % 2 == 0
     state = _rand(seed + 2, B, C) if seed % 3 else None
     _scan_check(_rand(seed, B, T, C, dtype=dtype), _rand(seed + 1, B, T, C, dtype=dtype, scale=2.0, shift=1.5).clamp(-23, 23),
                 state, reverse, _rand(seed + 3, B, T, C, dtype=dtype), _rand(seed + 4, B, C))
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+def test_scan_same_bits_every_time(reverse):
+    x, gate, dh = (_rand(s, 2, 30000, 40) for s in (1, 2, 3))
+    x.requires_grad_(True), gate.requires_grad_(True)
+
+    def run():
+        h, last = fused_lncc.fused_gated_scan(x, gate, reverse=reverse)
+        return (h, last, *torch.autograd.grad(h, (x, gate), dh))
+    first = run()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(run(), first))
 
 
 @pytest.mark.parametrize("reverse", [False, True])
@@ -264,6 +278,21 @@ def test_scan_past_32_bits():
     _close(h[-1:, -40:, -8:], ref, "h", 40)
     _close(last[-1:, -8:], ref, "last", 40)
     assert h[0].abs().max() == 0
+
+
+def test_scan_past_32_bits_along_time():
+    T, C = 2 ** 22, 520   # few channels: T is cut, and the last tiles lie past 2^31 elements
+    x = torch.zeros(1, T, C, dtype=BF16, device="cuda")
+    gate = torch.zeros(1, T, C, dtype=BF16, device="cuda")
+    x[0, -40:, -8:] = _rand(1, 40, 8, dtype=BF16)
+    h, last = fused_lncc.fused_gated_scan(x, gate)
+    ref = ob.gated_scan(x[:, -40:, -8:], gate[:, -40:, -8:])
+    _close(h[:, -40:, -8:], ref, "h", 40)
+    _close(last[:, -8:], ref, "last", 40)
+    assert h[0, :-40].abs().max() == 0
+    h, last = fused_lncc.fused_gated_scan(x, gate, reverse=True)
+    ref = ob.gated_scan(x[:, -40:, -8:], gate[:, -40:, -8:], reverse=True)
+    _close(h[:, -40:, -8:], ref, "h", 40)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
