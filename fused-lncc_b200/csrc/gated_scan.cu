@@ -340,26 +340,36 @@ template <typename T, int V, int LANES> __global__ void __launch_bounds__(kThrea
 
 template <typename T, int V, int LANES, bool SPLIT> __global__ void __launch_bounds__(kThreads, 2) back_run_kernel(const Args p) {
   const Place<V, LANES> at(p);
+  const T* gate = static_cast<const T*>(p.gate) + at.b * p.gate_b + at.c;
+  const T* x = static_cast<const T*>(p.x) + at.b * p.x_b + at.c;
+  const T* dh = static_cast<const T*>(p.dh) + at.b * p.dh_b + at.c;
+  const int64_t keeps = (p.T + kKeep - 1) / kKeep, last = at.live ? (at.to - 1) / kKeep * kKeep : 0;
+  Steps<T, V> sg, sx, sd;
+  // fp32: the last steps come in while the state is formed (48 -> 43 us at 6 x 4093 x 389; two 16-bit channels a thread have no
+  // registers left for it, 31 -> 35 us at 107520 x 96)
+  const bool ahead = SPLIT && sizeof(T) == 4 && at.live && last + kKeep <= at.to;
+  if (ahead) {
+    sg.template load<true>(gate, p.gate_t, last, at.to);
+    sx.template load<true>(x, p.x_t, last, at.to);
+    sd.template load<true>(dh, p.dh_t, last, at.to);
+  }
   float q[V];
   if (SPLIT) wait_for_previous_kernel();
 #pragma unroll
   for (int v = 0; v < V; v++) q[v] = p.dlast && at.c < p.C ? p.dlast[at.b * p.C + at.c + v] : 0.f;
   if (SPLIT) start_state<V, LANES>(p, at, true, q);
   if (!at.live) return;
-  const T* gate = static_cast<const T*>(p.gate) + at.b * p.gate_b + at.c;
-  const T* x = static_cast<const T*>(p.x) + at.b * p.x_b + at.c;
-  const T* dh = static_cast<const T*>(p.dh) + at.b * p.dh_b + at.c;
   T* dx = static_cast<T*>(p.dx) + at.b * p.out_b + at.c;
   T* dgate = static_cast<T*>(p.dgate) + at.b * p.out_b + at.c;
-  const int64_t keeps = (p.T + kKeep - 1) / kKeep;
   const auto block = [&](auto full, int64_t t) {
     constexpr bool FULL = decltype(full)::value;
-    Steps<T, V> sg, sx, sd;
     float h[V], apart[kKeep][V];  // apart: h_{t-1} - x_t
     load_vec<float, V>(p.kept + (at.b * keeps + t / kKeep) * p.C + at.c, h);
-    sg.template load<FULL>(gate, p.gate_t, t, at.to);
-    sx.template load<FULL>(x, p.x_t, t, at.to);
-    sd.template load<FULL>(dh, p.dh_t, t, at.to);
+    if (!ahead || t != last) {
+      sg.template load<FULL>(gate, p.gate_t, t, at.to);
+      sx.template load<FULL>(x, p.x_t, t, at.to);
+      sd.template load<FULL>(dh, p.dh_t, t, at.to);
+    }
 #pragma unroll
     for (int i = 0; i < kKeep; i++) {
       if (!FULL && t + i >= at.to) break;
@@ -392,7 +402,7 @@ template <typename T, int V, int LANES, bool SPLIT> __global__ void __launch_bou
       store_vec<T, V>(to_gate, og);
     }
   };
-  int64_t t = (at.to - 1) / kKeep * kKeep;
+  int64_t t = last;
   if (t + kKeep > at.to) block(std::false_type(), t), t -= kKeep;
   for (; t >= at.from; t -= kKeep) block(std::true_type(), t);
   if (at.from == 0 && p.dstate && LNCC_IN(at.b * p.C + at.c, V, p.B * p.C))
