@@ -292,8 +292,9 @@ int lncc_launch_count(int64_t B, int64_t D, int64_t H, int64_t W, int kernel_siz
  * dtype (LNCC_F32, LNCC_BF16, LNCC_F16) is the type of every array whose parameter is a void*, except where said;
  * float* parameters are fp32 for every dtype. All arithmetic and every sum is fp32; results are rounded once, on the
  * store. Strides are in elements. Results are the same bits run after run: no sum's order depends on timing. Pointers
- * need the alignment of their element, scratch 16 bytes; arrays whose rows lie on 16-byte boundaries run fastest. No
- * counterpart in the reference.
+ * need the alignment of their element, scratch 16 bytes; arrays whose rows lie on 16-byte boundaries run fastest. Inputs
+ * and outputs do not overlap. In the checked build the global accesses of these kernels are range-checked; what TMA reads
+ * is bounded by its tensor maps. No counterpart in the reference.
  */
 
 /*
@@ -320,7 +321,8 @@ int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, i
 /*
  * The gated linear recurrence over (B, T, C):
  *   a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t, h_0 = state,
- * for t = 1 .. T, or from the last step to the first with reverse != 0. gate = +inf keeps the state, -inf drops it.
+ * for t = 1 .. T, or from the last step to the first with reverse != 0. gate = +inf keeps the state, -inf drops it (for
+ * 16-bit dtypes a gate below -87 counts as -87).
  *   x, gate  : batch strides x_b, gate_b, time strides x_t, gate_t.
  *   state    : NULL (zeros) or (B, C).
  *   h        : (B, T, C) contiguous.        last: (B, C), the state after the last step taken (T == 0: state).
@@ -349,6 +351,9 @@ enum lncc_activation { LNCC_ACT_SILU = 0, LNCC_ACT_GELU = 1, LNCC_ACT_RELU = 2 }
  *   x          : M rows of K, x_stride elements apart.     w_gate, w_up: (F, K) contiguous.     w_down: (N, F) contiguous.
  *   y          : (M, N) contiguous.
  * Limits: K, F, N <= 2^20, M <= 2^30 - 1 (LNCC_ERR_TOO_LARGE).
+ * The scratch starts with a word that lncc_check_abort reads, as the loss's workspace does: a bounded wait of the products
+ * (2 s each) that ran out gives LNCC_ERR_ABORTED there and NaN results. For 16-bit dtypes h (and dg, du in the backward pass)
+ * are rounded to dtype between the products; for up to four tokens h stays fp32.
  */
 size_t lncc_gated_ffn_scratch_bytes(int64_t M, int64_t K, int64_t F, int64_t N, int dtype, int backward);
 int lncc_gated_ffn_forward(const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down,
