@@ -914,6 +914,9 @@ static Plan plan_for(const Args& a, bool backward) {
   return p;
 }
 
+// Unnamed, so that the marks of what this library has asked the device for are its own: the checked build, loaded beside it, has
+// kernels of its own under the same names.
+namespace {
 struct Call {
   const Args& a;
   Plan plan;
@@ -1050,6 +1053,8 @@ struct Call {
     }
   }
 };
+
+}  // namespace
 
 static int tokens_of(int64_t M) { return M <= 1 ? 1 : M <= 2 ? 2 : 4; }
 static bool few(const Args& a) {
