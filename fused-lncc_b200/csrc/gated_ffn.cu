@@ -235,6 +235,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x == 64) {  // the maps are the launch's own: they may come in before the kernel ahead has ended
+    prefetch_map(&g.a0);
+    prefetch_map(&g.b0);
+    if (KIND == HIDDEN || KIND == DX || KIND == DW_UP) prefetch_map(&g.a1);
+    if (gated(KIND) || KIND == DX) prefetch_map(&g.b1);
+    if (KIND == HIDDEN) prefetch_map(&g.b2);
+  }
   if (warp == 1) {
     tmem_alloc<512>(smem_addr(&tmem_at));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
@@ -617,9 +624,10 @@ __device__ __noinline__ float gate_in_order(const NearZero& z, int64_t row, int6
 
 // fp32: dg, du and h, taken apart, from g, u and dh (rows ld apart, like the results). Eight neighbours a thread.
 // ReLU's derivative jumps at g = 0, where the last bits of g decide and one element that falls the other way is off by all of
-// its gradient. The sum of the tensor cores and the plain fp32 sum in the order of k are each within (K + 64) 2^-24 |x| |w|
-// of the exact one; where g is closer to 0 than both together, it is formed again as the plain sum (about one gate in
-// 2500 at K = 389; forming all of them so took 100 us of 413 at 4093 x 389 x 1037).
+// its gradient. The plain fp32 sum in the order of k is within K 2^-24 |x| |w| of the exact one, and the sum of the tensor
+// cores within (64 + K/256) 2^-24 |x| |w|: 16 cut additions in each accumulator, the parts left out, one rounding for each
+// 256 of K. Where g is closer to 0 than both together, it is formed again as the plain sum (about one gate in 2700 at
+// K = 389; forming all of them so took 100 us of 413 at 4093 x 389 x 1037).
 template <int ACT>
 __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g, const float* __restrict__ u,
                                                     const float* __restrict__ dh, __nv_bfloat16* dg, __nv_bfloat16* du,
@@ -642,7 +650,7 @@ __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g,
     }
     if (ACT == LNCC_ACT_RELU) {
       const int64_t row = i / z.ld, col = i - row * z.ld;
-      const float near = here ? z.norms[row] * (float(z.K + 64) * 1.1920929e-7f) : 0.f;
+      const float near = here ? z.norms[row] * (float(z.K + 64 + z.K / 256) * 5.9604645e-8f) : 0.f;
 #pragma unroll
       for (int k = 0; k < 8; k++) {
         const bool again = here && col + k < z.F && !(fabsf(vg[k]) > near * z.norms[z.M + col + k]);
@@ -832,7 +840,7 @@ inline int64_t lead(int64_t cols) { return (cols + 15) / 16 * 16; }  // rows of 
 // How a product is cut into tiles and its inner axis into splits: the cheapest by a model of the time in clocks. A block of
 // 64 of a tile of 256 columns takes 590 and one of 128 columns 515 (measured; the tensor cores then wait for A's share of
 // shared memory, not for products), a tile 1500 around them; partial sums are written and read at 2200 bytes a clock, and
-// their join costs a launch. Of equal ones the fewest splits.
+// their join costs a launch (9000 clocks with what the host pays for it). Of equal ones the fewest splits.
 struct Cut {
   int bn, m_tiles, n_tiles, splits, per_split;
 };
@@ -844,12 +852,11 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
     if (kind == HIDDEN && bn == 128) break;
     const int width = gated(kind) ? bn / 2 : bn;
     const int64_t m_tiles = ceil_div(rows, 256), n_tiles = ceil_div(cols, width), tiles = m_tiles * n_tiles * whichs;
-    for (int want = 1; want <= 64; want++) {
+    for (const int want : {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 18, 20, 24, 28, 32, 37, 48, 64}) {
       if (want > 1 && (gated(kind) || kind == DH || blocks < 4 * want)) break;
       const int64_t per = ceil_div(blocks, want), splits = ceil_div(blocks, per);
-      if (splits != want) continue;
       double t = double(ceil_div(tiles * splits, pairs)) * (double(per) * parts * (bn == 256 ? 590 : 515) + 1500);
-      if (splits > 1) t += 6000 + 8.0 * double(splits) * whichs * double(rows) * double(cols) / 2200;
+      if (splits > 1) t += 9000 + 8.0 * double(splits) * whichs * double(rows) * double(cols) / 2200;
       if (best.bn == 0 || t < 0.98 * least) {
         best = {bn, int(m_tiles), int(n_tiles), int(splits), int(per)};
         least = t;
@@ -1101,13 +1108,13 @@ template <typename T> static int few_forward(const Args& a, void* scratch, cudaS
   return few_tokens<T, 1>(a, h, st);
 }
 
-static int forward(const Args& a, void* scratch, cudaStream_t stream) {
+static int forward(const Args& a, const Plan& plan, void* scratch, cudaStream_t stream) {
   if (few(a)) {
     if (a.dtype == LNCC_F32) return few_forward<float>(a, scratch, stream);
     if (a.dtype == LNCC_BF16) return few_forward<__nv_bfloat16>(a, scratch, stream);
     return few_forward<__half>(a, scratch, stream);
   }
-  Call c = {a, plan_for(a, false), static_cast<char*>(scratch), stream, LNCC_OK};
+  Call c = {a, plan, static_cast<char*>(scratch), stream, LNCC_OK};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg),
                wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu), wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd),
                h = c.hidden(c.plan.h);
@@ -1117,8 +1124,8 @@ static int forward(const Args& a, void* scratch, cudaStream_t stream) {
   return c.status;
 }
 
-static int backward(const Args& a, void* scratch, cudaStream_t stream) {
-  Call c = {a, plan_for(a, true), static_cast<char*>(scratch), stream, LNCC_OK};
+static int backward(const Args& a, const Plan& plan, void* scratch, cudaStream_t stream) {
+  Call c = {a, plan, static_cast<char*>(scratch), stream, LNCC_OK};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), dy = c.operand(a.dy, a.M, a.N, a.dy_stride, c.plan.dy),
                wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg), wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu),
                wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd);
@@ -1183,14 +1190,14 @@ int lncc_gated_ffn_forward(const void* x, int64_t x_stride, const void* w_gate, 
   if (!ffn::good(x, dtype) || !ffn::good(w_gate, dtype) || !ffn::good(w_up, dtype) || !ffn::good(w_down, dtype) ||
       !ffn::good(y, dtype) || (x_stride < K && M > 1))
     return LNCC_ERR_BAD_ARG;
-  if (!scratch || !blk::aligned(scratch, 16) || scratch_bytes < lncc_gated_ffn_scratch_bytes(M, K, F, N, dtype, 0))
-    return LNCC_ERR_WORKSPACE;
-  const int cb = blk::check_begin();
-  if (cb != LNCC_OK) return cb;
   ffn::Args p = {};
   p.x = x, p.x_stride = x_stride, p.wg = w_gate, p.wu = w_up, p.wd = w_down, p.act = act, p.dtype = dtype, p.y = y;
   p.M = M, p.K = K, p.F = F, p.N = N;
-  const int run = ffn::forward(p, scratch, stream);
+  const ffn::Plan plan = ffn::plan_for(p, false);
+  if (!scratch || !blk::aligned(scratch, 16) || scratch_bytes < plan.total) return LNCC_ERR_WORKSPACE;
+  const int cb = blk::check_begin();
+  if (cb != LNCC_OK) return cb;
+  const int run = ffn::forward(p, plan, scratch, stream);
   const int ended = blk::check_end(stream);
   return run != LNCC_OK ? run : ended;
 }
@@ -1213,15 +1220,15 @@ int lncc_gated_ffn_backward(const void* dy, int64_t dy_stride, const void* x, in
   if (!ffn::good(x, dtype) || !ffn::good(w_gate, dtype) || !ffn::good(w_up, dtype) || !ffn::good(w_down, dtype) ||
       !ffn::good(dy, dtype) || (x_stride < K && M > 1) || (dy_stride < N && M > 1))
     return LNCC_ERR_BAD_ARG;
-  if (!scratch || !blk::aligned(scratch, 16) || scratch_bytes < lncc_gated_ffn_scratch_bytes(M, K, F, N, dtype, 1))
-    return LNCC_ERR_WORKSPACE;
-  const int cb = blk::check_begin();
-  if (cb != LNCC_OK) return cb;
   ffn::Args p = {};
   p.x = x, p.x_stride = x_stride, p.dy = dy, p.dy_stride = dy_stride, p.wg = w_gate, p.wu = w_up, p.wd = w_down;
   p.act = act, p.dtype = dtype, p.dx = dx, p.dwg = dw_gate, p.dwu = dw_up, p.dwd = dw_down;
   p.M = M, p.K = K, p.F = F, p.N = N;
-  const int run = ffn::backward(p, scratch, stream);
+  const ffn::Plan plan = ffn::plan_for(p, true);
+  if (!scratch || !blk::aligned(scratch, 16) || scratch_bytes < plan.total) return LNCC_ERR_WORKSPACE;
+  const int cb = blk::check_begin();
+  if (cb != LNCC_OK) return cb;
+  const int run = ffn::backward(p, plan, scratch, stream);
   const int ended = blk::check_end(stream);
   return run != LNCC_OK ? run : ended;
 }
