@@ -208,10 +208,14 @@ template <int KIND, int BN, int ACT, typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ Gemm g) {
   constexpr int STAGES = stages(BN), BT = b_tile(BN), HALF = BN / 2;
   constexpr bool AM = a_mn(KIND), BM = b_mn(KIND), F32 = sizeof(T) == 4;
-  constexpr int ACCS = KIND == HIDDEN ? 1 : 2;         // accumulators in tensor memory
+  // Tiles of accumulators in tensor memory. HIDDEN of 256 columns has one: dh then alternates between two places, so it may
+  // run while the last tile is read, and g and u wait for that.
+  constexpr bool ONE = KIND == HIDDEN && BN == 256;
+  constexpr int ACCS = ONE ? 1 : 2;
+  constexpr int DH_BYTES = BN == 256 ? 8192 : 4096;    // a CTA's share of Wd in a stage: 64 or 32 columns
   constexpr int PARTS = F32 ? 6 : 1;                   // products of parts of the operands
   constexpr int CHUNK = F32 ? kChunk : 1 << 30;        // blocks that one accumulator takes
-  static_assert(KIND != HIDDEN || (BN == 256 && !F32), "dh's share of B is one block of 64 columns a CTA");
+  static_assert(KIND != HIDDEN || !F32, "fp32 has GATES and DH");
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
   const uint32_t tiles_at = smem_addr(smem);
@@ -275,7 +279,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             const bool dh = KIND == HIDDEN && b < g.k_steps2;              // HIDDEN: dh first
             const bool second = KIND == DX && b >= g.k_steps;              // DX: du Wu after dg Wg
             const int k = 64 * (KIND == HIDDEN && !dh ? b - g.k_steps2 : second ? b - g.k_steps : b);
-            if (rank == 0) mbar_expect(full + 8 * stage, 2 * (kATile + (dh ? 8192 : BT)));
+            if (rank == 0) mbar_expect(full + 8 * stage, 2 * (kATile + (dh ? DH_BYTES : BT)));
             const CUtensorMap* am = dh || second ? &g.a1 : a_first;
             if (AM) {
               tma_load(am, at, bar, m0, k, pa);
@@ -283,8 +287,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             } else {
               tma_load(am, at, bar, k, m0, pa);
             }
-            if (dh) {  // half of the tile's 128 columns of Wd, which memory holds along F
-              tma_load(&g.b2, bt, bar, w.n * HALF + int(rank) * 64, k, pb);
+            if (dh) {  // half of the tile's columns of Wd, which memory holds along F
+              tma_load(&g.b2, bt, bar, w.n * HALF + int(rank) * (HALF / 2), k, pb);
             } else if (gated(KIND)) {  // the gate's rows in one CTA, the up projection's in the other
               tma_load(rank ? &g.b1 : &g.b0, bt, bar, k, w.n * HALF, pb);
             } else if (BM) {
@@ -318,15 +322,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         const int steps = (F32 ? min(CHUNK, w.to - c) : w.to - c) * PARTS;
         const int acc = ACCS == 2 ? turn & 1 : 0;
         const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
-        // HIDDEN: dh alternates between two places, so it may run while the last tile is read; g and u wait for that
-        const uint32_t d_dh = tmem + BN + (turn & 1) * HALF, d = tmem + (ACCS == 2 ? acc * 256 : 0);
-        if (KIND != HIDDEN) {
+        const uint32_t d = tmem + (ACCS == 2 ? acc * 256 : 0), d_dh = ONE ? tmem + BN + (turn & 1) * HALF : d + BN;
+        if (!ONE) {
           if (!(ok = mbar_wait(acc_empty + 8 * acc, acc_phase ^ 1, gave_up))) break;
           fence_after();
         }
         for (int s = 0; s < steps; s++) {
           const bool dh = KIND == HIDDEN && s < g.k_steps2;
-          if (KIND == HIDDEN && s == g.k_steps2) {
+          if (ONE && s == g.k_steps2) {
             if (!(ok = mbar_wait(acc_empty, acc_phase ^ 1, gave_up))) break;
             fence_after();
           }
@@ -334,8 +337,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           fence_after();
           const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile;
           const uint64_t da = AM ? desc_mn(at, 8192) : desc_k(at);
-          const uint64_t db = BM || dh ? desc_mn(bt, 8192) : desc_k(bt);
-          const uint64_t a_step = AM ? 128 : 2, b_step = BM || dh ? 128 : 2;
+          const uint64_t db = dh && BN == 128 ? desc_mn_32(bt) : BM || dh ? desc_mn(bt, 8192) : desc_k(bt);
+          const uint64_t a_step = AM ? 128 : 2, b_step = dh && BN == 128 ? 64 : BM || dh ? 128 : 2;
           const bool first = s == 0 || (KIND == HIDDEN && s == g.k_steps2);
 #pragma unroll
           for (int k = 0; k < 4; k++)
@@ -454,7 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
               if (ok) {
                 tmem_load(at, v[0]);
                 tmem_load(at + HALF, v[1]);
-                if (KIND == HIDDEN) tmem_load(at + BN + (turn & 1) * HALF, v[2]);
+                if (KIND == HIDDEN) tmem_load(at + BN + (ONE ? (turn & 1) * HALF : 0), v[2]);
                 wait_ld(v[0]);
                 wait_ld(v[1]);
                 if (KIND == HIDDEN) wait_ld(v[2]);
@@ -849,13 +852,19 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
   Cut best = {};
   double least = 0;
   for (int bn = 256; bn >= 128; bn -= 128) {
-    if (kind == HIDDEN && bn == 128) break;
     const int width = gated(kind) ? bn / 2 : bn;
     const int64_t m_tiles = ceil_div(rows, 256), n_tiles = ceil_div(cols, width), tiles = m_tiles * n_tiles * whichs;
     for (const int want : {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 18, 20, 24, 28, 32, 37, 48, 64}) {
       if (want > 1 && (gated(kind) || kind == DH || blocks < 4 * want)) break;
       const int64_t per = ceil_div(blocks, want), splits = ceil_div(blocks, per);
       double t = double(ceil_div(tiles * splits, pairs)) * (double(per) * parts * (bn == 256 ? 590 : 515) + 1500);
+      // HIDDEN on 256 columns: g and u of the next tile wait for the epilogue, and only dh, half of the blocks, runs meanwhile.
+      // On 128 columns everything overlaps, but a block costs more. Measured, clocks a tile: 10900 and 5000 at 2 + 2 blocks
+      // (107520 x 96 x 256: 69 us against 61), 11800 and 7000 at 4 + 4 (68 against 74), 15700 and 11750 at 8 + 8.
+      if (kind == HIDDEN) {
+        const double half = double(per) / 2, wide = 9700 + 590 * half;
+        t = double(ceil_div(tiles, pairs)) * (bn == 128 ? 2600 + 1200 * half : wide > 1690 * half ? wide : 1690 * half);
+      }
       if (splits > 1) t += 9000 + 8.0 * double(splits) * whichs * double(rows) * double(cols) / 2200;
       if (best.bn == 0 || t < 0.98 * least) {
         best = {bn, int(m_tiles), int(n_tiles), int(splits), int(per)};
@@ -999,8 +1008,7 @@ struct Call {
     }
   }
   template <int KIND, typename T> void launch_type(Gemm& g, int bn) {
-    if constexpr (KIND == HIDDEN) launch_act<KIND, 256, T>(g);
-    else if (bn == 256) launch_act<KIND, 256, T>(g);
+    if (bn == 256) launch_act<KIND, 256, T>(g);
     else launch_act<KIND, 128, T>(g);
   }
 
@@ -1030,7 +1038,7 @@ struct Call {
     const int a_box = a_mn(KIND) ? 64 : 128, b_box = b_mn(KIND) ? 64 : c.bn / 2;
     constexpr bool second_a = KIND == HIDDEN || KIND == DX || KIND == DW_UP, second_b = gated(KIND) || KIND == DX;
     if (!make_map(&g.a0, a0, a_box) || (second_a && !make_map(&g.a1, a1, a_box)) || !make_map(&g.b0, b0, b_box) ||
-        (second_b && !make_map(&g.b1, b1, b_box)) || (KIND == HIDDEN && !make_map(&g.b2, b2, 64))) {
+        (second_b && !make_map(&g.b1, b1, b_box)) || (KIND == HIDDEN && !make_map(&g.b2, b2, 64, c.bn / 4))) {
       status = LNCC_ERR_CUDA;
       return;
     }

@@ -95,6 +95,10 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return desc_common(a
 __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t block_bytes) {
   return desc_common(addr) | (uint64_t(block_bytes >> 4) << 16);
 }
+// MN-major with the 64-byte swizzle: one block of 32 rows, units of 8 inner steps 512 bytes apart, 16 steps are 1024.
+__device__ __forceinline__ uint64_t desc_mn_32(uint32_t addr) {
+  return uint64_t((addr & 0x3FFFF) >> 4) | (1ull << 16) | (uint64_t(512 >> 4) << 32) | (1ull << 46) | (4ull << 61);
+}
 // Instruction descriptor: fp32 accumulators, 256 rows of the pair, n columns.
 __device__ __forceinline__ uint32_t instr_desc(bool bf16, bool a_mn, bool b_mn, int n) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) |
@@ -178,15 +182,17 @@ struct Matrix {
   int planes;
   bool bf16;
 };
-// Map of boxes of 64 elements by `box_rows` rows; what a box reaches past the matrix reads as zero.
-inline bool make_map(CUtensorMap* map, const Matrix& m, int box_rows) {
+// Map of boxes of 64 elements by `box_rows` rows (or of 32, with the 64-byte swizzle); what a box reaches past the matrix reads
+// as zero.
+inline bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int box_cols = 64) {
   const EncodeTiled encode = encode_tiled();
   if (!encode) return false;
   const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), cuuint64_t(m.planes)};
   const cuuint64_t strides[2] = {cuuint64_t(m.ld) * 2, m.planes > 1 ? cuuint64_t(m.plane) * 2 : cuuint64_t(m.ld) * 2};
-  const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {cuuint32_t(box_cols), cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
   return encode(map, m.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, m.p, dims, strides, box,
-                steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 

@@ -390,6 +390,54 @@ def test_ffn_empty_and_some_gradients():
         _near(g, ref[name], BF16)
 
 
+def test_ffn_past_32_bits():
+    M, K, F, N = 2 ** 31 // 2048 + 300, 16, 2048, 24   # the hidden matrices pass 2^31 elements
+    x, dy = torch.zeros(M, K, dtype=BF16, device="cuda"), torch.zeros(M, N, dtype=BF16, device="cuda")
+    x[-200:], dy[-200:] = _rand(1, 200, K, dtype=BF16), _rand(2, 200, N, dtype=BF16)
+    _, wg, wu, wd, _ = _ffn_tensors(1, K, F, N, BF16, 3)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = fused_lncc.fused_gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    ref = ob.gated_ffn(x[-200:], wg, wu, wd, "silu", dy[-200:])
+    _near(y[-200:].detach(), ref["y"], BF16)
+    _near(grads[0][-200:], ref["dx"], BF16)
+    for name, g in zip(("dw_gate", "dw_up", "dw_down"), grads[1:]):
+        _near(g, ref[name], BF16)
+    assert y[:-200].abs().max() == 0 and grads[0][:-200].abs().max() == 0
+
+
+def test_ffn_one_matrix_for_gate_and_up():
+    x, wg, _, wd, dy = _ffn_tensors(140, 64, 96, 64, F32, 21)
+    wg.requires_grad_(True)
+    (g,) = torch.autograd.grad(fused_lncc.fused_gated_ffn(x, wg, wg, wd), wg, dy)
+    ref = ob.gated_ffn(x, wg, wg, wd, "silu", dy)
+    _near(g, ref["dw_gate"] + ref["dw_up"], F32)
+
+
+def test_ffn_relu_gates_at_zero():
+    """fp32 gates that are exactly 0, or closer to 0 than any order of summation can tell: the derivative there is that of the
+    plain sum in the order of k, and an exact 0 has derivative 0."""
+    M, K, F = 130, 300, 72
+    x, wg = _rand(1, M, K), _rand(2, F, K)
+    x[:, K // 2:], wg[:, K // 2:] = x[:, :K // 2], -wg[:, :K // 2]      # every gate is 0 up to rounding
+    x[5] = 0
+    _, _, wu, wd, dy = _ffn_tensors(M, K, F, 64, F32, 4)
+    x.requires_grad_(True)
+    (dx,) = torch.autograd.grad(fused_lncc.fused_gated_ffn(x, wg, wu, wd, "relu"), x, dy)
+    xs, ws = x.detach().cpu(), wg.cpu()
+    # a multiply-add rounds once: the sum of products in 64 bits, rounded to fp32 after each (their products are exact there)
+    g = torch.zeros(M, F, dtype=torch.float64)
+    for k in range(K):
+        g = (g + xs[:, k, None].double() * ws[None, :, k].double()).float().double()
+    on = (g > 0).double().cuda()
+    assert 0 < on.mean() < 1
+    x64, g64 = x.detach().double(), g.cuda()
+    dh = dy.double() @ wd.double()
+    want = (dh * (x64 @ wu.double().T) * on) @ wg.double() + (dh * g64.clamp(min=0)) @ wu.double()
+    _near(dx, want, F32)
+    assert dx[5].isfinite().all()
+
+
 def test_ffn_same_bits_every_time():
     x, wg, wu, wd, dy = _ffn_tensors(3000, 96, 160, 96, BF16, 5)
     wg.requires_grad_(True), wd.requires_grad_(True)
