@@ -119,7 +119,7 @@ def build_torch_ops(force=False, verbose=False):
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in includes),
            "-o", out + ".tmp", src, f"-L{LIB_DIR}", f"-l:{os.path.basename(lib)}", f"-L{os.path.join(torch_dir, 'lib')}",
-           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     _run(cmd, out, verbose)
     os.replace(out + ".tmp", out)
     return out

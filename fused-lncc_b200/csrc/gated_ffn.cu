@@ -6,15 +6,19 @@
 //
 // Every product runs on the tensor cores, in one kernel whose epilogue does what follows it: UP forms g and u side by side
 // in tensor memory and writes h alone; HIDDEN forms dh, g and u (again, from x) and writes dg, du and h (for fp32 GATES
-// writes g and u, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is split over
-// the GPU, fp32 partial sums that a last kernel adds in order.
+// writes g and u, DH dh, and a kernel of its own reads the three); the others write a result or, where a long inner axis is
+// split over the GPU, fp32 partial sums that a last kernel adds in order.
 //
 // A pair of CTAs takes a tile of 256 rows by up to 256 columns (cta_group::2): each loads its 128 rows of A and half the
 // columns of B, 64 steps of the inner axis at a time, into a ring of TMA stages; one thread of the pair issues
-// the products into tensor memory, and eight warps of each CTA read finished tiles back while the next one runs.
+// the products into tensor memory, and sixteen warps of each CTA read finished tiles back while the next one runs.
 // Halving B between the pair matters: a tile of 256 x 256 asks L2 for 64 bytes a clock and SM at the full rate of the
 // tensor cores, one of 128 x 256 for 96. The grid stays (one pair for each two SMs) and walks over the tiles, columns
 // first, so that the pairs at work share rows of A and the weights stay in L2.
+// Measured at 16384 x 1024 x 4096 bf16, each kernel by itself: UP 174 us (1580 TFLOP/s), DOWN 96 and DX 186 (1430 and 1480, four rounds of tiles for 3.46);
+// DW_UP 185, DW_DOWN 96, HIDDEN 363 (1140, its dh on 128 columns). The products alone,
+// with no loads and no epilogue, take 588 clocks a block of a tile of 256 x 256, DX's 609. At 107520 x 96 x 256, where bytes count: UP 34 us
+// (2.2 TB/s), HIDDEN 61 (3.4 TB/s), the epilogue's instructions and latency bounding both.
 //
 // Nothing of the hidden layer is kept between forward and backward. Forming g and u again costs 4 of 22 M F K products of a
 // training step, and saves writing and reading 4 M F bytes and a rounding of g and u.

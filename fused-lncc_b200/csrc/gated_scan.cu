@@ -13,6 +13,9 @@
 // kernel finds most of what it reads again in L2. Backward the same runs from the end, and h is formed again, 16 steps at a
 // time, from the fp32 states that the forward pass kept before each 16; that reads h's 2 or 4 bytes a step less than
 // saving h would, and h_{t-1} is not rounded to 16 bits.
+// Measured: 2 x 32768 x 256 fp16 16 + 21 us (its bytes once: 15), 107520 x 96 bf16 11 + 16 forward and 13 + 29 backward (10, 17),
+// 6 x 4093 x 389 fp32 19 + 26 and 23 + 44 (18, 29). One kernel that reads everything once, tiles waiting for earlier tiles' sums,
+// took 47 us for the first: at four blocks an SM too few bytes are in flight while tiles wait.
 #include "lncc_block.cuh"
 
 #include <type_traits>

@@ -7,8 +7,9 @@
 // then the centred squares are summed in fp32 without a second read (the two-step variance does not cancel). LANES is
 // a power of two and E the smaller one that holds the row, so a warp takes 8 rows of 64 or one of 384 or 512, and a block one
 // of up to 8192. Arithmetic is packed, two elements an instruction: at 107520 x 384 the kernels were bound by issuing 257
-// instructions a row forward and 391 backward. Both directions are bound by their bytes; thread blocks stay and walk over the rows, so that the weight
-// is loaded once and, backward, each thread keeps the fp32 sums of dw and db of its own columns. The next three rows are
+// instructions a row forward and 391 backward. Both directions are bound by their bytes now: 107520 x 384 bf16 forward 28 us
+// (5.9 TB/s), backward 46 us (5.4 TB/s). Thread blocks stay and walk over the rows, so that the weight is loaded once and,
+// backward, each thread keeps the fp32 sums of dw and db of its own columns. The next three rows are
 // under way meanwhile, copied asynchronously into shared memory that only the thread itself reads (so no barrier waits for
 // them): with one row ahead in registers 24 KB an SM were in flight, and the forward pass took 60 us where its bytes
 // take 25 (107520 x 384 bf16). The sums of the threads of a block meet in shared memory and those of the blocks in a

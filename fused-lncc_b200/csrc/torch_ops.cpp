@@ -9,6 +9,8 @@
 #include "lncc.h"
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -51,6 +53,14 @@ std::string shape_of(const Tensor& t) {
   return s + ")";
 }
 
+// Whether a call on x may go straight to the function below, as it does in eager mode: nothing (tracing, functional or
+// Python tensors, a dispatch mode) stands between it and the CUDA kernel. A call through the dispatcher costs a microsecond.
+bool straight(const Tensor& x) {
+  const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
+  const c10::DispatchKeySet keys = (x.key_set() | tls.included_) - tls.excluded_ - c10::autograd_dispatch_keyset_with_ADInplaceOrView -
+                                   c10::DispatchKeySet(c10::DispatchKey::BackendSelect);
+  return keys.highestPriorityTypeId() == c10::DispatchKey::CUDA;
+}
 // An operator as torch sees it, so that a compiled graph records the call.
 template <typename F> auto op_of(const char* name, F*) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -80,31 +90,43 @@ Tensor rows_of(const Tensor& t) {
 Tensor channels_last_axis(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 const void* ptr(const Tensor& t) { return t.numel() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
-Tensor bytes_of(size_t n, const Tensor& like) {
-  return at::empty({int64_t(n)}, like.options().dtype(at::kByte));
-}
+// A call's scratch, from torch's allocator and on the current stream like a tensor's memory.
+struct Scratch {
+  c10::DataPtr at;
+  explicit Scratch(size_t n) {
+    if (n) at = c10::cuda::CUDACachingAllocator::get()->allocate(n);
+  }
+  void* get() const { return at.get(); }
+};
+Tensor new_tensor(at::IntArrayRef sizes, const at::TensorOptions& options) { return at::detail::empty_cuda(sizes, options); }
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 Tensor or_undefined(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 optional<Tensor> or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
 // ---- layer norm -------------------------------------------------------------------------------------------------------
-std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
-                                              double eps, bool keep) {
+// y, and the statistics where they are wanted
+Tensor norm_rows(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias, double eps, float* mean, float* rstd) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t width = x.size(-1), rows = x.numel() / width;
-  Tensor y = at::empty(x.sizes(), x.options());
-  const auto f32 = x.options().dtype(at::kFloat);
-  Tensor mean = at::empty({keep ? rows : 0}, f32), rstd = at::empty({keep ? rows : 0}, f32);
+  Tensor y = new_tensor(x.sizes(), x.options());
   if (rows) {
     const Tensor xr = rows_of(x);
     const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
     const at::ScalarType wt = weight ? weight->scalar_type() : bias ? bias->scalar_type() : x.scalar_type();
     check_status(lncc_layer_norm_forward(ptr(xr), xr.stride(0), mut(w), mut(b), dtype_code(x.scalar_type()), dtype_code(wt),
-                                         rows, width, float(eps), mut(y), static_cast<float*>(mut(mean)),
-                                         static_cast<float*>(mut(rstd)), stream_of(x)),
+                                         rows, width, float(eps), mut(y), mean, rstd, stream_of(x)),
                  "layer_norm forward");
   }
+  return y;
+}
+std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& bias,
+                                              double eps, bool keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = keep ? x.numel() / x.size(-1) : 0;
+  const auto f32 = x.options().dtype(at::kFloat);
+  const Tensor mean = new_tensor({rows}, f32), rstd = new_tensor({rows}, f32);
+  const Tensor y = norm_rows(x, weight, bias, eps, static_cast<float*>(mut(mean)), static_cast<float*>(mut(rstd)));
   return {y, mean, rstd};
 }
 
@@ -113,16 +135,16 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy, const T
                                                        bool need_x, bool need_params) {
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t width = x.size(-1), rows = x.numel() / width;
-  Tensor dx = need_x ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  Tensor dx = need_x ? new_tensor(x.sizes(), x.options()) : new_tensor({0}, x.options());
   const auto params = x.options().dtype(wdtype);
-  Tensor dw = at::empty({need_params ? width : 0}, params), db = at::empty({need_params ? width : 0}, params), ws;
+  Tensor dw = new_tensor({need_params ? width : 0}, params), db = new_tensor({need_params ? width : 0}, params);
   const Tensor xr = rows ? rows_of(x) : x, dr = rows ? rows_of(dy) : dy, w = weight ? weight->contiguous() : Tensor();
   const size_t n = need_params ? lncc_layer_norm_scratch_bytes(rows, width) : 0;
-  if (n) ws = bytes_of(n, x);
+  const Scratch ws(n);
   check_status(lncc_layer_norm_backward(ptr(dr), rows ? dr.stride(0) : width, ptr(xr), rows ? xr.stride(0) : width, mut(w),
                                         dtype_code(x.scalar_type()), dtype_code(wdtype), rows, width,
                                         static_cast<const float*>(ptr(mean)), static_cast<const float*>(ptr(rstd)),
-                                        need_x ? mut(dx) : nullptr, mut(dw), mut(db), mut(ws), n, stream_of(x)),
+                                        need_x ? mut(dx) : nullptr, mut(dw), mut(db), ws.get(), n, stream_of(x)),
                "layer_norm backward");
   return {dx, dw, db};
 }
@@ -132,7 +154,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
                         double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = op_of("fused_lncc::layer_norm", layer_norm);
-    auto [y, mean, rstd] = op.call(x, weight, bias, eps, true);
+    auto [y, mean, rstd] = straight(x) ? layer_norm(x, weight, bias, eps, true) : op.call(x, weight, bias, eps, true);
     ctx->save_for_backward({x, or_undefined(weight), mean, rstd});
     const optional<Tensor>& p = weight ? weight : bias;
     ctx->saved_data["wdtype"] = int64_t(p ? p->scalar_type() : x.scalar_type());
@@ -148,8 +170,10 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
     const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1),
                need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [dx, dw, db] = op.call(grads[0], saved[0], or_none(saved[1]), saved[2], saved[3],
-                                at::ScalarType(ctx->saved_data["wdtype"].toInt()), need_x, need_w || need_b);
+    const auto wdtype = at::ScalarType(ctx->saved_data["wdtype"].toInt());
+    auto [dx, dw, db] = straight(grads[0]) && straight(saved[0])
+                            ? layer_norm_backward(grads[0], saved[0], or_none(saved[1]), saved[2], saved[3], wdtype, need_x, need_w || need_b)
+                            : op.call(grads[0], saved[0], or_none(saved[1]), saved[2], saved[3], wdtype, need_x, need_w || need_b);
     return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), need_b ? db : Tensor(), Tensor()};
   }
 };
@@ -175,6 +199,7 @@ Tensor fused_layer_norm(const Tensor& x, const optional<Tensor>& weight, const o
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return LayerNormNode::apply(x, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView below;
+  if (straight(x)) return norm_rows(x, weight, bias, eps, nullptr, nullptr);
   static const auto op = op_of("fused_lncc::layer_norm", layer_norm);
   return std::get<0>(op.call(x, weight, bias, eps, false));
 }
@@ -186,13 +211,13 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan(const Tensor& x_, const Tensor& ga
   const Tensor x = channels_last_axis(x_), gate = channels_last_axis(gate_), s = state ? state->contiguous() : Tensor();
   const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
   const auto f32 = x.options().dtype(at::kFloat);
-  Tensor h = at::empty({B, T, C}, x.options()), last = at::empty({B, C}, f32);
-  Tensor kept = at::empty({keep ? int64_t(lncc_gated_scan_kept_bytes(B, T, C) / 4) : 0}, f32);
+  Tensor h = new_tensor({B, T, C}, x.options()), last = new_tensor({B, C}, f32);
+  Tensor kept = new_tensor({keep ? int64_t(lncc_gated_scan_kept_bytes(B, T, C) / 4) : 0}, f32);
   const size_t n = lncc_gated_scan_scratch_bytes(B, T, C);
-  const Tensor ws = n ? bytes_of(n, x) : Tensor();
+  const Scratch ws(n);
   check_status(lncc_gated_scan_forward(ptr(x), x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
                                        static_cast<const float*>(mut(s)), dtype_code(x.scalar_type()), B, T, C, reverse,
-                                       mut(h), static_cast<float*>(mut(last)), static_cast<float*>(mut(kept)), mut(ws), n,
+                                       mut(h), static_cast<float*>(mut(last)), static_cast<float*>(mut(kept)), ws.get(), n,
                                        stream_of(x)),
                "gated_scan forward");
   return {h, last, kept};
@@ -206,14 +231,14 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_backward(const Tensor& dh_, const 
   const Tensor dl = dlast ? dlast->contiguous() : Tensor();
   const int64_t B = x.size(0), T = x.size(1), C = x.size(2);
   const auto f32 = x.options().dtype(at::kFloat);
-  Tensor dx = at::empty({B, T, C}, x.options()), dgate = at::empty({B, T, C}, x.options());
-  Tensor dstate = need_state ? at::empty({B, C}, f32) : at::empty({0}, f32);
+  Tensor dx = new_tensor({B, T, C}, x.options()), dgate = new_tensor({B, T, C}, x.options());
+  Tensor dstate = need_state ? new_tensor({B, C}, f32) : new_tensor({0}, f32);
   const size_t n = lncc_gated_scan_scratch_bytes(B, T, C);
-  const Tensor ws = n ? bytes_of(n, x) : Tensor();
+  const Scratch ws(n);
   check_status(lncc_gated_scan_backward(ptr(dh), dh.stride(0), dh.stride(1), static_cast<const float*>(mut(dl)), ptr(x),
                                         x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
                                         static_cast<const float*>(ptr(kept)), dtype_code(x.scalar_type()), B, T, C, reverse,
-                                        mut(dx), mut(dgate), static_cast<float*>(mut(dstate)), mut(ws), n, stream_of(x)),
+                                        mut(dx), mut(dgate), static_cast<float*>(mut(dstate)), ws.get(), n, stream_of(x)),
                "gated_scan backward");
   return {dx, dgate, dstate};
 }
@@ -223,7 +248,7 @@ struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
                                bool reverse) {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = op_of("fused_lncc::gated_scan", gated_scan);
-    auto [h, last, kept] = op.call(x, gate, state, reverse, true);
+    auto [h, last, kept] = straight(x) ? gated_scan(x, gate, state, reverse, true) : op.call(x, gate, state, reverse, true);
     ctx->save_for_backward({x, gate, kept});
     ctx->saved_data["reverse"] = reverse;
     ctx->saved_data["state"] = state.has_value();
@@ -237,8 +262,10 @@ struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor dh = grads[0].defined() ? grads[0] : at::zeros_like(saved[0], at::MemoryFormat::Contiguous);
     const bool need_state = ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2);  // edges of given tensors alone
-    auto [dx, dgate, dstate] = op.call(dh, or_none(grads[1]), saved[0], saved[1], saved[2],
-                                       ctx->saved_data["reverse"].toBool(), need_state);
+    const bool reverse = ctx->saved_data["reverse"].toBool();
+    auto [dx, dgate, dstate] = straight(dh) && straight(saved[0])
+                                   ? gated_scan_backward(dh, or_none(grads[1]), saved[0], saved[1], saved[2], reverse, need_state)
+                                   : op.call(dh, or_none(grads[1]), saved[0], saved[1], saved[2], reverse, need_state);
     return {ctx->needs_input_grad(0) ? dx : Tensor(), ctx->needs_input_grad(1) ? dgate : Tensor(),
             need_state ? dstate : Tensor(), Tensor()};
   }
@@ -263,7 +290,8 @@ std::tuple<Tensor, Tensor> fused_gated_scan(const Tensor& x, const Tensor& gate,
   }
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = op_of("fused_lncc::gated_scan", gated_scan);
-  auto [h, last, kept] = op.call(x, gate, or_none(state), reverse, false);
+  auto [h, last, kept] =
+      straight(x) ? gated_scan(x, gate, or_none(state), reverse, false) : op.call(x, gate, or_none(state), reverse, false);
   return {h, last};
 }
 
@@ -273,14 +301,14 @@ Tensor gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, cons
   const int64_t F = w_gate.size(0), K = w_gate.size(1), N = w_down.size(0), M = x.numel() / K;
   auto shape = x.sizes().vec();
   shape.back() = N;
-  Tensor y = at::empty(shape, x.options());
+  Tensor y = new_tensor(shape, x.options());
   if (!M) return y;
   const Tensor xr = rows_of(x), wg = w_gate.contiguous(), wu = w_up.contiguous(), wd = w_down.contiguous();
   const int dt = dtype_code(x.scalar_type());
   const size_t n = lncc_gated_ffn_scratch_bytes(M, K, F, N, dt, 0);
-  const Tensor ws = bytes_of(n, x);
+  const Scratch ws(n);
   check_status(lncc_gated_ffn_forward(ptr(xr), xr.stride(0), ptr(wg), ptr(wu), ptr(wd), dt, int(act), M, K, F, N, mut(y),
-                                      mut(ws), n, stream_of(x)),
+                                      ws.get(), n, stream_of(x)),
                "gated_ffn forward");
   return y;
 }
@@ -291,17 +319,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> gated_ffn_backward(const Tensor& dy, 
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t F = w_gate.size(0), K = w_gate.size(1), N = w_down.size(0), M = x.numel() / K;
   const auto out = [&](bool need, const Tensor& of) {
-    return need ? at::empty(of.sizes(), x.options()) : at::empty({0}, x.options());
+    return need ? new_tensor(of.sizes(), x.options()) : new_tensor({0}, x.options());
   };
-  Tensor dx = out(need_x, x), dwg = out(need_gate, w_gate), dwu = out(need_up, w_up), dwd = out(need_down, w_down), ws;
+  Tensor dx = out(need_x, x), dwg = out(need_gate, w_gate), dwu = out(need_up, w_up), dwd = out(need_down, w_down);
   const Tensor xr = M ? rows_of(x) : x, dr = M ? rows_of(dy) : dy;
   const Tensor wg = w_gate.contiguous(), wu = w_up.contiguous(), wd = w_down.contiguous();
   const int dt = dtype_code(x.scalar_type());
   const size_t n = M ? lncc_gated_ffn_scratch_bytes(M, K, F, N, dt, 1) : 0;
-  if (n) ws = bytes_of(n, x);
+  const Scratch ws(n);
   check_status(lncc_gated_ffn_backward(ptr(dr), M ? dr.stride(0) : N, ptr(xr), M ? xr.stride(0) : K, ptr(wg), ptr(wu), ptr(wd),
                                        dt, int(act), M, K, F, N, need_x ? mut(dx) : nullptr, need_gate ? mut(dwg) : nullptr,
-                                       need_up ? mut(dwu) : nullptr, need_down ? mut(dwd) : nullptr, mut(ws), n, stream_of(x)),
+                                       need_up ? mut(dwu) : nullptr, need_down ? mut(dwd) : nullptr, ws.get(), n, stream_of(x)),
                "gated_ffn backward");
   return {dx, dwg, dwu, dwd};
 }
@@ -313,7 +341,7 @@ struct GatedFFNNode : torch::autograd::Function<GatedFFNNode> {
     static const auto op = op_of("fused_lncc::gated_ffn", gated_ffn);
     ctx->save_for_backward({x, w_gate, w_up, w_down});
     ctx->saved_data["act"] = act;
-    return op.call(x, w_gate, w_up, w_down, act);
+    return straight(x) ? gated_ffn(x, w_gate, w_up, w_down, act) : op.call(x, w_gate, w_up, w_down, act);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = op_of("fused_lncc::gated_ffn_backward", gated_ffn_backward);
@@ -321,8 +349,11 @@ struct GatedFFNNode : torch::autograd::Function<GatedFFNNode> {
     bool need[4];
     for (int i = 0; i < 4; i++) need[i] = ctx->needs_input_grad(i);
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [dx, dwg, dwu, dwd] = op.call(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["act"].toInt(),
-                                       need[0], need[1], need[2], need[3]);
+    const int64_t act = ctx->saved_data["act"].toInt();
+    auto [dx, dwg, dwu, dwd] =
+        straight(grads[0]) && straight(saved[0])
+            ? gated_ffn_backward(grads[0], saved[0], saved[1], saved[2], saved[3], act, need[0], need[1], need[2], need[3])
+            : op.call(grads[0], saved[0], saved[1], saved[2], saved[3], act, need[0], need[1], need[2], need[3]);
     return {need[0] ? dx : Tensor(), need[1] ? dwg : Tensor(), need[2] ? dwu : Tensor(), need[3] ? dwd : Tensor(), Tensor()};
   }
 };
@@ -345,7 +376,7 @@ Tensor fused_gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up
     return GatedFFNNode::apply(x, w_gate, w_up, w_down, act);
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = op_of("fused_lncc::gated_ffn", gated_ffn);
-  return op.call(x, w_gate, w_up, w_down, act);
+  return straight(x) ? gated_ffn(x, w_gate, w_up, w_down, act) : op.call(x, w_gate, w_up, w_down, act);
 }
 
 }  // namespace
