@@ -124,10 +124,6 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 template <int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t dst) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(COLS) : "memory");
 }
-template <int COLS> __device__ __forceinline__ void tmem_free(uint32_t addr) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(COLS));
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
-}
 // 16 or 8 columns of the warp's 32 lanes; the values may be read after wait_ld() has named them.
 __device__ __forceinline__ void tmem_load(uint32_t addr, uint32_t (&v)[16]) {
   asm volatile(
