@@ -10,6 +10,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <ATen/record_function.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -53,13 +54,17 @@ std::string shape_of(const Tensor& t) {
   return s + ")";
 }
 
-// Whether a call on x may go straight to the function below, as it does in eager mode: nothing (tracing, functional or
-// Python tensors, a dispatch mode) stands between it and the CUDA kernel. A call through the dispatcher costs a microsecond.
-bool straight(const Tensor& x) {
+c10::DispatchKeySet keys_of(const Tensor& t) { return t.defined() ? t.key_set() : c10::DispatchKeySet(); }
+c10::DispatchKeySet keys_of(const optional<Tensor>& t) { return t ? keys_of(*t) : c10::DispatchKeySet(); }
+// Whether a call on these tensors, all that it takes, may go straight to the function below, as it does in eager mode: nothing
+// (tracing, functional, Python or negated tensors, a dispatch mode, a profiler) stands between it and the CUDA kernel. A call
+// through the dispatcher costs a microsecond.
+template <typename... Ts> bool straight(const Ts&... ts) {
   const c10::impl::LocalDispatchKeySet tls = c10::impl::tls_local_dispatch_key_set();
-  const c10::DispatchKeySet keys = (x.key_set() | tls.included_) - tls.excluded_ - c10::autograd_dispatch_keyset_with_ADInplaceOrView -
+  const c10::DispatchKeySet keys = ((keys_of(ts) | ...) | tls.included_) - tls.excluded_ -
+                                   c10::autograd_dispatch_keyset_with_ADInplaceOrView -
                                    c10::DispatchKeySet(c10::DispatchKey::BackendSelect);
-  return keys.highestPriorityTypeId() == c10::DispatchKey::CUDA;
+  return keys.highestPriorityTypeId() == c10::DispatchKey::CUDA && !at::hasCallbacks();
 }
 // An operator as torch sees it, so that a compiled graph records the call.
 template <typename F> auto op_of(const char* name, F*) {
@@ -88,7 +93,13 @@ Tensor rows_of(const Tensor& t) {
 }
 // channels contiguous, other strides as they are
 Tensor channels_last_axis(const Tensor& t) { return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
-const void* ptr(const Tensor& t) { return t.numel() ? t.const_data_ptr() : nullptr; }
+// The memory of t; null, which the entry points take as "not given", only where there is none to read or write.
+const void* ptr(const Tensor& t) {
+  if (!t.defined() || !t.numel()) return nullptr;
+  const void* const p = t.const_data_ptr();
+  TORCH_CHECK(p, "fused_lncc: a tensor without memory of its own (a subclass?) reached a kernel call");
+  return p;
+}
 void* mut(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 // A call's scratch, from torch's allocator and on the current stream like a tensor's memory.
 struct Scratch {
@@ -114,7 +125,7 @@ Tensor norm_rows(const Tensor& x, const optional<Tensor>& weight, const optional
     const Tensor xr = rows_of(x);
     const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
     const at::ScalarType wt = weight ? weight->scalar_type() : bias ? bias->scalar_type() : x.scalar_type();
-    check_status(lncc_layer_norm_forward(ptr(xr), xr.stride(0), mut(w), mut(b), dtype_code(x.scalar_type()), dtype_code(wt),
+    check_status(lncc_layer_norm_forward(ptr(xr), xr.stride(0), ptr(w), ptr(b), dtype_code(x.scalar_type()), dtype_code(wt),
                                          rows, width, float(eps), mut(y), mean, rstd, stream_of(x)),
                  "layer_norm forward");
   }
@@ -141,7 +152,7 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy, const T
   const Tensor xr = rows ? rows_of(x) : x, dr = rows ? rows_of(dy) : dy, w = weight ? weight->contiguous() : Tensor();
   const size_t n = need_params ? lncc_layer_norm_scratch_bytes(rows, width) : 0;
   const Scratch ws(n);
-  check_status(lncc_layer_norm_backward(ptr(dr), rows ? dr.stride(0) : width, ptr(xr), rows ? xr.stride(0) : width, mut(w),
+  check_status(lncc_layer_norm_backward(ptr(dr), rows ? dr.stride(0) : width, ptr(xr), rows ? xr.stride(0) : width, ptr(w),
                                         dtype_code(x.scalar_type()), dtype_code(wdtype), rows, width,
                                         static_cast<const float*>(ptr(mean)), static_cast<const float*>(ptr(rstd)),
                                         need_x ? mut(dx) : nullptr, mut(dw), mut(db), ws.get(), n, stream_of(x)),
@@ -154,7 +165,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
                         double eps) {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = op_of("fused_lncc::layer_norm", layer_norm);
-    auto [y, mean, rstd] = straight(x) ? layer_norm(x, weight, bias, eps, true) : op.call(x, weight, bias, eps, true);
+    auto [y, mean, rstd] = straight(x, weight, bias) ? layer_norm(x, weight, bias, eps, true) : op.call(x, weight, bias, eps, true);
     ctx->save_for_backward({x, or_undefined(weight), mean, rstd});
     const optional<Tensor>& p = weight ? weight : bias;
     ctx->saved_data["wdtype"] = int64_t(p ? p->scalar_type() : x.scalar_type());
@@ -171,7 +182,7 @@ struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
                need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
     at::AutoDispatchBelowADInplaceOrView below;
     const auto wdtype = at::ScalarType(ctx->saved_data["wdtype"].toInt());
-    auto [dx, dw, db] = straight(grads[0]) && straight(saved[0])
+    auto [dx, dw, db] = straight(grads[0], saved[0], saved[1], saved[2], saved[3])
                             ? layer_norm_backward(grads[0], saved[0], or_none(saved[1]), saved[2], saved[3], wdtype, need_x, need_w || need_b)
                             : op.call(grads[0], saved[0], or_none(saved[1]), saved[2], saved[3], wdtype, need_x, need_w || need_b);
     return {need_x ? dx : Tensor(), need_w ? dw : Tensor(), need_b ? db : Tensor(), Tensor()};
@@ -199,7 +210,7 @@ Tensor fused_layer_norm(const Tensor& x, const optional<Tensor>& weight, const o
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return LayerNormNode::apply(x, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView below;
-  if (straight(x)) return norm_rows(x, weight, bias, eps, nullptr, nullptr);
+  if (straight(x, weight, bias)) return norm_rows(x, weight, bias, eps, nullptr, nullptr);
   static const auto op = op_of("fused_lncc::layer_norm", layer_norm);
   return std::get<0>(op.call(x, weight, bias, eps, false));
 }
@@ -216,7 +227,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan(const Tensor& x_, const Tensor& ga
   const size_t n = lncc_gated_scan_scratch_bytes(B, T, C);
   const Scratch ws(n);
   check_status(lncc_gated_scan_forward(ptr(x), x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
-                                       static_cast<const float*>(mut(s)), dtype_code(x.scalar_type()), B, T, C, reverse,
+                                       static_cast<const float*>(ptr(s)), dtype_code(x.scalar_type()), B, T, C, reverse,
                                        mut(h), static_cast<float*>(mut(last)), static_cast<float*>(mut(kept)), ws.get(), n,
                                        stream_of(x)),
                "gated_scan forward");
@@ -235,7 +246,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_scan_backward(const Tensor& dh_, const 
   Tensor dstate = need_state ? new_tensor({B, C}, f32) : new_tensor({0}, f32);
   const size_t n = lncc_gated_scan_scratch_bytes(B, T, C);
   const Scratch ws(n);
-  check_status(lncc_gated_scan_backward(ptr(dh), dh.stride(0), dh.stride(1), static_cast<const float*>(mut(dl)), ptr(x),
+  check_status(lncc_gated_scan_backward(ptr(dh), dh.stride(0), dh.stride(1), static_cast<const float*>(ptr(dl)), ptr(x),
                                         x.stride(0), x.stride(1), ptr(gate), gate.stride(0), gate.stride(1),
                                         static_cast<const float*>(ptr(kept)), dtype_code(x.scalar_type()), B, T, C, reverse,
                                         mut(dx), mut(dgate), static_cast<float*>(mut(dstate)), ws.get(), n, stream_of(x)),
@@ -248,7 +259,7 @@ struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
                                bool reverse) {
     at::AutoDispatchBelowADInplaceOrView below;
     static const auto op = op_of("fused_lncc::gated_scan", gated_scan);
-    auto [h, last, kept] = straight(x) ? gated_scan(x, gate, state, reverse, true) : op.call(x, gate, state, reverse, true);
+    auto [h, last, kept] = straight(x, gate, state) ? gated_scan(x, gate, state, reverse, true) : op.call(x, gate, state, reverse, true);
     ctx->save_for_backward({x, gate, kept});
     ctx->saved_data["reverse"] = reverse;
     ctx->saved_data["state"] = state.has_value();
@@ -263,7 +274,7 @@ struct GatedScanNode : torch::autograd::Function<GatedScanNode> {
     const Tensor dh = grads[0].defined() ? grads[0] : at::zeros_like(saved[0], at::MemoryFormat::Contiguous);
     const bool need_state = ctx->saved_data["state"].toBool() && ctx->needs_input_grad(2);  // edges of given tensors alone
     const bool reverse = ctx->saved_data["reverse"].toBool();
-    auto [dx, dgate, dstate] = straight(dh) && straight(saved[0])
+    auto [dx, dgate, dstate] = straight(dh, grads[1], saved[0], saved[1], saved[2])
                                    ? gated_scan_backward(dh, or_none(grads[1]), saved[0], saved[1], saved[2], reverse, need_state)
                                    : op.call(dh, or_none(grads[1]), saved[0], saved[1], saved[2], reverse, need_state);
     return {ctx->needs_input_grad(0) ? dx : Tensor(), ctx->needs_input_grad(1) ? dgate : Tensor(),
@@ -291,7 +302,7 @@ std::tuple<Tensor, Tensor> fused_gated_scan(const Tensor& x, const Tensor& gate,
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = op_of("fused_lncc::gated_scan", gated_scan);
   auto [h, last, kept] =
-      straight(x) ? gated_scan(x, gate, or_none(state), reverse, false) : op.call(x, gate, or_none(state), reverse, false);
+      straight(x, gate, state) ? gated_scan(x, gate, or_none(state), reverse, false) : op.call(x, gate, or_none(state), reverse, false);
   return {h, last};
 }
 
@@ -341,7 +352,7 @@ struct GatedFFNNode : torch::autograd::Function<GatedFFNNode> {
     static const auto op = op_of("fused_lncc::gated_ffn", gated_ffn);
     ctx->save_for_backward({x, w_gate, w_up, w_down});
     ctx->saved_data["act"] = act;
-    return straight(x) ? gated_ffn(x, w_gate, w_up, w_down, act) : op.call(x, w_gate, w_up, w_down, act);
+    return straight(x, w_gate, w_up, w_down) ? gated_ffn(x, w_gate, w_up, w_down, act) : op.call(x, w_gate, w_up, w_down, act);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = op_of("fused_lncc::gated_ffn_backward", gated_ffn_backward);
@@ -351,7 +362,7 @@ struct GatedFFNNode : torch::autograd::Function<GatedFFNNode> {
     at::AutoDispatchBelowADInplaceOrView below;
     const int64_t act = ctx->saved_data["act"].toInt();
     auto [dx, dwg, dwu, dwd] =
-        straight(grads[0]) && straight(saved[0])
+        straight(grads[0], saved[0], saved[1], saved[2], saved[3])
             ? gated_ffn_backward(grads[0], saved[0], saved[1], saved[2], saved[3], act, need[0], need[1], need[2], need[3])
             : op.call(grads[0], saved[0], saved[1], saved[2], saved[3], act, need[0], need[1], need[2], need[3]);
     return {need[0] ? dx : Tensor(), need[1] ? dwg : Tensor(), need[2] ? dwu : Tensor(), need[3] ? dwd : Tensor(), Tensor()};
@@ -376,7 +387,7 @@ Tensor fused_gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up
     return GatedFFNNode::apply(x, w_gate, w_up, w_down, act);
   at::AutoDispatchBelowADInplaceOrView below;
   static const auto op = op_of("fused_lncc::gated_ffn", gated_ffn);
-  return straight(x) ? gated_ffn(x, w_gate, w_up, w_down, act) : op.call(x, w_gate, w_up, w_down, act);
+  return straight(x, w_gate, w_up, w_down) ? gated_ffn(x, w_gate, w_up, w_down, act) : op.call(x, w_gate, w_up, w_down, act);
 }
 
 }  // namespace

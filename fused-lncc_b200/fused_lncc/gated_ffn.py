@@ -8,6 +8,7 @@ x: (..., K); w_gate, w_up: (F, K); w_down: (N, F), as torch.nn.Linear lays its w
 bfloat16 or float16. Sums are fp32. Nothing of the hidden layer is saved for the backward pass: it forms g, u and h again.
 """
 import torch
+from torch.overrides import has_torch_function
 
 from . import _native
 
@@ -24,6 +25,6 @@ def fused_gated_ffn(x, w_gate, w_up, w_down, activation="silu"):
     if act is None:
         raise ValueError(f"fused_lncc: gated_ffn: activation must be 'silu', 'gelu' or 'relu', got {activation!r}")
     module = _native.load()
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or has_torch_function((x, w_gate, w_up, w_down)):
         return torch.ops.fused_lncc.fused_gated_ffn(x, w_gate, w_up, w_down, act)
     return module.gated_ffn(x, w_gate, w_up, w_down, act)

@@ -10,6 +10,7 @@ throughout; h is rounded to x's type as it is written, and no rounded value is c
 again from fp32 states that the forward pass kept, so nothing of h is saved.
 """
 import torch
+from torch.overrides import has_torch_function
 
 from . import _native
 
@@ -23,6 +24,6 @@ def fused_gated_scan(x, gate, state=None, reverse=False):
     A gate of +inf keeps the state and ignores x_t, one of -inf forgets the state (x_t and the state have to be finite
     all the same: the formula multiplies them by zero). RuntimeError for wrong shapes, types or devices."""
     module = _native.load()
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or has_torch_function((x, gate, state)):
         return torch.ops.fused_lncc.fused_gated_scan(x, gate, state, reverse)
     return module.gated_scan(x, gate, state, reverse)

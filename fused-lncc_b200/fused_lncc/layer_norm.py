@@ -7,6 +7,7 @@ gradients the types of what they belong to. Statistics and sums are fp32; the we
 summed in a fixed order, so they are the same bits run after run. Strided rows are read where they lie.
 """
 import torch
+from torch.overrides import has_torch_function
 
 from . import _native
 
@@ -18,6 +19,6 @@ def fused_layer_norm(x, weight=None, bias=None, eps=1e-5):
     RuntimeError for tensors that are not on one CUDA device, of another type or of the wrong shape. A row with a NaN or
     an infinity gives NaN in that row (and in the weight's gradient), as the formula does."""
     module = _native.load()
-    if torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or has_torch_function((x, weight, bias)):
         return torch.ops.fused_lncc.fused_layer_norm(x, weight, bias, eps)
     return module.layer_norm(x, weight, bias, eps)
