@@ -11,6 +11,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/record_function.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -111,6 +112,13 @@ struct Scratch {
 };
 Tensor new_tensor(at::IntArrayRef sizes, const at::TensorOptions& options) { return at::detail::empty_cuda(sizes, options); }
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+// The operators have no forward-mode derivative. Below the autograd keys a tangent would be lost, and torch takes a missing one
+// for zero.
+template <typename... Ts> void refuse_tangents(const char* what, const Ts&... ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  TORCH_CHECK_NOT_IMPLEMENTED(!((ts.defined() && ts._fw_grad(0).defined()) || ...), "fused_lncc: ", what,
+                              ": forward-mode derivatives are not implemented");
+}
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 Tensor or_undefined(const optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
 optional<Tensor> or_none(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
@@ -207,6 +215,7 @@ Tensor fused_layer_norm(const Tensor& x, const optional<Tensor>& weight, const o
   }
   TORCH_CHECK(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(),
               "fused_lncc: layer_norm: weight and bias must have one type");
+  refuse_tangents(what, x, w, b);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b)))
     return LayerNormNode::apply(x, weight, bias, eps);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -295,6 +304,7 @@ std::tuple<Tensor, Tensor> fused_gated_scan(const Tensor& x, const Tensor& gate,
                 "fused_lncc: gated_scan: state must be (B, C), got ", shape_of(state), " for x ", shape_of(x));
     state = state.to(at::kFloat);
   }
+  refuse_tangents(what, x, gate, state);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(gate) || wants_grad(state))) {
     const variable_list r = GatedScanNode::apply(x, gate, or_none(state), reverse);
     return {r[0], r[1]};
@@ -383,6 +393,7 @@ Tensor fused_gated_ffn(const Tensor& x, const Tensor& w_gate, const Tensor& w_up
                   w_down.sym_size(1) == w_gate.sym_size(0),
               "fused_lncc: gated_ffn: expect x (..., K), w_gate and w_up (F, K), w_down (N, F), got ", shape_of(x), ", ",
               shape_of(w_gate), ", ", shape_of(w_up), ", ", shape_of(w_down));
+  refuse_tangents(what, x, w_gate, w_up, w_down);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w_gate) || wants_grad(w_up) || wants_grad(w_down)))
     return GatedFFNNode::apply(x, w_gate, w_up, w_down, act);
   at::AutoDispatchBelowADInplaceOrView below;
