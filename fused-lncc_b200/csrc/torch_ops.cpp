@@ -76,6 +76,7 @@ template <typename F> auto op_of(const char* name, F*) {
 Tensor rows_of(const Tensor& t) {
   const int64_t c = t.size(-1);
   if (t.is_contiguous()) return t.dim() == 2 ? t : t.view({-1, c});
+  if (t.dim() == 1) return t.contiguous().view({1, c});
   Tensor r = t;
   if (t.dim() != 2) {
     // leading axes that follow one another collapse into one
