@@ -594,18 +594,32 @@ template <typename T, typename TO> __global__ void __launch_bounds__(256) pack_k
   }
 }
 
-// Euclidean norms of the rows of x and then of Wg, a warp a row.
+// Euclidean norms of the rows of x and then of Wg, a warp a row: 0 for a row of zeros alone, NaN for one that holds a NaN. Where
+// the squares leave the range of fp32 the row is taken relative to its largest element.
 __global__ void __launch_bounds__(256) norms_kernel(const float* __restrict__ x, int64_t x_stride, const float* __restrict__ w,
                                                     float* norms, int64_t M, int64_t F, int64_t K) {
   begin_after_previous();
   const int64_t row = int64_t(blockIdx.x) * 8 + threadIdx.x / 32;
   if (row >= M + F) return;
   const float* p = row < M ? x + row * x_stride : w + (row - M) * K;
-  float s = 0.f;
-  for (int64_t k = threadIdx.x % 32; k < K; k += 32) s = fmaf(p[k], p[k], s);
+  const int lane = threadIdx.x % 32;
+  const auto squares = [&](float scale) {  // the same number in every lane
+    float s = 0.f;
+    for (int64_t k = lane; k < K; k += 32) s = fmaf(p[k] * scale, p[k] * scale, s);
 #pragma unroll
-  for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (threadIdx.x % 32 == 0 && LNCC_IN(row, 1, M + F)) norms[row] = sqrtf(s);
+    for (int o = 16; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+  };
+  float s = squares(1.f), norm = sqrtf(s);
+  if (s < 1e-30f || s > 1e30f) {
+    float most = 0.f;
+    for (int64_t k = lane; k < K; k += 32) most = fmaxf(most, fabsf(p[k]));
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int e = most > 0.f && most <= 3.4028235e38f ? max(-126, min(126, -ilogbf(most))) : 0;
+    norm = ldexpf(sqrtf(squares(ldexpf(1.f, e))), -e);
+  }
+  if (lane == 0 && LNCC_IN(row, 1, M + F)) norms[row] = norm;
 }
 struct NearZero {  // what a gate of ReLU is formed again from
   const float *x, *w, *norms;
@@ -635,8 +649,9 @@ __device__ __noinline__ float gate_in_order(const NearZero& z, int64_t row, int6
 // ReLU's derivative jumps at g = 0, where the last bits of g decide and one element that falls the other way is off by all of
 // its gradient. The plain fp32 sum in the order of k is within K 2^-24 |x| |w| of the exact one, and the sum of the tensor
 // cores within (64 + K/256) 2^-24 |x| |w|: 16 cut additions in each accumulator, the parts left out, one rounding for each
-// 256 of K. Where g is closer to 0 than both together, it is formed again as the plain sum (about one gate in 2700 at
-// K = 389; forming all of them so took 100 us of 413 at 4093 x 389 x 1037).
+// 256 of K. Where g is closer to 0 than both together, it is formed again as the plain sum (about one gate in 2700 of dense
+// normal rows at K = 389; forming all of them so took 100 us of 413 at 4093 x 389 x 1037). Rows of zeros (padded tokens) and of
+// NaN are left out: every order of summation gives 0 and NaN there (half the tokens of 4096 x 1024 x 2048 zero: 21 ms with them).
 template <int ACT>
 __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g, const float* __restrict__ u,
                                                     const float* __restrict__ dh, __nv_bfloat16* dg, __nv_bfloat16* du,
@@ -659,10 +674,11 @@ __global__ void __launch_bounds__(256) parts_kernel(const float* __restrict__ g,
     }
     if (ACT == LNCC_ACT_RELU) {
       const int64_t row = i / z.ld, col = i - row * z.ld;
-      const float near = here ? z.norms[row] * (float(z.K + 64 + z.K / 256) * 5.9604645e-8f) : 0.f;
+      const float norm = here ? z.norms[row] : 0.f, near = norm * (float(z.K + 64 + z.K / 256) * 5.9604645e-8f);
 #pragma unroll
       for (int k = 0; k < 8; k++) {
-        const bool again = here && col + k < z.F && !(fabsf(vg[k]) > near * z.norms[z.M + col + k]);
+        const float norm_w = here && col + k < z.F ? z.norms[z.M + col + k] : 0.f, bound = near * norm_w;
+        const bool again = norm != 0.f && norm_w != 0.f && bound == bound && !(fabsf(vg[k]) > bound);
         for (unsigned rest = __ballot_sync(0xffffffffu, again); rest; rest &= rest - 1) {
           const int who = __ffs(rest) - 1;
           const float v = gate_in_order(z, __shfl_sync(0xffffffffu, row, who), __shfl_sync(0xffffffffu, col, who) + k, stages[threadIdx.x / 32]);
