@@ -102,11 +102,26 @@ def build_library(force=False, checked=False, verbose=False, out=None):
     return out
 
 
+def torch_mark():
+    """The last bytes of libfused_lncc_torch.so: that it is whole, and the torch that it was compiled against, whose C++
+    interface changes from version to version. fused_lncc/_native.py looks for them."""
+    import torch
+    return f"fused_lncc token blocks for torch {torch.__version__}, cxx11 abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}".encode()
+
+
+def _ends_with(path, mark):
+    if not os.path.exists(path) or os.path.getsize(path) < len(mark):
+        return False
+    with open(path, "rb") as f:
+        f.seek(-len(mark), os.SEEK_END)
+        return f.read() == mark
+
+
 def build_torch_ops(force=False, verbose=False):
     """Compile csrc/torch_ops.cpp against the torch that is installed and the library beside it; return its path."""
     out, src = TORCH_OPS_PATH, os.path.join(CSRC, "torch_ops.cpp")
     lib = build_library(verbose=verbose)
-    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(map(os.path.getmtime, _includes(src))):
+    if not force and _ends_with(out, torch_mark()) and os.path.getmtime(out) >= max(map(os.path.getmtime, _includes(src))):
         return out
     import torch
     torch_dir = os.path.dirname(torch.__file__)
@@ -121,6 +136,8 @@ def build_torch_ops(force=False, verbose=False):
            "-o", out + ".tmp", src, f"-L{LIB_DIR}", f"-l:{os.path.basename(lib)}", f"-L{os.path.join(torch_dir, 'lib')}",
            "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     _run(cmd, out, verbose)
+    with open(out + ".tmp", "ab") as f:
+        f.write(torch_mark())
     os.replace(out + ".tmp", out)
     return out
 

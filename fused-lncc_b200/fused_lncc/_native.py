@@ -1,5 +1,6 @@
 """Loads libfused_lncc_torch.so, which gives torch the token-block operators (csrc/torch_ops.cpp), and tells torch.compile
-their shapes. Like the C library it is built in-tree once where it is missing, and there is no fallback."""
+their shapes. Like the C library it is built in-tree once where it is missing, or was built against another torch, and there
+is no fallback. The loss needs none of it: a library that does not load is an error of the token-block functions alone."""
 import importlib.machinery
 import importlib.util
 import os
@@ -14,6 +15,21 @@ KEEP = 16  # steps of the gated scan from one kept state to the next (lncc_gated
 
 _lock = threading.Lock()
 _module = None
+
+
+def _mark():
+    """The last bytes of a library that is whole and was built against the torch that is installed (build.py: torch_mark)."""
+    return f"fused_lncc token blocks for torch {torch.__version__}, cxx11 abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}".encode()
+
+
+def _matches():
+    mark = _mark()
+    try:
+        with open(OPS_PATH, "rb") as f:
+            f.seek(-len(mark), os.SEEK_END)
+            return f.read() == mark
+    except OSError:
+        return False
 
 
 def _build():
@@ -35,12 +51,16 @@ def load():
     if _module is None:
         with _lock:
             if _module is None:
-                if not os.path.exists(OPS_PATH):
+                if not _matches():
                     _build()
                 _lib.load()
-                loader = importlib.machinery.ExtensionFileLoader("libfused_lncc_torch", OPS_PATH)
-                module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
-                loader.exec_module(module)
+                try:
+                    loader = importlib.machinery.ExtensionFileLoader("libfused_lncc_torch", OPS_PATH)
+                    module = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+                    loader.exec_module(module)
+                except ImportError as e:
+                    raise RuntimeError(f"fused_lncc: {OPS_PATH} does not load ({e}); build it again with "
+                                       "build.py --force") from e
                 _register_fakes()
                 _module = module
     return _module
@@ -81,5 +101,8 @@ def _register_fakes():
                      for need, t in ((need_x, x), (need_gate, w_gate), (need_up, w_up), (need_down, w_down)))
 
 
-if os.path.exists(OPS_PATH):
-    load()
+if _matches():
+    try:
+        load()
+    except (RuntimeError, OSError, AttributeError):  # the first call of a token-block function raises it
+        pass
