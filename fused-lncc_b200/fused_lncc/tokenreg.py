@@ -34,8 +34,9 @@ class TokenBlock(nn.Module):
         self.norm1, self.norm2 = nn.LayerNorm(width), nn.LayerNorm(width)  # parameters alone; the kernels read them
         self.mix_in = nn.Linear(width, 2 * width)
         self.mix_out = nn.Linear(width, width)
-        with torch.no_grad():  # gates that remember from a few tokens to some hundreds
-            self.mix_in.bias[width:] = torch.linspace(1.0, 6.0, width)
+        with torch.no_grad():  # in either direction gates that remember from a few tokens to some hundreds
+            for part in self.mix_in.bias[width:].split([width // 2, width - width // 2]):
+                part.copy_(torch.linspace(1.0, 6.0, len(part)))
         self.w_gate = nn.Parameter(torch.randn(hidden, width) * width ** -0.5)
         self.w_up = nn.Parameter(torch.randn(hidden, width) * width ** -0.5)
         self.w_down = nn.Parameter(torch.randn(width, hidden) * hidden ** -0.5 * 0.5)
