@@ -186,10 +186,17 @@ inline bool make_map(CUtensorMap* map, const Matrix& m, int box_rows, int box_co
   const cuuint64_t dims[3] = {cuuint64_t(m.cols), cuuint64_t(m.rows), cuuint64_t(m.planes)};
   const cuuint64_t strides[2] = {cuuint64_t(m.ld) * 2, m.planes > 1 ? cuuint64_t(m.plane) * 2 : cuuint64_t(m.ld) * 2};
   const cuuint32_t box[3] = {cuuint32_t(box_cols), cuuint32_t(box_rows), 1}, steps[3] = {1, 1, 1};
-  return encode(map, m.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, m.p, dims, strides, box,
-                steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const auto encoded = [&] {
+    return encode(map, m.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, m.p, dims, strides, box,
+                  steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encoded()) return true;
+  // The driver encodes for the thread's context, and a thread that has not yet used the device through the runtime (a new
+  // thread, or autograd's, whose memory came from a cache) has none.
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encoded();
 }
 
 }  // namespace tc
