@@ -28,9 +28,11 @@
 // keeps h in fp32 (fp16, more than four tokens: 2.9e-4 of the result against 2.1e-4; bf16 2.4e-3 against 1.7e-3); in calls of
 // a few hundred values the factor scatters, at 5 x 48 x 79 between 1.25 and 1.63 in nine draws of ten. fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
 // the nine products are summed, smallest first (the other three are below 2^-24 of the result). The tensor cores cut, not
-// round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of the result. So for fp32 an
-// accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each time. An
-// infinity taken apart meets zeros: it gives NaN where fp32 would give an infinity.
+// round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of an fp32 result. So for fp32 an
+// accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each time. The 16-bit
+// products with long inner axes do so every 2048: sums over 131072 tokens that do not cancel came out 8.5e-4 too small
+// in one accumulator, more than fp16's own rounding, and 2.4e-5 now, at the same speed. (g, u and dh, whose inner axes are the
+// block's widths, take one accumulator for 16-bit types: 8e-6 at 1024.) An infinity taken apart meets zeros: it gives NaN where fp32 would give an infinity.
 #include "lncc_tc.cuh"
 
 #include <type_traits>
@@ -48,7 +50,7 @@ enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
 constexpr int kEpilogueWarps = 16;         // of a CTA: four for each quarter of the lanes of tensor memory
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0 TMA, 1 products, 4 - 19 epilogue
 constexpr int kATile = 128 * 64 * 2;       // bytes of a CTA's share of A in a stage
-constexpr int kChunk = 4;                  // blocks of 64 that an accumulator of fp32 takes
+constexpr int kChunk = 4, kChunk16 = 32;   // blocks of 64 that an accumulator takes: fp32, and 16-bit types where sums are long
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == DW_UP || kind == DW_DOWN; }
 __host__ __device__ constexpr bool b_mn(int kind) { return kind == DH || kind == DX || kind == DW_UP || kind == DW_DOWN; }
@@ -223,7 +225,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   constexpr int ACCS = ONE ? 1 : 2;
   constexpr int DH_BYTES = BN == 256 ? 8192 : 4096;    // a CTA's share of Wd in a stage: 64 or 32 columns
   constexpr int PARTS = F32 ? 6 : 1;                   // products of parts of the operands
-  constexpr int CHUNK = F32 ? kChunk : 1 << 30;        // blocks that one accumulator takes
+  constexpr bool PROMOTED = F32 || !gated(KIND);       // accumulators take a chunk each, and are added up in registers
+  constexpr int CHUNK = F32 ? kChunk : PROMOTED ? kChunk16 : 1 << 30;
   static_assert(KIND != HIDDEN || !F32, "fp32 has GATES and DH");
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
@@ -279,7 +282,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       const int m0 = w.m * 256 + int(rank) * 128;
       const CUtensorMap* a_first = KIND == DW_UP && w.which ? &g.a1 : &g.a0;
       for (int c = w.from; c < w.to && ok; c += CHUNK) {
-        const int c_end = F32 ? min(c + CHUNK, w.to) : w.to;
+        const int c_end = PROMOTED ? min(c + CHUNK, w.to) : w.to;
         for (int part = 0; part < PARTS && ok; part++) {
           const int pa = F32 ? kPlaneA[part] : 0, pb = F32 ? kPlaneB[part] : 0;
           for (int b = c; b < c_end; b++) {
@@ -328,7 +331,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     for (int t = blockIdx.x / 2; t < tiles && ok; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
       for (int c = w.from; c < w.to && ok; c += CHUNK, turn++) {
-        const int steps = (F32 ? min(CHUNK, w.to - c) : w.to - c) * PARTS;
+        const int steps = (PROMOTED ? min(CHUNK, w.to - c) : w.to - c) * PARTS;
         const int acc = ACCS == 2 ? turn & 1 : 0;
         const uint32_t acc_phase = ACCS == 2 ? (turn >> 1) & 1 : turn & 1;
         const uint32_t d = tmem + (ACCS == 2 ? acc * 256 : 0), d_dh = ONE ? tmem + BN + (turn & 1) * HALF : d + BN;
@@ -374,19 +377,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(peer_addr(acc_empty + 8 * acc, 0));
       };
-      // where an ordinary result of this tile goes: its type, or partial sums in fp32
+      // where an ordinary 16-bit result of this tile goes: its type, or partial sums in fp32
       const auto put = [&](int64_t col, const float (&v)[16]) {
-        if (g.splits > 1 || sizeof(T) == 4) {
+        if (g.splits > 1) {
           const int64_t ld = (g.cols + 3) / 4 * 4;
-          float* to = g.splits > 1 ? g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld
-                                   : static_cast<float*>(w.which ? g.out1 : g.out0);
+          float* to = g.partial + (int64_t(w.split) * g.whichs + w.which) * g.rows * ld;
           uint32_t o[8];
 #pragma unroll
           for (int i = 0; i < 16; i += 8) {
 #pragma unroll
             for (int j = 0; j < 8; j++) o[j] = __float_as_uint(v[i + j]);
-            emit<float, 8>(to, g.splits > 1 ? ld : g.ld, row0, col + i, g.rows, g.splits > 1 ? ld : g.cols,
-                           g.splits > 1 ? 16 : g.align, o, stage);
+            emit<float, 8>(to, ld, row0, col + i, g.rows, ld, 16, o, stage);
           }
         } else if constexpr (sizeof(T) == 2) {
           uint32_t o[8];
@@ -396,7 +397,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         }
       };
 
-      if constexpr (F32) {
+      if constexpr (PROMOTED) {
         constexpr int SUMS = gated(KIND) ? 2 * COLS : COLS;  // gated: columns of g, then of u
         float sum[SUMS];
 #pragma unroll
@@ -433,6 +434,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             }
             emit_parts(g.out0, g, row0, col0 + c, h, stage);
           }
+        } else if constexpr (!F32) {
+#pragma unroll
+          for (int c = 0; c < SUMS; c += 16) put(col0 + c, reinterpret_cast<const float(&)[16]>(sum[c]));
         } else {
 #pragma unroll
           for (int c = 0; c < SUMS; c += 8) {
@@ -457,7 +461,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
         for (int c = 0; c < COLS; c += 16) {
           __syncwarp();
           const int64_t col = col0 + c;
-          if constexpr (gated(KIND)) {
+          {
             uint32_t h[8], dg[8], du[8];
 #pragma unroll
             for (int half = 0; half < 2; half++) {  // eight columns at a time: 640 threads leave 102 registers each
@@ -494,16 +498,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
               emit<T, 8>(static_cast<T*>(g.out1), g.ld, row0, col, g.rows, g.cols, g.align, du, stage);
             }
             emit<T, 8>(static_cast<T*>(KIND == HIDDEN ? g.out2 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, h, stage);
-          } else {
-            uint32_t v[16];
-            if (ok) {
-              tmem_load(d + c, v);
-              wait_ld(v);
-            } else {
-              for (int i = 0; i < 16; i++) v[i] = kNaN;
-            }
-            if (c + 16 == COLS) done(acc);
-            if (rows_here) put(col, reinterpret_cast<const float(&)[16]>(v));
           }
         }
         turn++;
