@@ -23,10 +23,19 @@
 // Nothing of the hidden layer is kept between forward and backward. Forming g and u again costs 4 of 22 M F K products of a
 // training step, and saves writing and reading 4 M F bytes and a rounding of g and u.
 //
-// Roundings. For 16-bit types h, dg and du are rounded to the type, since they are operands of the next product; g, u and dh
-// never leave fp32. The result then holds two roundings of like size, its own and h's, and is sqrt 2 as far off as one that
-// keeps h in fp32 (fp16, more than four tokens: 2.9e-4 of the result against 2.1e-4; bf16 2.4e-3 against 1.7e-3); in calls of
-// a few hundred values the factor scatters, at 5 x 48 x 79 between 1.25 and 1.63 in nine draws of ten. fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
+// Roundings. g, u and dh never leave fp32; h, dg and du are operands of the next product. For bf16 they are rounded to the type.
+// The result then holds two roundings of like size, its own and h's, and is sqrt 2 as far off as one that
+// keeps h in fp32 (more than four tokens: 2.4e-3 of the result against 1.7e-3); in calls of
+// a few hundred values the factor scatters, at 5 x 48 x 79 between 1.25 and 1.63 in nine draws of ten.
+// fp16 would not do for them: its range is 2^-24 to 2^16, and hidden values of a block with small results pass 65504, and the
+// gradients of a mean over many tokens lie among its subnormal numbers (dWg was off by 4e-2 at dy = 1e-6). So with fp16 the
+// hidden matrices are held as two bf16 numbers each, 16 bits in fp32's range, and so is what they are multiplied with (fp16's 11
+// bits, exactly); three of the four products are summed, smallest first (the fourth is below 2^-18). UP and HIDDEN read fp16 as
+// it is. The result has its own rounding alone (2.1e-4, where an fp16 h gave 2.9e-4), and the products after the activation take
+// three times as long: 4096 x 768 x 2048 forward 69 us (44 in bf16), 107520 x 96 x 256 training 349 (196), 16384 x 1024 x 4096 2575
+// (1152). Rows of fp16 numbers times a power of 2 each, from a bound of the row, would run at bf16's speed, but lose what
+// lies 2^-29 below the bound, which is some 2^16 above a dense row's values and more where a few weights stand out.
+// fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
 // the nine products are summed, smallest first (the other three are below 2^-24 of the result). The tensor cores cut, not
 // round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of an fp32 result. So for fp32 an
 // accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each time. The 16-bit
@@ -50,16 +59,20 @@ enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
 constexpr int kEpilogueWarps = 16;         // of a CTA: four for each quarter of the lanes of tensor memory
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0 TMA, 1 products, 4 - 19 epilogue
 constexpr int kATile = 128 * 64 * 2;       // bytes of a CTA's share of A in a stage
-constexpr int kChunk = 4, kChunk16 = 32;   // blocks of 64 that an accumulator takes: fp32, and 16-bit types where sums are long
+// Blocks of 64 that an accumulator takes. Operands that are taken apart are read once for each product: 4 or 8 blocks of them
+// stay in L2 meanwhile.
+constexpr int kChunk = 4, kChunkHalf = 8, kChunkBf16 = 32;
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == DW_UP || kind == DW_DOWN; }
 __host__ __device__ constexpr bool b_mn(int kind) { return kind == DH || kind == DX || kind == DW_UP || kind == DW_DOWN; }
 __host__ __device__ constexpr bool gated(int kind) { return kind == UP || kind == GATES || kind == HIDDEN; }
+// products of parts of the operands
+__host__ __device__ constexpr int parts_of(int kind, int dtype) { return dtype == LNCC_F32 ? 6 : dtype == LNCC_F16 && !gated(kind) ? 3 : 1; }
 __host__ __device__ constexpr int b_tile(int bn) { return bn / 2 * 64 * 2; }  // a CTA's share of B
 __host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 6 : 8; }
 __host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256 + kEpilogueWarps * 32 * 9 * 4; }
 
-// Planes of the six products of operands that are taken apart, smallest first.
+// Planes of the six products of operands that are taken apart into three, smallest first; the last three are those of two.
 __device__ __constant__ const int8_t kPlaneA[6] = {2, 1, 0, 1, 0, 0}, kPlaneB[6] = {0, 1, 2, 0, 1, 0};
 
 struct Gemm {
@@ -169,6 +182,22 @@ __device__ __forceinline__ void take_apart(float v, __nv_bfloat16& hi, __nv_bflo
   mid = __float2bfloat16_rn(fine ? r : 0.f);
   lo = __float2bfloat16_rn(fine ? r - __bfloat162float(mid) : 0.f);
 }
+// Two neighbours of a hidden matrix as operands of the next product: rounded to bf16, or, for fp16, as the sum of two bf16
+// numbers that hold 16 bits (infinities become NaN).
+template <typename T> struct Words {  // of 16 columns of a row
+  uint32_t hi[8], lo[std::is_same<T, __half>::value ? 8 : 1];
+  __device__ __forceinline__ void put(int i, float a, float b) {
+    hi[i] = pack2<__nv_bfloat16>(a, b);
+    if constexpr (std::is_same<T, __half>::value)
+      lo[i] = pack2<__nv_bfloat16>(a - __uint_as_float(hi[i] << 16), b - __uint_as_float(hi[i] & 0xffff0000u));
+  }
+  __device__ __forceinline__ void emit_to(void* base, const Gemm& g, int64_t row0, int64_t col, uint32_t* stage) const {
+    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(base);
+    emit<__nv_bfloat16, 8>(to, g.ld, row0, col, g.rows, g.cols, g.align, hi, stage);
+    if constexpr (std::is_same<T, __half>::value)
+      emit<__nv_bfloat16, 8>(to + g.plane, g.ld, row0, col, g.rows, g.cols, g.align, lo, stage);
+  }
+};
 // Eight results of a row in fp32, as the three bf16 matrices that hold them.
 __device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t row0, int64_t col, const float (&v)[8],
                                            uint32_t* stage) {
@@ -224,9 +253,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   constexpr bool ONE = KIND == HIDDEN && BN == 256;
   constexpr int ACCS = ONE ? 1 : 2;
   constexpr int DH_BYTES = BN == 256 ? 8192 : 4096;    // a CTA's share of Wd in a stage: 64 or 32 columns
-  constexpr int PARTS = F32 ? 6 : 1;                   // products of parts of the operands
+  constexpr bool HALF_T = std::is_same<T, __half>::value;
+  constexpr int PARTS = parts_of(KIND, F32 ? LNCC_F32 : HALF_T ? LNCC_F16 : LNCC_BF16);
   constexpr bool PROMOTED = F32 || !gated(KIND);       // accumulators take a chunk each, and are added up in registers
-  constexpr int CHUNK = F32 ? kChunk : PROMOTED ? kChunk16 : 1 << 30;
+  constexpr int CHUNK = F32 ? kChunk : !PROMOTED ? 1 << 30 : HALF_T ? kChunkHalf : kChunkBf16;
   static_assert(KIND != HIDDEN || !F32, "fp32 has GATES and DH");
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
@@ -284,7 +314,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       for (int c = w.from; c < w.to && ok; c += CHUNK) {
         const int c_end = PROMOTED ? min(c + CHUNK, w.to) : w.to;
         for (int part = 0; part < PARTS && ok; part++) {
-          const int pa = F32 ? kPlaneA[part] : 0, pb = F32 ? kPlaneB[part] : 0;
+          const int pa = PARTS > 1 ? kPlaneA[6 - PARTS + part] : 0, pb = PARTS > 1 ? kPlaneB[6 - PARTS + part] : 0;
           for (int b = c; b < c_end; b++) {
             if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up))) break;
             const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile, bar = full_of_pair + 8 * stage;
@@ -462,7 +492,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           __syncwarp();
           const int64_t col = col0 + c;
           {
-            uint32_t h[8], dg[8], du[8];
+            Words<T> h, dg, du;
 #pragma unroll
             for (int half = 0; half < 2; half++) {  // eight columns at a time: 640 threads leave 102 registers each
               uint32_t v[3][8];
@@ -483,21 +513,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
 #pragma unroll
                 for (int j = 0; j < 2; j++) activate<ACT, true>(__uint_as_float(v[0][i + j]), a[j], da[j]);
                 const float u0 = __uint_as_float(v[1][i]), u1 = __uint_as_float(v[1][i + 1]);
-                h[half * 4 + i / 2] = pack2<T>(a[0] * u0, a[1] * u1);
+                h.put(half * 4 + i / 2, a[0] * u0, a[1] * u1);
                 if (KIND == HIDDEN) {
                   const float d0 = __uint_as_float(v[2][i]), d1 = __uint_as_float(v[2][i + 1]);
-                  dg[half * 4 + i / 2] = pack2<T>(d0 * u0 * da[0], d1 * u1 * da[1]);
-                  du[half * 4 + i / 2] = pack2<T>(d0 * a[0], d1 * a[1]);
+                  dg.put(half * 4 + i / 2, d0 * u0 * da[0], d1 * u1 * da[1]);
+                  du.put(half * 4 + i / 2, d0 * a[0], d1 * a[1]);
                 }
               }
             }
             if (c + 16 == COLS) done(acc);
             if (!rows_here) continue;
             if (KIND == HIDDEN) {
-              emit<T, 8>(static_cast<T*>(g.out0), g.ld, row0, col, g.rows, g.cols, g.align, dg, stage);
-              emit<T, 8>(static_cast<T*>(g.out1), g.ld, row0, col, g.rows, g.cols, g.align, du, stage);
+              dg.emit_to(g.out0, g, row0, col, stage);
+              du.emit_to(g.out1, g, row0, col, stage);
             }
-            emit<T, 8>(static_cast<T*>(KIND == HIDDEN ? g.out2 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, h, stage);
+            h.emit_to(KIND == HIDDEN ? g.out2 : g.out0, g, row0, col, stage);
           }
         }
         turn++;
@@ -554,8 +584,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) to[i] = from_f<T>(v[i]);
 }
 
-// Matrices that TMA cannot read as they lie (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows: up to
-// five in one launch, each with blocks of its own.
+// Matrices that TMA cannot read as they lie (fp32, or rows off the 16-byte boundary), and fp16 ones that meet the hidden
+// matrices, laid out as planes of aligned rows: up to five in one launch, each with blocks of its own.
 struct Pack {
   const void* src;
   void* dst;
@@ -582,11 +612,17 @@ template <typename T, typename TO> __global__ void __launch_bounds__(256) pack_k
     for (int i = 0; i < 8; i++) {
       const T v = col + i < m.cols && LNCC_IN(row * m.stride + col + i, 1, (m.rows - 1) * m.stride + m.cols)
                       ? src[row * m.stride + col + i] : from_f<T>(0.f);
-      if constexpr (sizeof(T) == 4) take_apart(v, o[0].e[i], o[1].e[i], o[2].e[i]);
-      else o[0].e[i] = v;
+      if constexpr (sizeof(T) == 4) {
+        take_apart(v, o[0].e[i], o[1].e[i], o[2].e[i]);
+      } else if constexpr (std::is_same<T, TO>::value) {
+        o[0].e[i] = v;
+      } else {
+        o[0].e[i] = __float2bfloat16_rn(to_f(v));
+        o[1].e[i] = __float2bfloat16_rn(to_f(v) - to_f(o[0].e[i]));
+      }
     }
 #pragma unroll
-    for (int k = 0; k < (sizeof(T) == 4 ? 3 : 1); k++)
+    for (int k = 0; k < (sizeof(T) == 4 ? 3 : std::is_same<T, TO>::value ? 1 : 2); k++)
       *reinterpret_cast<Vec<TO, 8>*>(dst + k * m.plane + row * m.ld + col) = o[k];
   }
 }
@@ -867,7 +903,7 @@ struct Cut {
   int bn, m_tiles, n_tiles, splits, per_split;
 };
 static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
-  const int pairs = sm_count() / 2, parts = dtype == LNCC_F32 ? 6 : 1;
+  const int pairs = sm_count() / 2, parts = parts_of(kind, dtype);
   Cut best = {};
   double least = 0;
   for (int bn = 256; bn >= 128; bn -= 128) {
@@ -896,8 +932,9 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
 
 // Scratch of a call, laid out in one place for its size and its use.
 struct Plan {
-  int planes;
+  int planes, hidden_planes;  // of operands as they are given, and of the hidden matrices and what they are multiplied with
   size_t x, wg, wu, wd, dy, h, dg, du, gate, up, dh, norms, partial, total;
+  size_t x2, wg2, wu2, wd2, dy2;  // fp16: as two planes
   int64_t ldf;
 };
 static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
@@ -913,24 +950,33 @@ static Plan plan_for(const Args& a, bool backward) {
     return p;
   }
   p.planes = a.dtype == LNCC_F32 ? 3 : 1;
+  p.hidden_planes = a.dtype == LNCC_F32 ? 3 : a.dtype == LNCC_F16 ? 2 : 1;
   p.ldf = lead(a.F);
   size_t at = kHeader;
-  const auto take = [&](int64_t rows, int64_t ld) {
+  const auto planes = [&](int n, int64_t rows, int64_t ld) {
     const size_t here = at;
-    at += round_up(size_t(p.planes) * rows * ld * 2);
+    at += round_up(size_t(n) * rows * ld * 2);
     return here;
   };
+  const auto take = [&](int64_t rows, int64_t ld) { return planes(p.planes, rows, ld); };
   p.x = take(a.M, lead(a.K));
   p.wg = take(a.F, lead(a.K));
   p.wu = take(a.F, lead(a.K));
   p.wd = take(a.N, p.ldf);
-  p.h = take(a.M, p.ldf);
+  p.h = planes(p.hidden_planes, a.M, p.ldf);
+  if (a.dtype == LNCC_F16 && !backward) p.wd2 = planes(2, a.N, p.ldf);
+  if (a.dtype == LNCC_F16 && backward) {
+    p.x2 = planes(2, a.M, lead(a.K));
+    p.dy2 = planes(2, a.M, lead(a.N));
+    p.wg2 = planes(2, a.F, lead(a.K));
+    p.wu2 = planes(2, a.F, lead(a.K));
+  }
   size_t most = 0;
   const auto partial = [&](size_t n) { most = n > most ? n : most; };
   if (backward) {
     p.dy = take(a.M, lead(a.N));
-    p.dg = take(a.M, p.ldf);
-    p.du = take(a.M, p.ldf);
+    p.dg = planes(p.hidden_planes, a.M, p.ldf);
+    p.du = planes(p.hidden_planes, a.M, p.ldf);
     if (a.dtype == LNCC_F32) {
       p.gate = at, at += round_up(size_t(a.M) * p.ldf * 4);
       p.up = at, at += round_up(size_t(a.M) * p.ldf * 4);
@@ -960,7 +1006,7 @@ struct Call {
   int status;
   bool first = true;      // the next product kernel is the call's first
   bool launched = false;  // a kernel of this call is in the stream
-  Packs packs = {};
+  Packs packs = {}, halves = {};  // matrices to lay out, and fp16 ones as two planes
 
   // every kernel of a call but its first may be launched while the one before it ends (begin_after_previous)
   template <typename K, typename... A> void run(K kernel, dim3 grid, int threads, int smem, const A&... args) {
@@ -981,24 +1027,37 @@ struct Call {
       if (rows == 1) m.ld = lead(cols);
       return m;
     }
-    m.p = scratch + to;
-    m.ld = lead(cols);
-    m.plane = rows * m.ld;
-    m.planes = plan.planes;
-    const int64_t blocks = ceil_div(rows * (m.ld / 8), 256), most = int64_t(sm_count()) * 8;
-    packs.job[packs.jobs++] = {src, m.p, stride, rows, cols, m.ld, m.plane, packs.blocks};
-    packs.blocks += int(blocks < most ? blocks : most);
+    lay_out(packs, m, src, stride, to, plan.planes);
     return m;
   }
+  // src, which `given` describes, as an operand of a product with a hidden matrix
+  Matrix beside_hidden(const Matrix& given, const void* src, int64_t stride, size_t to) {
+    if (a.dtype != LNCC_F16) return given;
+    Matrix m = given;
+    m.bf16 = true;
+    lay_out(halves, m, src, stride, to, 2);
+    return m;
+  }
+  void lay_out(Packs& in, Matrix& m, const void* src, int64_t stride, size_t to, int planes) {
+    m.p = scratch + to;
+    m.ld = lead(m.cols);
+    m.plane = m.rows * m.ld;
+    m.planes = planes;
+    const int64_t blocks = ceil_div(m.rows * (m.ld / 8), 256), most = int64_t(sm_count()) * 8;
+    in.job[in.jobs++] = {src, m.p, stride, m.rows, m.cols, m.ld, m.plane, in.blocks};
+    in.blocks += int(blocks < most ? blocks : most);
+  }
   void pack() {
-    if (packs.jobs == 0) return;
-    const dim3 grid = dim3(unsigned(packs.blocks));
-    if (a.dtype == LNCC_F32) run(pack_kernel<float, __nv_bfloat16>, grid, 256, 0, packs);
-    else if (a.dtype == LNCC_BF16) run(pack_kernel<__nv_bfloat16, __nv_bfloat16>, grid, 256, 0, packs);
-    else run(pack_kernel<__half, __half>, grid, 256, 0, packs);
+    if (packs.jobs) {
+      const dim3 grid = dim3(unsigned(packs.blocks));
+      if (a.dtype == LNCC_F32) run(pack_kernel<float, __nv_bfloat16>, grid, 256, 0, packs);
+      else if (a.dtype == LNCC_BF16) run(pack_kernel<__nv_bfloat16, __nv_bfloat16>, grid, 256, 0, packs);
+      else run(pack_kernel<__half, __half>, grid, 256, 0, packs);
+    }
+    if (halves.jobs) run(pack_kernel<__half, __nv_bfloat16>, dim3(unsigned(halves.blocks)), 256, 0, halves);
   }
   Matrix hidden(size_t at) const {
-    return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.planes, a.dtype != LNCC_F16};
+    return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.hidden_planes, true};
   }
 
   template <int KIND, int BN, int ACT, typename T> void launch(Gemm& g) {
@@ -1144,10 +1203,10 @@ static int forward(const Args& a, const Plan& plan, void* scratch, cudaStream_t 
   Call c = {a, plan, static_cast<char*>(scratch), stream, LNCC_OK};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg),
                wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu), wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd),
-               h = c.hidden(c.plan.h);
+               h = c.hidden(c.plan.h), wd2 = c.beside_hidden(wd, a.wd, a.F, c.plan.wd2);
   c.pack();
   c.product<UP>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, h.p, nullptr, nullptr, h.ld, h.plane);
-  c.product<DOWN>(h, h, wd, wd, wd, a.M, a.N, 1, a.F, 0, a.y, nullptr, nullptr, a.N, 0);
+  c.product<DOWN>(h, h, wd2, wd2, wd2, a.M, a.N, 1, a.F, 0, a.y, nullptr, nullptr, a.N, 0);
   return c.status;
 }
 
@@ -1157,6 +1216,10 @@ static int backward(const Args& a, const Plan& plan, void* scratch, cudaStream_t
                wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg), wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu),
                wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd);
   const Matrix h = c.hidden(c.plan.h), dg = c.hidden(c.plan.dg), du = c.hidden(c.plan.du);
+  Matrix x2 = x, dy2 = dy, wg2 = wg, wu2 = wu;
+  if (a.dwg || a.dwu) x2 = c.beside_hidden(x, a.x, a.x_stride, c.plan.x2);
+  if (a.dwd) dy2 = c.beside_hidden(dy, a.dy, a.dy_stride, c.plan.dy2);
+  if (a.dx) wg2 = c.beside_hidden(wg, a.wg, a.K, c.plan.wg2), wu2 = c.beside_hidden(wu, a.wu, a.K, c.plan.wu2);
   c.pack();
   if (a.dtype == LNCC_F32) {
     float *const gate = reinterpret_cast<float*>(c.scratch + c.plan.gate), *const up = reinterpret_cast<float*>(c.scratch + c.plan.up),
@@ -1176,13 +1239,13 @@ static int backward(const Args& a, const Plan& plan, void* scratch, cudaStream_t
   } else {
     c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
   }
-  if (a.dx) c.product<DX>(dg, du, wg, wu, wg, a.M, a.K, 1, a.F, 0, a.dx, nullptr, nullptr, a.K, 0);
+  if (a.dx) c.product<DX>(dg, du, wg2, wu2, wg2, a.M, a.K, 1, a.F, 0, a.dx, nullptr, nullptr, a.K, 0);
   if (a.dwg || a.dwu) {
     // one product for both where both are wanted
     const Matrix& first = a.dwg ? dg : du;
-    c.product<DW_UP>(first, du, x, x, x, a.F, a.K, a.dwg && a.dwu ? 2 : 1, a.M, 0, a.dwg ? a.dwg : a.dwu, a.dwu, nullptr, a.K, 0);
+    c.product<DW_UP>(first, du, x2, x2, x2, a.F, a.K, a.dwg && a.dwu ? 2 : 1, a.M, 0, a.dwg ? a.dwg : a.dwu, a.dwu, nullptr, a.K, 0);
   }
-  if (a.dwd) c.product<DW_DOWN>(dy, dy, h, h, h, a.N, a.F, 1, a.M, 0, a.dwd, nullptr, nullptr, a.F, 0);
+  if (a.dwd) c.product<DW_DOWN>(dy2, dy2, h, h, h, a.N, a.F, 1, a.M, 0, a.dwd, nullptr, nullptr, a.F, 0);
   return c.status;
 }
 
