@@ -481,7 +481,10 @@ int lncc_layer_norm_forward(const void* x, int64_t x_stride, const void* weight,
   const int st = norm::check_common(dtype, wdtype, rows, width, x, x_stride);
   if (st != LNCC_OK) return st;
   if (rows == 0) return LNCC_OK;
-  if (!y || !blk::aligned(y, blk::elem_size(dtype)) || (mean == nullptr) != (rstd == nullptr)) return LNCC_ERR_BAD_ARG;
+  const int we = blk::elem_size(wdtype);
+  if (!y || !blk::aligned(y, blk::elem_size(dtype)) || !blk::aligned(weight, we) || !blk::aligned(bias, we) ||
+      (mean == nullptr) != (rstd == nullptr) || !blk::aligned(mean, 4) || !blk::aligned(rstd, 4))
+    return LNCC_ERR_BAD_ARG;
   const int cb = blk::check_begin();
   if (cb != LNCC_OK) return cb;
   norm::Args a = {};
@@ -503,6 +506,8 @@ int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, i
   const int st = norm::check_common(dtype, wdtype, rows, width, x, x_stride);
   if (st != LNCC_OK) return st;
   const bool params = dweight || dbias;
+  const int we = blk::elem_size(wdtype);
+  if (!blk::aligned(dweight, we) || !blk::aligned(dbias, we)) return LNCC_ERR_BAD_ARG;
   if (rows == 0) {  // sums over no rows
     const size_t n = size_t(width) * blk::elem_size(wdtype);
     if (dweight && cudaMemsetAsync(dweight, 0, n, stream) != cudaSuccess) return LNCC_ERR_CUDA;
@@ -510,7 +515,8 @@ int lncc_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, i
     return LNCC_OK;
   }
   const int e = blk::elem_size(dtype);
-  if (!dy || !blk::aligned(dy, e) || (dy_stride < width && rows > 1) || !mean || !rstd || (dx && !blk::aligned(dx, e)))
+  if (!dy || !blk::aligned(dy, e) || (dy_stride < width && rows > 1) || !blk::aligned(weight, we) || !mean || !rstd ||
+      !blk::aligned(mean, 4) || !blk::aligned(rstd, 4) || (dx && !blk::aligned(dx, e)))
     return LNCC_ERR_BAD_ARG;
   if (params && (!scratch || !blk::aligned(scratch, 4) || scratch_bytes < lncc_layer_norm_scratch_bytes(rows, width)))
     return LNCC_ERR_WORKSPACE;
