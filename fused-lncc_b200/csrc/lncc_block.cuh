@@ -79,8 +79,9 @@ inline int sm_count() {
 }
 
 // In the bounds-checked build: zero this file's violation counter before a call's launches, and turn a count into
-// LNCC_ERR_CHECK after them. In the normal build both cost nothing.
-inline int check_begin() {
+// LNCC_ERR_CHECK after them. In the normal build both cost nothing. Static: each source file has a counter of its own, and one
+// function for all of them would read one file's.
+static inline int check_begin() {
 #ifdef LNCC_CHECKED
   const unsigned long long z = 0;
   return cudaMemcpyToSymbol(g_check_violations, &z, sizeof(z)) == cudaSuccess ? LNCC_OK : LNCC_ERR_CUDA;
@@ -88,7 +89,7 @@ inline int check_begin() {
   return LNCC_OK;
 #endif
 }
-inline int check_end(cudaStream_t stream) {
+static inline int check_end(cudaStream_t stream) {
   if (cudaGetLastError() != cudaSuccess) return LNCC_ERR_LAUNCH;
 #ifdef LNCC_CHECKED
   unsigned long long n = 0;
