@@ -1062,16 +1062,16 @@ struct Call {
 
   template <int KIND, int BN, int ACT, typename T> void launch(Gemm& g) {
     const int smem = smem_bytes(BN), pairs = sm_count() / 2;
-    static uint64_t asked;  // devices that were asked for this kernel's shared memory; asking twice does no harm
+    static Asked asked;
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || !(asked >> dev & 1)) {
+    if (cudaGetDevice(&dev) != cudaSuccess || !asked.has(dev)) {
       if (cudaFuncSetAttribute(product_kernel<KIND, BN, ACT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
           cudaSuccess) {
         cudaGetLastError();
         status = LNCC_ERR_SMEM;
         return;
       }
-      if (dev < 64) asked |= 1ull << dev;
+      asked.mark(dev);
     }
     const int64_t tiles = int64_t(g.m_tiles) * g.n_tiles * g.whichs * g.splits;
     run(product_kernel<KIND, BN, ACT, T>, dim3(unsigned(2 * (tiles < pairs ? tiles : pairs))), kThreads, smem, g);

@@ -408,10 +408,10 @@ template <typename T, int VEC, int E, int LANES> static void launch_lanes(const 
   constexpr int threads = threads_of<LANES>();
   const int ring = Rows<T, LANES, VEC, E, threads>::smem(), smem = backward ? 2 * ring : ring;
   const auto kernel = backward ? backward_kernel<T, LANES, VEC, E> : forward_kernel<T, LANES, VEC, E>;
-  static uint64_t asked[2];  // devices that were asked for this kernel's shared memory; asking twice does no harm
+  static Asked asked[2];
   int dev = 0;
-  if (smem > 40 * 1024 && cudaGetDevice(&dev) == cudaSuccess && dev < 64 && !(asked[backward] >> dev & 1)) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) asked[backward] |= 1ull << dev;
+  if (smem > 40 * 1024 && cudaGetDevice(&dev) == cudaSuccess && !asked[backward].has(dev)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) asked[backward].mark(dev);
   }
   kernel<<<grid, threads, smem, st>>>(a);
 }

@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace lncc {
 namespace blk {
 
@@ -67,16 +69,25 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // SMs of the current device (148 where it cannot be asked), read once per device.
 inline int sm_count() {
-  static int counts[64];
+  static std::atomic<int> counts[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (counts[dev] == 0) {
-    int n = 0;
+  int n = counts[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
-    counts[dev] = n;
+    counts[dev].store(n, std::memory_order_relaxed);
   }
-  return counts[dev];
+  return n;
 }
+
+// The devices that were asked for a kernel's shared memory, marked by any thread. Asking twice does no harm.
+struct Asked {
+  std::atomic<uint64_t> devices{0};
+  bool has(int dev) const { return dev < 64 && devices.load(std::memory_order_relaxed) >> dev & 1; }
+  void mark(int dev) {
+    if (dev < 64) devices.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+};
 
 // In the bounds-checked build: zero this file's violation counter before a call's launches, and turn a count into
 // LNCC_ERR_CHECK after them. In the normal build both cost nothing. Static: each source file has a counter of its own, and one

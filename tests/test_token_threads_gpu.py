@@ -59,3 +59,28 @@ assert all(t.isfinite().all() for t in g)
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_first_calls_of_many_threads_at_once():
+    """The library's marks of what a device was asked for are set by any thread, here by sixteen that start together, each on a
+    stream of its own, with kernels that no other test has to have run before."""
+    def work(i):
+        g = torch.Generator(device="cuda").manual_seed(i % 4)
+        x = torch.randn(33 + i % 4, 1000 + 8 * (i % 4), generator=g, device="cuda").half()
+        w = [torch.randn(*s, generator=g, device="cuda").half() * 0.03 for s in ((96, x.shape[1]), (96, x.shape[1]), (64, 96))]
+        y = fused_lncc.fused_layer_norm(x)
+        return fused_lncc.fused_gated_ffn(y, *w, activation=("silu", "gelu", "relu")[i % 3])
+    got, start = [None] * 16, threading.Barrier(16)
+
+    def thread(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            start.wait()
+            got[i] = work(i)
+            torch.cuda.current_stream().synchronize()
+    threads = [threading.Thread(target=thread, args=(i,)) for i in range(16)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(16):
+        assert torch.equal(got[i], work(i)), i
