@@ -23,19 +23,10 @@
 // Nothing of the hidden layer is kept between forward and backward. Forming g and u again costs 4 of 22 M F K products of a
 // training step, and saves writing and reading 4 M F bytes and a rounding of g and u.
 //
-// Roundings. g, u and dh never leave fp32; h, dg and du are operands of the next product. For bf16 they are rounded to the type.
-// The result then holds two roundings of like size, its own and h's, and is sqrt 2 as far off as one that
-// keeps h in fp32 (more than four tokens: 2.4e-3 of the result against 1.7e-3); in calls of
-// a few hundred values the factor scatters, at 5 x 48 x 79 between 1.25 and 1.63 in nine draws of ten.
-// fp16 would not do for them: its range is 2^-24 to 2^16, and hidden values of a block with small results pass 65504, and the
-// gradients of a mean over many tokens lie among its subnormal numbers (dWg was off by 4e-2 at dy = 1e-6). So with fp16 the
-// hidden matrices are held as two bf16 numbers each, 16 bits in fp32's range, and so is what they are multiplied with (fp16's 11
-// bits, exactly); three of the four products are summed, smallest first (the fourth is below 2^-18). UP and HIDDEN read fp16 as
-// it is. The result has its own rounding alone (2.1e-4, where an fp16 h gave 2.9e-4), and the products after the activation take
-// three times as long: 4096 x 768 x 2048 forward 69 us (44 in bf16), 107520 x 96 x 256 training 349 (196), 16384 x 1024 x 4096 2575
-// (1152). Rows of fp16 numbers times a power of 2 each, from a bound of the row, would run at bf16's speed, but lose what
-// lies 2^-29 below the bound, which is some 2^16 above a dense row's values and more where a few weights stand out.
-// fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
+// Roundings. For 16-bit types h, dg and du are rounded to the type's bits, since they are operands of the next product (for fp16
+// times a power of 2 a row, see below: its range would not hold them); g, u and dh never leave fp32. The result then holds two roundings of like size, its own and h's, and is sqrt 2 as far off as one that
+// keeps h in fp32 (fp16, more than four tokens: 2.9e-4 of the result against 2.1e-4; bf16 2.4e-3 against 1.7e-3); in calls of
+// a few hundred values the factor scatters, at 5 x 48 x 79 between 1.25 and 1.63 in nine draws of ten. fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
 // the nine products are summed, smallest first (the other three are below 2^-24 of the result). The tensor cores cut, not
 // round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of an fp32 result. So for fp32 an
 // accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each time. The 16-bit
@@ -59,20 +50,16 @@ enum Kind { UP, GATES, HIDDEN, DH, DOWN, DX, DW_UP, DW_DOWN };
 constexpr int kEpilogueWarps = 16;         // of a CTA: four for each quarter of the lanes of tensor memory
 constexpr int kThreads = 128 + 32 * kEpilogueWarps;  // warps 0 TMA, 1 products, 4 - 19 epilogue
 constexpr int kATile = 128 * 64 * 2;       // bytes of a CTA's share of A in a stage
-// Blocks of 64 that an accumulator takes. Operands that are taken apart are read once for each product: 4 or 8 blocks of them
-// stay in L2 meanwhile.
-constexpr int kChunk = 4, kChunkHalf = 8, kChunkBf16 = 32;
+constexpr int kChunk = 4, kChunk16 = 32;   // blocks of 64 that an accumulator takes: fp32, and 16-bit types where sums are long
 
 __host__ __device__ constexpr bool a_mn(int kind) { return kind == DW_UP || kind == DW_DOWN; }
 __host__ __device__ constexpr bool b_mn(int kind) { return kind == DH || kind == DX || kind == DW_UP || kind == DW_DOWN; }
 __host__ __device__ constexpr bool gated(int kind) { return kind == UP || kind == GATES || kind == HIDDEN; }
-// products of parts of the operands
-__host__ __device__ constexpr int parts_of(int kind, int dtype) { return dtype == LNCC_F32 ? 6 : dtype == LNCC_F16 && !gated(kind) ? 3 : 1; }
 __host__ __device__ constexpr int b_tile(int bn) { return bn / 2 * 64 * 2; }  // a CTA's share of B
 __host__ __device__ constexpr int stages(int bn) { return bn == 256 ? 6 : 8; }
 __host__ __device__ constexpr int smem_bytes(int bn) { return 1024 + stages(bn) * (kATile + b_tile(bn)) + 256 + kEpilogueWarps * 32 * 9 * 4; }
 
-// Planes of the six products of operands that are taken apart into three, smallest first; the last three are those of two.
+// Planes of the six products of operands that are taken apart, smallest first.
 __device__ __constant__ const int8_t kPlaneA[6] = {2, 1, 0, 1, 0, 0}, kPlaneB[6] = {0, 1, 2, 0, 1, 0};
 
 struct Gemm {
@@ -86,6 +73,9 @@ struct Gemm {
   int64_t ld, plane;         // of the results; plane for h taken apart
   int align;                 // bytes on which every row of the results starts: 32, 16 or the element's
   float* partial;            // [splits][whichs][rows][cols rounded up to 4], where splits > 1
+  int8_t* levels;            // fp16: of the hidden matrices, as the gated kinds write them
+  const int *row_h, *row_d, *most;  // and as level_kernel leaves them
+  int level_blocks;
   unsigned* abort_word;
   int clear_abort;
 };
@@ -182,22 +172,6 @@ __device__ __forceinline__ void take_apart(float v, __nv_bfloat16& hi, __nv_bflo
   mid = __float2bfloat16_rn(fine ? r : 0.f);
   lo = __float2bfloat16_rn(fine ? r - __bfloat162float(mid) : 0.f);
 }
-// Two neighbours of a hidden matrix as operands of the next product: rounded to bf16, or, for fp16, as the sum of two bf16
-// numbers that hold 16 bits (infinities become NaN).
-template <typename T> struct Words {  // of 16 columns of a row
-  uint32_t hi[8], lo[std::is_same<T, __half>::value ? 8 : 1];
-  __device__ __forceinline__ void put(int i, float a, float b) {
-    hi[i] = pack2<__nv_bfloat16>(a, b);
-    if constexpr (std::is_same<T, __half>::value)
-      lo[i] = pack2<__nv_bfloat16>(a - __uint_as_float(hi[i] << 16), b - __uint_as_float(hi[i] & 0xffff0000u));
-  }
-  __device__ __forceinline__ void emit_to(void* base, const Gemm& g, int64_t row0, int64_t col, uint32_t* stage) const {
-    __nv_bfloat16* to = static_cast<__nv_bfloat16*>(base);
-    emit<__nv_bfloat16, 8>(to, g.ld, row0, col, g.rows, g.cols, g.align, hi, stage);
-    if constexpr (std::is_same<T, __half>::value)
-      emit<__nv_bfloat16, 8>(to + g.plane, g.ld, row0, col, g.rows, g.cols, g.align, lo, stage);
-  }
-};
 // Eight results of a row in fp32, as the three bf16 matrices that hold them.
 __device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t row0, int64_t col, const float (&v)[8],
                                            uint32_t* stage) {
@@ -215,6 +189,51 @@ __device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t ro
     for (int i = 0; i < 4; i++) w[i] = pack2<__nv_bfloat16>(part[k][2 * i], part[k][2 * i + 1]);
     emit<__nv_bfloat16, 4>(static_cast<__nv_bfloat16*>(base) + k * g.plane, g.ld, row0, col, g.rows, g.cols, g.align, w, stage);
   }
+}
+
+// ---- the range of fp16 -------------------------------------------------------------------------------------------------
+// h, dg and du are operands of the next product, and as they are they need not lie in fp16's range: gates and up projections
+// of some hundreds give hidden values past 65504 in a block whose result is small, and the gradients of a mean over many tokens
+// lie among the subnormal numbers. So with fp16 a row of them is stored times a power of 2. Its largest value is not known
+// while its tiles are written (a bound like |x|_1 max|W| is some 2^16 above the values of a dense row, and more where a few
+// weights stand out), so each piece of 8 columns gets a power of its own, 2^(11 - 8k) with the smallest k that keeps the piece
+// below 2^15, and level_kernel then brings the pieces of a row to the power of the row's largest k. Steps of 8, of which k = 0
+// holds pieces whose largest value lies between 2^-4 and 2^4, leave few or none to rewrite. What is 2^-21 of its row's largest
+// value and more keeps fp16's 11 bits at least; the rest is right to 2^-32 of it.
+// The product that reads a row takes its power back out in the epilogue (DOWN, DX). The weights' gradients sum over rows of
+// different powers: there the other operand, x or dy, is copied with the row's power taken out of it, relative to the largest
+// of the call. dg and du share a power, since dx adds their products up. Measured beside bf16: 4096 x 768 x 2048 forward 54 us
+// (43), 107520 x 96 x 256 training 275 (197), 16384 x 1024 x 4096 training 1384 (1315); level_kernel's backward part 19, 33 and
+// 62 us of them, 101 where every row has pieces to rewrite. As two bf16 numbers each, 16 bits in fp32's range, h, dg and du took
+// three products for one: 69, 349 and 2575 us.
+constexpr int kStep = 8;
+constexpr int kNoLevel = -64;      // k of zeros
+constexpr int kLowest = -13;       // the least k otherwise
+enum Most { MOST_DY_H, MOST_X_D, MOSTS };  // largest e + kStep k of |dy| < 2^e and h, and of |x| and dg, du
+
+__device__ __forceinline__ float power_of_2(int e) { return __int_as_float((max(-126, min(126, e)) + 127) << 23); }
+// k of numbers whose largest absolute value is v
+__device__ __forceinline__ int level_of(float v) {
+  return v > 0.f ? max(kLowest, ((__float_as_int(v) >> 23) - 123) >> 3) : kNoLevel;
+}
+__device__ __forceinline__ float power_of_level(int k) { return power_of_2(11 - kStep * max(k, kLowest)); }
+// the largest finite |v[i]|, and `least`
+template <int N> __device__ __forceinline__ float largest(const float (&v)[N], float least) {
+  float m = least;
+#pragma unroll
+  for (int i = 0; i < N; i++) m = fmaxf(m, fabsf(v[i]));
+  if (m > 3.4028235e38f) {
+    m = least;
+#pragma unroll
+    for (int i = 0; i < N; i++) m = fmaxf(m, fabsf(v[i]) <= 3.4028235e38f ? fabsf(v[i]) : 0.f);
+  }
+  return m;
+}
+// one of the call's largest, of the blocks' ones, for a whole warp
+__device__ __forceinline__ int most_of(const int* most, int blocks, int which) {
+  int e = kStep * kNoLevel;
+  for (int i = threadIdx.x % 32; i < blocks; i += 32) e = max(e, most[which * blocks + i]);
+  return __reduce_max_sync(0xffffffffu, e);
 }
 
 // A call's kernels but the first are launched before the one ahead has ended. Each lets the next begin at once and waits here
@@ -253,10 +272,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
   constexpr bool ONE = KIND == HIDDEN && BN == 256;
   constexpr int ACCS = ONE ? 1 : 2;
   constexpr int DH_BYTES = BN == 256 ? 8192 : 4096;    // a CTA's share of Wd in a stage: 64 or 32 columns
-  constexpr bool HALF_T = std::is_same<T, __half>::value;
-  constexpr int PARTS = parts_of(KIND, F32 ? LNCC_F32 : HALF_T ? LNCC_F16 : LNCC_BF16);
+  constexpr int PARTS = F32 ? 6 : 1;                   // products of parts of the operands
   constexpr bool PROMOTED = F32 || !gated(KIND);       // accumulators take a chunk each, and are added up in registers
-  constexpr int CHUNK = F32 ? kChunk : !PROMOTED ? 1 << 30 : HALF_T ? kChunkHalf : kChunkBf16;
+  constexpr int CHUNK = F32 ? kChunk : PROMOTED ? kChunk16 : 1 << 30;
   static_assert(KIND != HIDDEN || !F32, "fp32 has GATES and DH");
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((uintptr_t(raw) + 1023) / 1024 * 1024);
@@ -314,7 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
       for (int c = w.from; c < w.to && ok; c += CHUNK) {
         const int c_end = PROMOTED ? min(c + CHUNK, w.to) : w.to;
         for (int part = 0; part < PARTS && ok; part++) {
-          const int pa = PARTS > 1 ? kPlaneA[6 - PARTS + part] : 0, pb = PARTS > 1 ? kPlaneB[6 - PARTS + part] : 0;
+          const int pa = F32 ? kPlaneA[part] : 0, pb = F32 ? kPlaneB[part] : 0;
           for (int b = c; b < c_end; b++) {
             if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up))) break;
             const uint32_t at = tiles_at + stage * (kATile + BT), bt = at + kATile, bar = full_of_pair + 8 * stage;
@@ -397,6 +415,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
     constexpr int COLS = gated(KIND) ? HALF / 4 : BN / 4;  // columns of a result that a warp takes
     uint32_t* const stage = reinterpret_cast<uint32_t*>(smem + STAGES * (kATile + BT) + 256) + (warp - 4) * kStageWords;
     int turn = 0;
+    constexpr bool LEVELS = std::is_same<T, __half>::value;
+    // weights' gradients: what their operands lack together
+    const float power_all =
+        LEVELS && AM ? power_of_2(most_of(g.most, g.level_blocks, KIND == DW_UP ? MOST_X_D : MOST_DY_H) - 26) : 1.f;
     for (int t = blockIdx.x / 2; t < tiles; t += pairs_at_work) {
       const Tile w = tile_of(g, t);
       const int64_t row0 = int64_t(w.m) * 256 + rank * 128 + sub * 32;
@@ -465,6 +487,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
             emit_parts(g.out0, g, row0, col0 + c, h, stage);
           }
         } else if constexpr (!F32) {
+          if (LEVELS) {
+            float power = power_all;
+            if (!AM && row0 + lane < g.rows) power = power_of_2(kStep * (KIND == DOWN ? g.row_h : g.row_d)[row0 + lane] - 11);
+#pragma unroll
+            for (int c = 0; c < SUMS; c++) sum[c] *= power;
+          }
 #pragma unroll
           for (int c = 0; c < SUMS; c += 16) put(col0 + c, reinterpret_cast<const float(&)[16]>(sum[c]));
         } else {
@@ -492,7 +520,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           __syncwarp();
           const int64_t col = col0 + c;
           {
-            Words<T> h, dg, du;
+            uint32_t h[8], dg[8], du[8];
+            uint32_t levels = 0;  // a byte a piece: of h, and then of dg and du
 #pragma unroll
             for (int half = 0; half < 2; half++) {  // eight columns at a time: 640 threads leave 102 registers each
               uint32_t v[3][8];
@@ -507,27 +536,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
               } else {
                 for (int i = 0; i < 8; i++) v[0][i] = v[1][i] = v[2][i] = kNaN;
               }
+              float fh[8], fdg[8], fdu[8];
 #pragma unroll
               for (int i = 0; i < 8; i += 2) {
                 float a[2], da[2];
 #pragma unroll
                 for (int j = 0; j < 2; j++) activate<ACT, true>(__uint_as_float(v[0][i + j]), a[j], da[j]);
                 const float u0 = __uint_as_float(v[1][i]), u1 = __uint_as_float(v[1][i + 1]);
-                h.put(half * 4 + i / 2, a[0] * u0, a[1] * u1);
+                fh[i] = a[0] * u0, fh[i + 1] = a[1] * u1;
                 if (KIND == HIDDEN) {
                   const float d0 = __uint_as_float(v[2][i]), d1 = __uint_as_float(v[2][i + 1]);
-                  dg.put(half * 4 + i / 2, d0 * u0 * da[0], d1 * u1 * da[1]);
-                  du.put(half * 4 + i / 2, d0 * a[0], d1 * a[1]);
+                  fdg[i] = d0 * u0 * da[0], fdg[i + 1] = d1 * u1 * da[1];
+                  fdu[i] = d0 * a[0], fdu[i + 1] = d1 * a[1];
+                }
+              }
+              float power_h = 1.f, power_d = 1.f;
+              if (LEVELS) {
+                const int k = level_of(largest(fh, 0.f));
+                power_h = power_of_level(k);
+                levels |= uint32_t(k & 255) << 8 * half;
+                if (KIND == HIDDEN) {
+                  const int kd = level_of(largest(fdg, largest(fdu, 0.f)));
+                  power_d = power_of_level(kd);
+                  levels |= uint32_t(kd & 255) << 16 + 8 * half;
+                }
+              }
+#pragma unroll
+              for (int i = 0; i < 8; i += 2) {
+                const float ph = power_h, pd = power_d;
+                h[half * 4 + i / 2] = LEVELS ? pack2<T>(fh[i] * ph, fh[i + 1] * ph) : pack2<T>(fh[i], fh[i + 1]);
+                if (KIND == HIDDEN) {
+                  dg[half * 4 + i / 2] = LEVELS ? pack2<T>(fdg[i] * pd, fdg[i + 1] * pd) : pack2<T>(fdg[i], fdg[i + 1]);
+                  du[half * 4 + i / 2] = LEVELS ? pack2<T>(fdu[i] * pd, fdu[i + 1] * pd) : pack2<T>(fdu[i], fdu[i + 1]);
                 }
               }
             }
             if (c + 16 == COLS) done(acc);
             if (!rows_here) continue;
             if (KIND == HIDDEN) {
-              dg.emit_to(g.out0, g, row0, col, stage);
-              du.emit_to(g.out1, g, row0, col, stage);
+              emit<T, 8>(static_cast<T*>(g.out0), g.ld, row0, col, g.rows, g.cols, g.align, dg, stage);
+              emit<T, 8>(static_cast<T*>(g.out1), g.ld, row0, col, g.rows, g.cols, g.align, du, stage);
             }
-            h.emit_to(KIND == HIDDEN ? g.out2 : g.out0, g, row0, col, stage);
+            emit<T, 8>(static_cast<T*>(KIND == HIDDEN ? g.out2 : g.out0), g.ld, row0, col, g.rows, g.cols, g.align, h, stage);
+            if (LEVELS && row0 + lane < g.rows && col < g.cols) {
+              const int64_t at = (row0 + lane) * ((g.cols + 15) / 16) + col / 16;
+              if (!LNCC_IN(at, 1, g.rows * ((g.cols + 15) / 16))) continue;
+              if (KIND == HIDDEN) reinterpret_cast<uint32_t*>(g.levels)[at] = levels;
+              else reinterpret_cast<uint16_t*>(g.levels)[at] = uint16_t(levels);
+            }
           }
         }
         turn++;
@@ -584,8 +640,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     if (col + i < cols && LNCC_IN(row * cols + col + i, 1, rows * cols)) to[i] = from_f<T>(v[i]);
 }
 
-// Matrices that TMA cannot read as they lie (fp32, or rows off the 16-byte boundary), and fp16 ones that meet the hidden
-// matrices, laid out as planes of aligned rows: up to five in one launch, each with blocks of its own.
+// Matrices that TMA cannot read as they lie (fp32, or rows off the 16-byte boundary) laid out as planes of aligned rows: up to
+// five in one launch, each with blocks of its own.
 struct Pack {
   const void* src;
   void* dst;
@@ -612,18 +668,154 @@ template <typename T, typename TO> __global__ void __launch_bounds__(256) pack_k
     for (int i = 0; i < 8; i++) {
       const T v = col + i < m.cols && LNCC_IN(row * m.stride + col + i, 1, (m.rows - 1) * m.stride + m.cols)
                       ? src[row * m.stride + col + i] : from_f<T>(0.f);
-      if constexpr (sizeof(T) == 4) {
-        take_apart(v, o[0].e[i], o[1].e[i], o[2].e[i]);
-      } else if constexpr (std::is_same<T, TO>::value) {
-        o[0].e[i] = v;
-      } else {
-        o[0].e[i] = __float2bfloat16_rn(to_f(v));
-        o[1].e[i] = __float2bfloat16_rn(to_f(v) - to_f(o[0].e[i]));
-      }
+      if constexpr (sizeof(T) == 4) take_apart(v, o[0].e[i], o[1].e[i], o[2].e[i]);
+      else o[0].e[i] = v;
     }
 #pragma unroll
-    for (int k = 0; k < (sizeof(T) == 4 ? 3 : std::is_same<T, TO>::value ? 1 : 2); k++)
+    for (int k = 0; k < (sizeof(T) == 4 ? 3 : 1); k++)
       *reinterpret_cast<Vec<TO, 8>*>(dst + k * m.plane + row * m.ld + col) = o[k];
+  }
+}
+
+// fp16: brings the pieces of each hidden row to the row's largest level, and finds what the sums over tokens start from; a
+// group of `lanes` threads a row.
+struct LevelArgs {
+  __half *h, *dg, *du;                  // dg, du, x, dy null: forward
+  const __half *x, *dy;
+  int64_t x_stride, dy_stride, M, K, F, N, ld;
+  int lanes;                            // a power of 2 up to 32
+  const int8_t* levels;
+  int *row_h, *row_d, *most;            // most: [MOSTS][blocks]
+};
+// e with |p[i]| < 2^e for the finite ones of a row; lanes share it
+__device__ __forceinline__ int exponent_of_row(const __half* p, int64_t n, int lane, int lanes) {
+  uint32_t most = 0;
+  const auto one = [&](uint32_t bits) {
+    bits &= 0x7fffu;
+    if (bits < 0x7c00u) most = max(most, bits);
+  };
+  int64_t done = 0;
+  if (reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+    done = n / 8 * 8;
+    for (int64_t i = lane; i < n / 8; i += lanes) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      one(v.x), one(v.x >> 16), one(v.y), one(v.y >> 16), one(v.z), one(v.z >> 16), one(v.w), one(v.w >> 16);
+    }
+  }
+  for (int64_t i = done + lane; i < n; i += lanes) one(reinterpret_cast<const uint16_t*>(p)[i]);
+  return most ? ilogbf(__half2float(__ushort_as_half(uint16_t(most)))) + 1 : kStep * kNoLevel;
+}
+template <bool BACK> __global__ void __launch_bounds__(256) level_kernel(const LevelArgs p) {
+  begin_after_previous();
+  __shared__ int meet[MOSTS][8];
+  int most[MOSTS] = {kStep * kNoLevel, kStep * kNoLevel};
+  const int lane = threadIdx.x % p.lanes, groups = 256 / p.lanes;
+  const int64_t pieces = (p.F + 15) / 16;  // pairs of pieces of a row
+  const auto across = [&](int k) {  // the largest of the row's lanes
+    for (int o = p.lanes / 2; o > 0; o /= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, o));
+    return k;
+  };
+  // a warp's lanes take the same number of turns
+  for (int64_t r0 = int64_t(blockIdx.x) * groups; r0 < p.M; r0 += int64_t(gridDim.x) * groups) {
+    const int64_t row = r0 + threadIdx.x / p.lanes;
+    const bool here = row < p.M;
+    const auto levels = [&](int64_t i) {  // of pair i, a byte each
+      return BACK ? reinterpret_cast<const uint32_t*>(p.levels)[row * pieces + i]
+                  : reinterpret_cast<const uint16_t*>(p.levels)[row * pieces + i];
+    };
+    const auto level = [](uint32_t w, int byte) { return int(int8_t(w >> 8 * byte)); };
+    int kh = kNoLevel, kd = kNoLevel;
+    for (int64_t i = lane; here && i < pieces; i += p.lanes) {
+      const uint32_t w = levels(i);
+      kh = max(kh, max(level(w, 0), level(w, 1)));
+      if (BACK) kd = max(kd, max(level(w, 2), level(w, 3)));
+    }
+    kh = across(kh), kd = BACK ? across(kd) : kd;
+    for (int64_t i = lane; here && i < pieces; i += p.lanes) {
+      const uint32_t w = levels(i);
+      constexpr int PIECES = BACK ? 6 : 2;  // two of h, of dg and of du
+      typedef Vec<__half, 8> V;
+      V v[PIECES];
+      V* at[PIECES];
+      int steps[PIECES];
+#pragma unroll
+      for (int j = 0; j < PIECES; j++) {  // all loads first
+        const int64_t from = row * p.ld + i * 16 + j % 2 * 8;
+        const int k = level(w, j < 2 ? j : 2 + j % 2);
+        at[j] = reinterpret_cast<V*>((j < 2 ? p.h : j < 4 ? p.dg : p.du) + from);
+        steps[j] = k == kNoLevel || !LNCC_IN(from, 8, p.M * p.ld) ? 0 : k - (j < 2 ? kh : kd);
+        if (steps[j]) v[j] = *at[j];
+      }
+#pragma unroll
+      for (int j = 0; j < PIECES; j++) {
+        if (!steps[j]) continue;
+        const float power = power_of_2(kStep * steps[j]);
+#pragma unroll
+        for (int c = 0; c < 8; c++) v[j].e[c] = __float2half_rn(__half2float(v[j].e[c]) * power);
+        *at[j] = v[j];
+      }
+    }
+    int ey = 0, ex = 0;
+    if (BACK) {
+      ex = across(here ? exponent_of_row(p.x + row * p.x_stride, p.K, lane, p.lanes) : 0);
+      ey = across(here ? exponent_of_row(p.dy + row * p.dy_stride, p.N, lane, p.lanes) : 0);
+    }
+    if (!here || lane != 0 || !LNCC_IN(row, 1, p.M)) continue;
+    p.row_h[row] = kh;
+    if (!BACK) continue;
+    p.row_d[row] = kd;
+    if (kh != kNoLevel) most[MOST_DY_H] = max(most[MOST_DY_H], ey + kStep * kh);
+    if (kd != kNoLevel) most[MOST_X_D] = max(most[MOST_X_D], ex + kStep * kd);
+  }
+  if (!BACK) return;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < MOSTS; i++) {
+    const int e = __reduce_max_sync(0xffffffffu, most[i]);
+    if (threadIdx.x % 32 == 0) meet[i][threadIdx.x / 32] = e;
+  }
+  __syncthreads();
+  if (threadIdx.x >= MOSTS) return;
+  int e = meet[threadIdx.x][0];
+  for (int i = 1; i < 8; i++) e = max(e, meet[threadIdx.x][i]);
+  if (LNCC_IN(threadIdx.x * gridDim.x + blockIdx.x, 1, MOSTS * gridDim.x)) p.most[threadIdx.x * gridDim.x + blockIdx.x] = e;
+}
+// x and dy for the weights' gradients, in aligned rows: a row times the power of 2 that its dg and du, or its h, lack.
+struct Rescale {
+  const __half *x, *dy;  // null: not wanted
+  int64_t x_stride, dy_stride, M, K, N, ld_x, ld_dy;
+  __half *to_x, *to_dy;
+  const int *row_h, *row_d, *most;
+  int level_blocks;
+};
+__global__ void __launch_bounds__(256) rescale_kernel(const Rescale p) {
+  begin_after_previous();
+#pragma unroll
+  for (int which = 0; which < 2; which++) {
+    const __half* src = which ? p.dy : p.x;
+    if (src == nullptr) continue;
+    const int most = most_of(p.most, p.level_blocks, which ? MOST_DY_H : MOST_X_D);
+    const int* levels = which ? p.row_h : p.row_d;
+    __half* dst = which ? p.to_dy : p.to_x;
+    const int64_t stride = which ? p.dy_stride : p.x_stride, cols = which ? p.N : p.K, ld = which ? p.ld_dy : p.ld_x;
+    const bool whole = reinterpret_cast<uintptr_t>(src) % 16 == 0 && stride % 8 == 0;
+    const uint32_t per_row = uint32_t(ld / 8);
+    for (int64_t q = int64_t(blockIdx.x) * 256 + threadIdx.x; q < p.M * per_row; q += int64_t(gridDim.x) * 256) {
+      const int64_t row = q / per_row, col = (q - row * per_row) * 8;
+      const int k = levels[row], e = 15 - most + kStep * k;
+      const float power = k == kNoLevel || e < -126 ? 0.f : power_of_2(e);
+      const __half* from = src + row * stride + col;
+      Vec<__half, 8> v;
+      if (whole && col + 8 <= cols) {
+        v = *reinterpret_cast<const Vec<__half, 8>*>(from);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v.e[i] = col + i < cols ? from[i] : __half(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; i++) v.e[i] = __float2half_rn(__half2float(v.e[i]) * power);
+      if (LNCC_IN(row * ld + col, 8, p.M * ld)) *reinterpret_cast<Vec<__half, 8>*>(dst + row * ld + col) = v;
+    }
   }
 }
 
@@ -903,7 +1095,7 @@ struct Cut {
   int bn, m_tiles, n_tiles, splits, per_split;
 };
 static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
-  const int pairs = sm_count() / 2, parts = parts_of(kind, dtype);
+  const int pairs = sm_count() / 2, parts = dtype == LNCC_F32 ? 6 : 1;
   Cut best = {};
   double least = 0;
   for (int bn = 256; bn >= 128; bn -= 128) {
@@ -932,9 +1124,8 @@ static Cut cut_for(int kind, int dtype, int64_t rows, int64_t cols, int whichs, 
 
 // Scratch of a call, laid out in one place for its size and its use.
 struct Plan {
-  int planes, hidden_planes;  // of operands as they are given, and of the hidden matrices and what they are multiplied with
-  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, dh, norms, partial, total;
-  size_t x2, wg2, wu2, wd2, dy2;  // fp16: as two planes
+  int planes;
+  size_t x, wg, wu, wd, dy, h, dg, du, gate, up, dh, norms, levels, row_h, row_d, most, scaled_x, scaled_dy, partial, total;
   int64_t ldf;
 };
 static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int whichs, int64_t blocks) {
@@ -942,6 +1133,7 @@ static size_t partial_bytes(int kind, int dtype, int64_t rows, int64_t cols, int
   return c.splits > 1 ? size_t(c.splits) * whichs * rows * ((cols + 3) / 4 * 4) * 4 : 0;
 }
 static int64_t k_steps(int64_t k) { return ceil_div(k, 64); }
+static int level_blocks() { return 8 * sm_count(); }
 static bool few(const Args& a);
 static Plan plan_for(const Args& a, bool backward) {
   Plan p = {};
@@ -950,33 +1142,34 @@ static Plan plan_for(const Args& a, bool backward) {
     return p;
   }
   p.planes = a.dtype == LNCC_F32 ? 3 : 1;
-  p.hidden_planes = a.dtype == LNCC_F32 ? 3 : a.dtype == LNCC_F16 ? 2 : 1;
   p.ldf = lead(a.F);
   size_t at = kHeader;
-  const auto planes = [&](int n, int64_t rows, int64_t ld) {
+  const auto take = [&](int64_t rows, int64_t ld) {
     const size_t here = at;
-    at += round_up(size_t(n) * rows * ld * 2);
+    at += round_up(size_t(p.planes) * rows * ld * 2);
     return here;
   };
-  const auto take = [&](int64_t rows, int64_t ld) { return planes(p.planes, rows, ld); };
   p.x = take(a.M, lead(a.K));
   p.wg = take(a.F, lead(a.K));
   p.wu = take(a.F, lead(a.K));
   p.wd = take(a.N, p.ldf);
-  p.h = planes(p.hidden_planes, a.M, p.ldf);
-  if (a.dtype == LNCC_F16 && !backward) p.wd2 = planes(2, a.N, p.ldf);
-  if (a.dtype == LNCC_F16 && backward) {
-    p.x2 = planes(2, a.M, lead(a.K));
-    p.dy2 = planes(2, a.M, lead(a.N));
-    p.wg2 = planes(2, a.F, lead(a.K));
-    p.wu2 = planes(2, a.F, lead(a.K));
+  p.h = take(a.M, p.ldf);
+  if (a.dtype == LNCC_F16) {
+    p.levels = at, at += round_up(size_t(a.M) * ceil_div(a.F, 16) * (backward ? 4 : 2));
+    p.row_h = at, at += round_up(size_t(a.M) * 4);
+    if (backward) {
+      p.row_d = at, at += round_up(size_t(a.M) * 4);
+      p.most = at, at += round_up(size_t(MOSTS) * level_blocks() * 4);
+      p.scaled_x = take(a.M, lead(a.K));
+      p.scaled_dy = take(a.M, lead(a.N));
+    }
   }
   size_t most = 0;
   const auto partial = [&](size_t n) { most = n > most ? n : most; };
   if (backward) {
     p.dy = take(a.M, lead(a.N));
-    p.dg = planes(p.hidden_planes, a.M, p.ldf);
-    p.du = planes(p.hidden_planes, a.M, p.ldf);
+    p.dg = take(a.M, p.ldf);
+    p.du = take(a.M, p.ldf);
     if (a.dtype == LNCC_F32) {
       p.gate = at, at += round_up(size_t(a.M) * p.ldf * 4);
       p.up = at, at += round_up(size_t(a.M) * p.ldf * 4);
@@ -1006,7 +1199,7 @@ struct Call {
   int status;
   bool first = true;      // the next product kernel is the call's first
   bool launched = false;  // a kernel of this call is in the stream
-  Packs packs = {}, halves = {};  // matrices to lay out, and fp16 ones as two planes
+  Packs packs = {};
 
   // every kernel of a call but its first may be launched while the one before it ends (begin_after_previous)
   template <typename K, typename... A> void run(K kernel, dim3 grid, int threads, int smem, const A&... args) {
@@ -1027,37 +1220,47 @@ struct Call {
       if (rows == 1) m.ld = lead(cols);
       return m;
     }
-    lay_out(packs, m, src, stride, to, plan.planes);
-    return m;
-  }
-  // src, which `given` describes, as an operand of a product with a hidden matrix
-  Matrix beside_hidden(const Matrix& given, const void* src, int64_t stride, size_t to) {
-    if (a.dtype != LNCC_F16) return given;
-    Matrix m = given;
-    m.bf16 = true;
-    lay_out(halves, m, src, stride, to, 2);
-    return m;
-  }
-  void lay_out(Packs& in, Matrix& m, const void* src, int64_t stride, size_t to, int planes) {
     m.p = scratch + to;
-    m.ld = lead(m.cols);
-    m.plane = m.rows * m.ld;
-    m.planes = planes;
-    const int64_t blocks = ceil_div(m.rows * (m.ld / 8), 256), most = int64_t(sm_count()) * 8;
-    in.job[in.jobs++] = {src, m.p, stride, m.rows, m.cols, m.ld, m.plane, in.blocks};
-    in.blocks += int(blocks < most ? blocks : most);
+    m.ld = lead(cols);
+    m.plane = rows * m.ld;
+    m.planes = plan.planes;
+    const int64_t blocks = ceil_div(rows * (m.ld / 8), 256), most = int64_t(sm_count()) * 8;
+    packs.job[packs.jobs++] = {src, m.p, stride, rows, cols, m.ld, m.plane, packs.blocks};
+    packs.blocks += int(blocks < most ? blocks : most);
+    return m;
   }
   void pack() {
-    if (packs.jobs) {
-      const dim3 grid = dim3(unsigned(packs.blocks));
-      if (a.dtype == LNCC_F32) run(pack_kernel<float, __nv_bfloat16>, grid, 256, 0, packs);
-      else if (a.dtype == LNCC_BF16) run(pack_kernel<__nv_bfloat16, __nv_bfloat16>, grid, 256, 0, packs);
-      else run(pack_kernel<__half, __half>, grid, 256, 0, packs);
-    }
-    if (halves.jobs) run(pack_kernel<__half, __nv_bfloat16>, dim3(unsigned(halves.blocks)), 256, 0, halves);
+    if (packs.jobs == 0) return;
+    const dim3 grid = dim3(unsigned(packs.blocks));
+    if (a.dtype == LNCC_F32) run(pack_kernel<float, __nv_bfloat16>, grid, 256, 0, packs);
+    else if (a.dtype == LNCC_BF16) run(pack_kernel<__nv_bfloat16, __nv_bfloat16>, grid, 256, 0, packs);
+    else run(pack_kernel<__half, __half>, grid, 256, 0, packs);
   }
+  // fp16: after the hidden matrices, their rows' levels; the copies of x and dy that the sums over tokens take
+  void level() {
+    int lanes = 4;
+    while (lanes < 32 && lanes * 64 < a.F) lanes *= 2;  // four pairs of pieces a lane, or more
+    const LevelArgs r = {halves(plan.h), halves(plan.dg), halves(plan.du), static_cast<const __half*>(a.x), static_cast<const __half*>(a.dy),
+                         a.x_stride, a.dy_stride, a.M, a.K, a.F, a.N, plan.ldf, lanes,
+                         reinterpret_cast<const int8_t*>(scratch + plan.levels), ints(plan.row_h), ints(plan.row_d), ints(plan.most)};
+    run(a.dy ? level_kernel<true> : level_kernel<false>, dim3(unsigned(level_blocks())), 256, 0, r);
+  }
+  void rescale(Matrix& x, Matrix& dy) {
+    const bool want_x = a.dwg || a.dwu, want_dy = a.dwd != nullptr;
+    if (!want_x && !want_dy) return;
+    x = {scratch + plan.scaled_x, a.M, a.K, lead(a.K), 0, 1, false};
+    dy = {scratch + plan.scaled_dy, a.M, a.N, lead(a.N), 0, 1, false};
+    const Rescale r = {want_x ? static_cast<const __half*>(a.x) : nullptr, want_dy ? static_cast<const __half*>(a.dy) : nullptr,
+                       a.x_stride, a.dy_stride, a.M, a.K, a.N, x.ld, dy.ld, halves(plan.scaled_x), halves(plan.scaled_dy),
+                       ints(plan.row_h), ints(plan.row_d), ints(plan.most), level_blocks()};
+    const int64_t blocks = ceil_div(a.M * (x.ld > dy.ld ? x.ld : dy.ld) / 8, 256), most = int64_t(sm_count()) * 8;
+    run(rescale_kernel, dim3(unsigned(blocks < most ? blocks : most)), 256, 0, r);
+  }
+  int* ints(size_t at) const { return reinterpret_cast<int*>(scratch + at); }
+  __half* halves(size_t at) const { return reinterpret_cast<__half*>(scratch + at); }
+
   Matrix hidden(size_t at) const {
-    return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.hidden_planes, true};
+    return {scratch + at, a.M, a.F, plan.ldf, a.M * plan.ldf, plan.planes, a.dtype != LNCC_F16};
   }
 
   template <int KIND, int BN, int ACT, typename T> void launch(Gemm& g) {
@@ -1127,6 +1330,10 @@ struct Call {
     for (int al = 16; al <= 32; al *= 2)
       if (aligned(out0, al) && aligned(out1, al) && aligned(out2, al) && ld * es % al == 0) g.align = al;
     g.partial = reinterpret_cast<float*>(scratch + plan.partial);
+    if (a.dtype == LNCC_F16) {
+      g.levels = reinterpret_cast<int8_t*>(scratch + plan.levels);
+      g.row_h = ints(plan.row_h), g.row_d = ints(plan.row_d), g.most = ints(plan.most), g.level_blocks = level_blocks();
+    }
     g.abort_word = reinterpret_cast<unsigned*>(scratch);
     g.clear_abort = first;
     first = false;
@@ -1203,10 +1410,11 @@ static int forward(const Args& a, const Plan& plan, void* scratch, cudaStream_t 
   Call c = {a, plan, static_cast<char*>(scratch), stream, LNCC_OK};
   const Matrix x = c.operand(a.x, a.M, a.K, a.x_stride, c.plan.x), wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg),
                wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu), wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd),
-               h = c.hidden(c.plan.h), wd2 = c.beside_hidden(wd, a.wd, a.F, c.plan.wd2);
+               h = c.hidden(c.plan.h);
   c.pack();
   c.product<UP>(x, x, wg, wu, wg, a.M, a.F, 1, a.K, 0, h.p, nullptr, nullptr, h.ld, h.plane);
-  c.product<DOWN>(h, h, wd2, wd2, wd2, a.M, a.N, 1, a.F, 0, a.y, nullptr, nullptr, a.N, 0);
+  if (a.dtype == LNCC_F16) c.level();
+  c.product<DOWN>(h, h, wd, wd, wd, a.M, a.N, 1, a.F, 0, a.y, nullptr, nullptr, a.N, 0);
   return c.status;
 }
 
@@ -1216,10 +1424,6 @@ static int backward(const Args& a, const Plan& plan, void* scratch, cudaStream_t
                wg = c.operand(a.wg, a.F, a.K, a.K, c.plan.wg), wu = c.operand(a.wu, a.F, a.K, a.K, c.plan.wu),
                wd = c.operand(a.wd, a.N, a.F, a.F, c.plan.wd);
   const Matrix h = c.hidden(c.plan.h), dg = c.hidden(c.plan.dg), du = c.hidden(c.plan.du);
-  Matrix x2 = x, dy2 = dy, wg2 = wg, wu2 = wu;
-  if (a.dwg || a.dwu) x2 = c.beside_hidden(x, a.x, a.x_stride, c.plan.x2);
-  if (a.dwd) dy2 = c.beside_hidden(dy, a.dy, a.dy_stride, c.plan.dy2);
-  if (a.dx) wg2 = c.beside_hidden(wg, a.wg, a.K, c.plan.wg2), wu2 = c.beside_hidden(wu, a.wu, a.K, c.plan.wu2);
   c.pack();
   if (a.dtype == LNCC_F32) {
     float *const gate = reinterpret_cast<float*>(c.scratch + c.plan.gate), *const up = reinterpret_cast<float*>(c.scratch + c.plan.up),
@@ -1239,13 +1443,18 @@ static int backward(const Args& a, const Plan& plan, void* scratch, cudaStream_t
   } else {
     c.product<HIDDEN>(x, dy, wg, wu, wd, a.M, a.F, 1, a.K, a.N, dg.p, du.p, h.p, h.ld, h.plane);
   }
-  if (a.dx) c.product<DX>(dg, du, wg2, wu2, wg2, a.M, a.K, 1, a.F, 0, a.dx, nullptr, nullptr, a.K, 0);
+  Matrix sum_x = x, sum_dy = dy;  // as the sums over tokens take them
+  if (a.dtype == LNCC_F16) {
+    c.level();
+    c.rescale(sum_x, sum_dy);
+  }
+  if (a.dx) c.product<DX>(dg, du, wg, wu, wg, a.M, a.K, 1, a.F, 0, a.dx, nullptr, nullptr, a.K, 0);
   if (a.dwg || a.dwu) {
     // one product for both where both are wanted
     const Matrix& first = a.dwg ? dg : du;
-    c.product<DW_UP>(first, du, x2, x2, x2, a.F, a.K, a.dwg && a.dwu ? 2 : 1, a.M, 0, a.dwg ? a.dwg : a.dwu, a.dwu, nullptr, a.K, 0);
+    c.product<DW_UP>(first, du, sum_x, sum_x, sum_x, a.F, a.K, a.dwg && a.dwu ? 2 : 1, a.M, 0, a.dwg ? a.dwg : a.dwu, a.dwu, nullptr, a.K, 0);
   }
-  if (a.dwd) c.product<DW_DOWN>(dy2, dy2, h, h, h, a.N, a.F, 1, a.M, 0, a.dwd, nullptr, nullptr, a.F, 0);
+  if (a.dwd) c.product<DW_DOWN>(sum_dy, sum_dy, h, h, h, a.N, a.F, 1, a.M, 0, a.dwd, nullptr, nullptr, a.F, 0);
   return c.status;
 }
 

@@ -5,9 +5,9 @@
     g = x w_gate^T,  u = x w_up^T,  h = act(g) u,  y = h w_down^T
 
 x: (..., K); w_gate, w_up: (F, K); w_down: (N, F), as torch.nn.Linear lays its weights out; all of one type, float32,
-bfloat16 or float16. Sums are fp32; beyond four tokens the hidden values are rounded to bfloat16 between the products where the type
-is bfloat16, and held to 16 bits in float32's range where it is float16. Nothing of the hidden layer is saved for the backward
-pass: it forms g, u and h again.
+bfloat16 or float16. Sums are fp32; for 16-bit types and more than four tokens the hidden values are rounded to the type's bits between
+the products, in float16 too without its range: hidden values past 65504 and gradients below 2^-24 are held. Nothing of the
+hidden layer is saved for the backward pass: it forms g, u and h again.
 """
 import torch
 from torch.overrides import has_torch_function

@@ -353,8 +353,9 @@ enum lncc_activation { LNCC_ACT_SILU = 0, LNCC_ACT_GELU = 1, LNCC_ACT_RELU = 2 }
  * Limits: K, F, N <= 2^20, M <= 2^30 - 1 (LNCC_ERR_TOO_LARGE).
  * The scratch starts with a word that lncc_check_abort reads, as the loss's workspace does: a bounded wait of the products
  * (2 s each) that ran out gives LNCC_ERR_ABORTED there and NaN results. Between the products h (and dg, du in the backward
- * pass) are rounded to bf16 for LNCC_BF16, and held to 16 bits in fp32's range for LNCC_F16; for up to four tokens h stays fp32.
- * An infinity in an operand of LNCC_F32 or LNCC_F16 may give NaN where the formula gives an infinity.
+ * pass) are rounded to bf16 for LNCC_BF16, and to 11 bits for LNCC_F16, not to fp16's range: what is below 2^-21 of a token's
+ * largest hidden value is right to 2^-32 of that. For up to four tokens h stays fp32. An infinity in an operand of LNCC_F32 may
+ * give NaN where the formula gives an infinity.
  */
 size_t lncc_gated_ffn_scratch_bytes(int64_t M, int64_t K, int64_t F, int64_t N, int dtype, int backward);
 int lncc_gated_ffn_forward(const void* x, int64_t x_stride, const void* w_gate, const void* w_up, const void* w_down,
