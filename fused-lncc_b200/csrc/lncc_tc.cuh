@@ -38,8 +38,11 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Arrive on a barrier given by its cluster address, to say that tensor memory has been read (the loads are complete and
-// fenced). Relaxed: a release would also wait for the thread's stores to global memory, a thousand clocks a tile.
+// Arrive on a barrier given by its cluster address, to say that a warp has read its part of tensor memory. What is ordered by it
+// are reads before the products that write there next, no data that the other side would read: every lane's loads have
+// ended at its wait_ld (their values are in registers), fence_before and __syncwarp put that before lane 0's arrival, and the
+// thread that issues the products comes after it by its wait and fence_after. So it may be relaxed: a release would also wait
+// for the thread's stores to global memory, a thousand clocks a tile.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
