@@ -202,7 +202,7 @@ __device__ __forceinline__ void emit_parts(void* base, const Gemm& g, int64_t ro
 // value and more keeps fp16's 11 bits at least; the rest is right to 2^-32 of it.
 // The product that reads a row takes its power back out in the epilogue (DOWN, DX). The weights' gradients sum over rows of
 // different powers: there the other operand, x or dy, is copied with the row's power taken out of it, relative to the largest
-// of the call. dg and du share a power, since dx adds their products up. Measured beside bf16: 4096 x 768 x 2048 forward 54 us
+// of the call. dg and du share a power, since dx adds their products up. Measured beside bf16: 4096 x 768 x 2048 forward 52 us
 // (43), 107520 x 96 x 256 training 275 (197), 16384 x 1024 x 4096 training 1384 (1315); level_kernel's backward part 19, 33 and
 // 62 us of them, 101 where every row has pieces to rewrite. As two bf16 numbers each, 16 bits in fp32's range, h, dg and du took
 // three products for one: 69, 349 and 2575 us.
@@ -451,6 +451,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
 
       if constexpr (PROMOTED) {
         constexpr int SUMS = gated(KIND) ? 2 * COLS : COLS;  // gated: columns of g, then of u
+        int row_level = 0;  // on its way while the products run
+        if (LEVELS && !AM && row0 + lane < g.rows) row_level = (KIND == DOWN ? g.row_h : g.row_d)[row0 + lane];
         float sum[SUMS];
 #pragma unroll
         for (int i = 0; i < SUMS; i++) sum[i] = 0.f;
@@ -488,8 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) product
           }
         } else if constexpr (!F32) {
           if (LEVELS) {
-            float power = power_all;
-            if (!AM && row0 + lane < g.rows) power = power_of_2(kStep * (KIND == DOWN ? g.row_h : g.row_d)[row0 + lane] - 11);
+            const float power = AM ? power_all : power_of_2(kStep * row_level - 11);
 #pragma unroll
             for (int c = 0; c < SUMS; c++) sum[c] *= power;
           }
