@@ -15,7 +15,9 @@
 // saving h would, and h_{t-1} is not rounded to 16 bits.
 // Measured: 2 x 32768 x 256 fp16 16 + 21 us (its bytes once: 15), 107520 x 96 bf16 11 + 16 forward and 13 + 29 backward (10, 17),
 // 6 x 4093 x 389 fp32 19 + 26 and 23 + 44 (18, 29). One kernel that reads everything once, tiles waiting for earlier tiles' sums,
-// took 47 us for the first: at four blocks an SM too few bytes are in flight while tiles wait.
+// took 47 us for the first: at four blocks an SM too few bytes are in flight while tiles wait. Registers are at the caps that the
+// launch bounds set (64, and 128 backward), and 16 steps' loads do not quite fit beside the arithmetic: most first passes and runs
+// spill up to 40 bytes a thread, back_run 32 to 104; it also forms each gate twice, once for h and once for the gradients.
 #include "lncc_block.cuh"
 
 #include <type_traits>

@@ -104,3 +104,23 @@ def test_profiler_sees_the_operators():
     with profile(activities=[ProfilerActivity.CPU]) as p:
         ln(*args)
     assert any(e.key == "fused_lncc::layer_norm" for e in p.key_averages())
+
+
+@pytest.mark.parametrize("name", list(CALLS))
+def test_under_a_function_mode(name):
+    """torch.device as a context is one; gradients come through it as without."""
+    f, make = CALLS[name]
+    args = [a.requires_grad_(True) for a in make()]
+    want = _outs(f(*args))
+    want_grads = torch.autograd.grad([o.sum() for o in want], args)
+    with torch.device("cuda"):
+        got = _outs(f(*args))
+        grads = torch.autograd.grad([o.sum() for o in got], args)
+    for a, b in zip((*got, *grads), (*want, *want_grads)):
+        assert torch.equal(a, b)
+
+
+def test_torch_func_grad_is_refused():
+    x = CALLS["norm"][1]()[0]
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda t: ln(t).sum())(x)
