@@ -24,15 +24,17 @@
 // training step, and saves writing and reading 4 M F bytes and a rounding of g and u.
 //
 // Roundings. For 16-bit types h, dg and du are rounded to the type's bits, since they are operands of the next product (for fp16
-// times a power of 2 a row, see below: its range would not hold them); g, u and dh never leave fp32. The result then holds two roundings of like size, its own and h's, and is sqrt 2 as far off as one that
-// keeps h in fp32 (fp16, more than four tokens: 2.9e-4 of the result against 2.1e-4; bf16 2.4e-3 against 1.7e-3); in calls of
-// a few hundred values the factor scatters, at 5 x 48 x 79 between 1.25 and 1.63 in nine draws of ten. fp32 operands are taken apart into three bf16 numbers of 8 bits each, which hold all 24 bits, and six of
-// the nine products are summed, smallest first (the other three are below 2^-24 of the result). The tensor cores cut, not
-// round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of an fp32 result. So for fp32 an
-// accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each time. The 16-bit
-// products with long inner axes do so every 2048: sums over 131072 tokens that do not cancel came out 8.5e-4 too small
-// in one accumulator, more than fp16's own rounding, and 2.4e-5 now, at the same speed. (g, u and dh, whose inner axes are the
-// block's widths, take one accumulator for 16-bit types: 8e-6 at 1024.) An infinity taken apart meets zeros: it gives NaN where fp32 would give an infinity.
+// times a power of 2 a row, see below: its range would not hold them); g, u and dh never leave fp32. The result then holds two
+// roundings of like size, its own and h's, and is sqrt 2 as far off as one that keeps h in fp32 (more than four tokens, fp16:
+// 2.9e-4 of the result against 2.1e-4, bf16 2.4e-3 against 1.7e-3); in calls of a few hundred values the factor scatters, at 5 x
+// 48 x 79 between 1.25 and 1.63 in nine draws of ten. fp32 operands are taken apart into three bf16 numbers of 8 bits each,
+// which hold all 24 bits, and six of the nine products are summed, smallest first (the other three are below 2^-24 of the
+// result). An infinity taken apart meets zeros: it gives NaN where fp32 would give an infinity.
+// The tensor cores cut, not round, what they add to an accumulator: over an inner axis of 4096 that came to 1e-5 of an fp32
+// result. So for fp32 an accumulator takes 256 of the inner axis, and the epilogue adds these sums in registers, rounding each
+// time. The 16-bit products with long inner axes do so every 2048: sums over 131072 tokens that do not cancel came out 8.5e-4 too
+// small in one accumulator, more than fp16's own rounding, and 2.4e-5 now, at the same speed. (g, u and dh, whose inner axes are
+// the block's widths, take one accumulator for 16-bit types: 8e-6 at 1024.)
 #include "lncc_tc.cuh"
 
 #include <type_traits>
